@@ -12,6 +12,11 @@ Public API:
     is_available() -> bool          # gfx950 ROCm device + loadable kernel library
     pick_groupsize(in_features) -> int | None
 
+Beside the reference's API, the microscaled 4-bit tier (``mxfp4``:
+quantize_mxfp4, dequantize_mxfp4, mxfp4_linear, mxfp4_expert_linear) and expert
+routing (``experts``: sort_tokens_by_expert, gather_expert_rows,
+combine_expert_rows).
+
 Numerics are those of the reference eager path (``_int4/eager.py``): packed
 codes and scales equal the eager ones, the integer accumulators are exact, and
 the epilogue is the fp32 chain fl32(fl32(fl32(acc*xs)*ws)+b) rounded once to
@@ -26,6 +31,8 @@ import torch
 from . import native
 from ._codec import _INT4_GROUP_SIZE, _INT4_MAX, _pack_int4_row_major, _unpack_int4_row_major
 from .native import is_available as _native_available
+from .experts import ExpertPlan, combine_expert_rows, gather_expert_rows, max_experts, sort_tokens_by_expert
+from .mxfp4 import dequantize_mxfp4, mxfp4_expert_linear, mxfp4_linear, quantize_mxfp4
 
 __all__ = [
     "quantize_convrot_w4a4_weight",
@@ -41,6 +48,15 @@ __all__ = [
     "i8t_path_ok",
     "prepare_convrot_w8a8_weight_i8t",
     "max_quant_k",
+    "quantize_mxfp4",
+    "dequantize_mxfp4",
+    "mxfp4_linear",
+    "mxfp4_expert_linear",
+    "ExpertPlan",
+    "max_experts",
+    "sort_tokens_by_expert",
+    "gather_expert_rows",
+    "combine_expert_rows",
 ]
 
 # largest concatenated rank of the fused LoRA side path (padded to a multiple of 32)

@@ -12,6 +12,7 @@ back to anything else.
 from __future__ import annotations
 
 import collections
+import contextlib
 import ctypes
 import importlib.machinery
 import importlib.util
@@ -81,6 +82,18 @@ _SIGNATURES = {
                                       + [_vp, ctypes.c_size_t, _vp], _i),
     "cr_convrot_w4a4_linear_packed_workspace": ([_i, _i, _i, _i], ctypes.c_size_t),
     "cr_convrot_dequant": ([_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp], _i),
+    "cr_mxfp4_quant": ([_vp, _i, _vp, _vp, _i, _i, _i, _vp], _i),
+    "cr_mxfp4_dequant": ([_vp, _vp, _vp, _i, _i, _i, _i, _vp], _i),
+    "cr_mxfp4_linear_workspace": ([_i, _i], ctypes.c_size_t),
+    "cr_mxfp4_linear": ([_vp, _i, _vp, _vp, _vp, _i, _vp] + [_i] * 4 + [_vp, ctypes.c_size_t, _vp], _i),
+    "cr_mxfp4_expert_linear": ([_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp] + [_i] * 4
+                               + [_vp, ctypes.c_size_t, _vp], _i),
+    "cr_max_experts": ([], _i),
+    "cr_expert_sort_workspace": ([_i, _i], ctypes.c_size_t),
+    "cr_expert_sort": ([_vp, _i, _vp, _vp, _vp, _i, _i, _vp, ctypes.c_size_t, _vp], _i),
+    "cr_expert_gather": ([_vp, _i, _vp, _vp, _vp] + [_i] * 4 + [_vp], _i),
+    "cr_expert_combine": ([_vp, _i, _vp, _vp, _vp] + [_i] * 3 + [_vp], _i),
+    "cr_expert_combine_grad": ([_vp, _i] + [_vp] * 6 + [_i] * 4 + [_vp], _i),
     "cr_max_quant_k": ([], _i),
     "cr_abi_version": ([], _i),
 }
@@ -204,6 +217,16 @@ def _stream(device) -> int:
     if _raw_stream is not None:
         return _raw_stream(index)
     return torch.cuda.current_stream(index).cuda_stream
+
+
+_same = contextlib.nullcontext()
+
+
+def on_device(device):
+    """Context in which ``device`` is the current one: a launch goes to a stream of
+    the current device."""
+    index = device.index
+    return _same if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
 
 
 # One reusable workspace per (device, stream): calls on a stream run in stream

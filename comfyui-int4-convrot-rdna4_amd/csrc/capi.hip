@@ -3,6 +3,7 @@
 
 #include "../../include/convrot_mi355x.h"
 #include "gemm_common.h"
+#include "mxfp4_gemm.h"
 
 namespace convrot {
 hipError_t rotquant_launch(const void* x, int in_dtype, const void* noise, int8_t* q, float* s,
@@ -46,6 +47,21 @@ hipError_t dequant_launch(const void* q, int bits, const float* s, void* out, in
                           hipStream_t st);
 hipError_t gemm_splitk_launch(const int8_t* Xp, const int8_t* Wp, const float* xs, const float* ws, float* accum,
                               int M, int N, int K, int nsplit, hipStream_t st);
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st);
+hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
+                                hipStream_t st);
+hipError_t mxfp4_gemm_launch(const MxProblem& p, hipStream_t st);
+int expert_max();
+size_t expert_sort_bytes(int R, int E);
+hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R,
+                              int E, hipStream_t st);
+hipError_t expert_gather_launch(const void* x, int dt, const int* position, const int* offsets, void* rows, int T, int k,
+                                int E, int D, hipStream_t st);
+hipError_t expert_combine_launch(const void* rows, int dt, const float* w, const int* position, void* out, int T, int k,
+                                 int D, hipStream_t st);
+hipError_t expert_combine_grad_launch(const void* rows, int dt, const float* w, const int* position, const int* offsets,
+                                      const void* d_out, void* d_rows, float* d_w, int T, int k, int E, int D,
+                                      hipStream_t st);
 }  // namespace convrot
 
 #define API extern "C" __attribute__((visibility("default")))
@@ -519,6 +535,130 @@ API int cr_convrot_dequant(const void* q, int bits, const void* scale, void* out
     if (N < 0 || K <= 0 || K % G != 0 || (long long)N * (K / 16) >= (1ll << 31)) return -1;
     return (int)convrot::dequant_launch(q, bits, reinterpret_cast<const float*>(scale), out, out_dtype, N, K, G,
                                         reinterpret_cast<hipStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------
+// Microscaled 4-bit floats and expert routing
+// ---------------------------------------------------------------------------
+
+static int mx_args_ok(int dtype, int M, int K, int G) {
+    if (!(G == 0 || G == 16 || G == 64 || G == 256)) return 0;
+    if (M < 0 || K <= 0 || K > (1 << 24) || K % convrot::MX_BLOCK != 0 || (G != 0 && K % G != 0)) return 0;
+    return dtype >= 0 && dtype <= 2;
+}
+
+API int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream) {
+    if (!mx_args_ok(in_dtype, M, K, G)) return -1;
+    return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, K, G, reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
+                         void* stream) {
+    if (!mx_args_ok(out_dtype, M, K, G)) return -1;
+    return (int)convrot::mxfp4_dequant_launch(codes, scales, out, out_dtype, M, K, G, reinterpret_cast<hipStream_t>(stream));
+}
+
+// Codes and scales of x, rows padded to a multiple of 128 values, after the counter region.
+struct MxPlan { size_t codes, scales, total; int Kp; };
+static MxPlan mx_plan(int M, int K) {
+    MxPlan p;
+    p.Kp = (K + 127) / 128 * 128;
+    p.codes = kSplitCounterBytes;
+    p.scales = p.codes + (size_t)M * (p.Kp / 2);                      // 64 bytes or more a row: stays 16-byte aligned
+    p.total = p.scales + ((size_t)M * (p.Kp / 32) + 15) / 16 * 16;
+    return p;
+}
+
+// x [rows, K] quantized into the workspace, then the product; `p` but for the activation's operand
+static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, void* workspace, size_t workspace_bytes,
+                         hipStream_t st) {
+    const MxPlan plan = mx_plan(rows, p.K);
+    if (workspace == nullptr || workspace_bytes < plan.total) return -1;
+    uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
+    p.a = ws + plan.codes;
+    p.as = ws + plan.scales;
+    p.Kp = plan.Kp;
+    const hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, G, st);
+    if (e != hipSuccess) return (int)e;
+    return (int)convrot::mxfp4_gemm_launch(p, st);
+}
+
+API size_t cr_mxfp4_linear_workspace(int M, int K) {
+    return M <= 0 || K <= 0 || K % convrot::MX_BLOCK != 0 ? 0 : mx_plan(M, K).total;
+}
+
+API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,
+                        void* out, int M, int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mx_args_ok(dtype, M, K, G) || N < 0 || bias_dtype < 0 || bias_dtype > 2) return -1;
+    if (M == 0 || N == 0) return 0;
+    convrot::MxProblem p{};
+    p.w = reinterpret_cast<const uint8_t*>(W);
+    p.ws = reinterpret_cast<const uint8_t*>(wscales);
+    p.bias = bias;
+    p.out = out;
+    p.R = M; p.N = N; p.K = K; p.E = 1; p.top_k = 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    return mx_linear_run(x, M, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k, const int* offsets, int E,
+                               const void* W, const void* wscales, const void* bias, int bias_dtype, void* out, int R,
+                               int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!mx_args_ok(dtype, R, K, G) || N < 0 || bias_dtype < 0 || bias_dtype > 2) return -1;
+    if (E < 1 || E > convrot::expert_max() || offsets == nullptr) return -1;
+    if (order != nullptr && (top_k < 1 || R % top_k != 0)) return -1;
+    if (R == 0 || N == 0) return 0;
+    convrot::MxProblem p{};
+    p.w = reinterpret_cast<const uint8_t*>(W);
+    p.ws = reinterpret_cast<const uint8_t*>(wscales);
+    p.bias = bias;
+    p.out = out;
+    p.offsets = offsets;
+    p.order = order;
+    p.R = R; p.N = N; p.K = K; p.E = E; p.top_k = order != nullptr ? top_k : 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    return mx_linear_run(x, R / p.top_k, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_max_experts(void) { return convrot::expert_max(); }
+
+static int expert_rows_ok(int dtype, int T, int k, int E, int D) {
+    return dtype >= 0 && dtype <= 2 && T >= 0 && k >= 1 && E >= 1 && D >= 1 && (long long)T * k < (1ll << 31);
+}
+
+API size_t cr_expert_sort_workspace(int R, int E) {
+    return R < 0 || E < 1 || E > convrot::expert_max() ? 0 : kSplitCounterBytes + convrot::expert_sort_bytes(R, E);
+}
+
+API int cr_expert_sort(const void* ids, int id_bytes, int* order, int* position, int* offsets, int R, int E,
+                       void* workspace, size_t workspace_bytes, void* stream) {
+    if ((id_bytes != 4 && id_bytes != 8) || R < 0 || E < 1 || E > convrot::expert_max()) return -1;
+    if (workspace == nullptr || workspace_bytes < cr_expert_sort_workspace(R, E)) return -1;
+    int* counts = reinterpret_cast<int*>(reinterpret_cast<uint8_t*>(workspace) + kSplitCounterBytes);
+    return (int)convrot::expert_sort_launch(ids, id_bytes, order, position, offsets, counts, R, E,
+                                            reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_expert_gather(const void* x, int dtype, const int* position, const int* offsets, void* rows, int T, int k, int E,
+                         int D, void* stream) {
+    if (!expert_rows_ok(dtype, T, k, E, D)) return -1;
+    if (T == 0) return 0;
+    return (int)convrot::expert_gather_launch(x, dtype, position, offsets, rows, T, k, E, D,
+                                              reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_expert_combine(const void* rows, int dtype, const float* weights, const int* position, void* out, int T, int k,
+                          int D, void* stream) {
+    if (!expert_rows_ok(dtype, T, k, 1, D)) return -1;
+    if (T == 0) return 0;
+    return (int)convrot::expert_combine_launch(rows, dtype, weights, position, out, T, k, D,
+                                               reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_expert_combine_grad(const void* rows, int dtype, const float* weights, const int* position, const int* offsets,
+                               const void* d_out, void* d_rows, float* d_weights, int T, int k, int E, int D, void* stream) {
+    if (!expert_rows_ok(dtype, T, k, E, D) || weights == nullptr) return -1;
+    if (T == 0) return 0;
+    return (int)convrot::expert_combine_grad_launch(rows, dtype, weights, position, offsets, d_out, d_rows, d_weights, T, k, E,
+                                                    D, reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_max_quant_k(void) { return convrot::rotquant_max_k(); }

@@ -1,0 +1,320 @@
+// Tokens sorted by expert and back.
+//
+// A token t has k slots; slot t k + j goes to expert ids[t, j], or to none where
+// that id is outside [0, E).  The plan is a stable counting sort of the slots:
+//   order[r]      the slot of sorted row r; -1 past the last used row
+//   position[s]   the sorted row of slot s; -1 for an unused one
+//   offsets[e]    expert e's rows are offsets[e] .. offsets[e + 1] - 1
+// Rows follow it: gathered[r] = x[order[r] / k], combined[t] = sum_j w[t, j]
+// rows[position[t, j]], and their gradients.  Every sum is taken over a token's
+// slots in slot order in fp32: nothing is added atomically, the same inputs give
+// the same bits.
+
+#include "mxfp4.h"
+
+namespace convrot {
+
+constexpr int SORT_THREADS = 256, SORT_WAVES = 4;
+constexpr int SORT_SLOTS = 4096;           // slots per workgroup
+constexpr int SORT_MAX_E = 1024;
+
+template <typename ID>
+__device__ __forceinline__ int expert_of(const ID* ids, int s, int R, int E) {
+    if (s >= R) return -1;
+    const ID id = ids[s];
+    return id >= 0 && id < (ID)E ? (int)id : -1;
+}
+
+// counts[b, e]: slots of workgroup b's run that go to expert e
+template <typename ID>
+__global__ __launch_bounds__(SORT_THREADS) void expert_count_kernel(const ID* __restrict__ ids, int* __restrict__ counts,
+                                                                    int R, int E) {
+    __shared__ int n[SORT_MAX_E];
+    for (int e = threadIdx.x; e < E; e += SORT_THREADS) n[e] = 0;
+    __syncthreads();
+    const int s0 = blockIdx.x * SORT_SLOTS;
+    for (int i = threadIdx.x; i < SORT_SLOTS && s0 + i < R; i += SORT_THREADS) {
+        const int e = expert_of(ids, s0 + i, R, E);
+        if (e >= 0) atomicAdd(&n[e], 1);                   // integers: the order does not matter
+    }
+    __syncthreads();
+    for (int e = threadIdx.x; e < E; e += SORT_THREADS) counts[(size_t)blockIdx.x * E + e] = n[e];
+}
+
+// Workgroup b places its run: expert e's first row there is offsets[e] plus the
+// counts of the runs before.  Each wave takes a quarter of the run in order; the
+// lanes that go to one expert find each other by the bits of its number.
+template <typename ID>
+__global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __restrict__ ids,
+                                                                    const int* __restrict__ counts, int* __restrict__ order,
+                                                                    int* __restrict__ position, int* __restrict__ offsets,
+                                                                    int R, int E, int runs) {
+    __shared__ int total[SORT_MAX_E], next[SORT_WAVES][SORT_MAX_E];
+    __shared__ int wave_sum[SORT_WAVES], used;
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int s0 = blockIdx.x * SORT_SLOTS;
+    constexpr int SPAN = SORT_SLOTS / SORT_WAVES;
+    for (int e = tid; e < SORT_WAVES * SORT_MAX_E; e += SORT_THREADS) (&next[0][0])[e] = 0;
+    __syncthreads();
+    for (int i = lane; i < SPAN; i += 64) {
+        const int e = expert_of(ids, s0 + wave * SPAN + i, R, E);
+        if (e >= 0) atomicAdd(&next[wave][e], 1);
+    }
+    // totals of all runs, and of the runs before this one
+    int carry = 0;
+    for (int e0 = 0; e0 < E; e0 += SORT_THREADS) {
+        const int e = e0 + tid;
+        int all = 0, before = 0;
+        if (e < E)
+            for (int b = 0; b < runs; ++b) {
+                const int c = counts[(size_t)b * E + e];
+                before += b < (int)blockIdx.x ? c : 0;
+                all += c;
+            }
+        int sum = all;
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) {
+            const int o = __shfl_up(sum, d);
+            if (lane >= d) sum += o;
+        }
+        if (lane == 63) wave_sum[wave] = sum;
+        __syncthreads();
+        int first = carry + sum - all;
+        for (int v = 0; v < SORT_WAVES; ++v) {
+            if (v < wave) first += wave_sum[v];
+            carry += wave_sum[v];
+        }
+        if (e < E) {
+            if (blockIdx.x == 0) offsets[e] = first;
+            total[e] = first + before;
+        }
+        __syncthreads();
+    }
+    if (tid == 0) {
+        used = carry;
+        if (blockIdx.x == 0) offsets[E] = carry;
+    }
+    // each wave's first row of each expert
+    for (int e = tid; e < E; e += SORT_THREADS) {
+        int at = total[e];
+        for (int v = 0; v < SORT_WAVES; ++v) {
+            const int c = next[v][e];
+            next[v][e] = at;
+            at += c;
+        }
+    }
+    __syncthreads();
+    for (int i = lane; i < SPAN; i += 64) {
+        const int s = s0 + wave * SPAN + i;
+        const int e = expert_of(ids, s, R, E);
+        unsigned long long same = __ballot(e >= 0);
+        for (int bit = 0; (E - 1) >> bit; ++bit) {
+            const bool one = (e >> bit) & 1;
+            const unsigned long long m = __ballot(one);
+            same &= one ? m : ~m;
+        }
+        int row = -1;
+        if (e >= 0) row = next[wave][e] + __popcll(same & ((1ull << lane) - 1));
+        wave_sync();
+        if (e >= 0 && (same >> lane) == 1ull) next[wave][e] = row + 1;      // the last of them
+        wave_sync();
+        if (s < R) position[s] = row;
+        if (row >= 0) order[row] = s;
+    }
+    for (int i = tid; i < SORT_SLOTS; i += SORT_THREADS)
+        if (s0 + i < R && s0 + i >= used) order[s0 + i] = -1;
+}
+
+// Rows by the plan (a row number outside it is taken for an unused slot).  A workgroup takes a token and its threads 16 bytes (or one
+// element) of the row each.
+template <int DT>
+struct RowVec {                              // 16 bytes of a row as floats
+    static constexpr int N = DT == DT_F32 ? 4 : 8;
+    static __device__ __forceinline__ void unpack(v4u_mx w, float (&v)[N]) {
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == DT_F32) v[j] = __uint_as_float(w[j]);
+            else {
+                v[2 * j] = DT == DT_BF16 ? bf16lo_to_f32(w[j]) : f16bits_to_f32(w[j]);
+                v[2 * j + 1] = DT == DT_BF16 ? bf16hi_to_f32(w[j]) : f16bits_to_f32(w[j] >> 16);
+            }
+        }
+    }
+    static __device__ __forceinline__ v4u_mx pack(const float (&v)[N]) {
+        v4u_mx w;
+#pragma unroll
+        for (int j = 0; j < 4; ++j) {
+            if constexpr (DT == DT_F32) w[j] = __float_as_uint(v[j]);
+            else w[j] = DT == DT_BF16 ? pack_bf16x2(v[2 * j], v[2 * j + 1]) : pack_f16x2(v[2 * j], v[2 * j + 1]);
+        }
+        return w;
+    }
+};
+
+// One piece of a row: 16 bytes (VEC) or one element.
+template <int DT, bool VEC>
+struct Piece {
+    static constexpr int N = VEC ? RowVec<DT>::N : 1;
+    static constexpr int ES = DT == DT_F32 ? 4 : 2;
+    static __device__ __forceinline__ void load(const uint8_t* row, int i, float (&v)[N]) {
+        if constexpr (VEC) RowVec<DT>::unpack(reinterpret_cast<const v4u_mx*>(row)[i], v);
+        else if constexpr (DT == DT_F32) v[0] = reinterpret_cast<const float*>(row)[i];
+        else {
+            const uint32_t h = reinterpret_cast<const uint16_t*>(row)[i];
+            v[0] = DT == DT_BF16 ? __uint_as_float(h << 16) : f16bits_to_f32(h);
+        }
+    }
+    static __device__ __forceinline__ void store(uint8_t* row, int i, const float (&v)[N]) {
+        if constexpr (VEC) reinterpret_cast<v4u_mx*>(row)[i] = RowVec<DT>::pack(v);
+        else if constexpr (DT == DT_F32) reinterpret_cast<float*>(row)[i] = v[0];
+        else reinterpret_cast<uint16_t*>(row)[i] = (uint16_t)(DT == DT_BF16 ? pack_bf16x2(v[0], 0.0f) : pack_f16x2(v[0], 0.0f));
+    }
+};
+
+// Zeros in the rows past the last used one; the grid's workgroups share them.
+template <int DT, bool VEC>
+__device__ __forceinline__ void zero_tail(uint8_t* rows, const int* offsets, int R, int E, int D) {
+    using P = Piece<DT, VEC>;
+    const float z[P::N] = {};
+    for (int r = max(offsets[E], 0) + blockIdx.x; r < R; r += gridDim.x)
+        for (int i = threadIdx.x; i < D / P::N; i += blockDim.x) P::store(rows + (size_t)r * D * P::ES, i, z);
+}
+
+// gathered[position[t, j]] = x[t]
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void expert_gather_kernel(const uint8_t* __restrict__ x, const int* __restrict__ position,
+                                                            const int* __restrict__ offsets, uint8_t* __restrict__ rows, int R,
+                                                            int k, int E, int D) {
+    using P = Piece<DT, VEC>;
+    const int t = blockIdx.x;
+    for (int i = threadIdx.x; i < D / P::N; i += 256) {
+        float v[P::N];
+        P::load(x + (size_t)t * D * P::ES, i, v);
+        for (int j = 0; j < k; ++j) {
+            const int r = position[(size_t)t * k + j];
+            if ((unsigned)r < (unsigned)R) P::store(rows + (size_t)r * D * P::ES, i, v);
+        }
+    }
+    zero_tail<DT, VEC>(rows, offsets, R, E, D);
+}
+
+// out[t] = sum_j w[t, j] rows[position[t, j]] (w NULL: 1)
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void expert_combine_kernel(const uint8_t* __restrict__ rows, const float* __restrict__ w,
+                                                             const int* __restrict__ position, uint8_t* __restrict__ out, int R,
+                                                             int k, int D) {
+    using P = Piece<DT, VEC>;
+    const int t = blockIdx.x;
+    for (int i = threadIdx.x; i < D / P::N; i += 256) {
+        float s[P::N] = {};
+        for (int j = 0; j < k; ++j) {
+            const int r = position[(size_t)t * k + j];
+            if ((unsigned)r >= (unsigned)R) continue;
+            const float f = w != nullptr ? w[(size_t)t * k + j] : 1.0f;
+            float v[P::N];
+            P::load(rows + (size_t)r * D * P::ES, i, v);
+#pragma unroll
+            for (int n = 0; n < P::N; ++n) s[n] = fmaf(f, v[n], s[n]);
+        }
+        P::store(out + (size_t)t * D * P::ES, i, s);
+    }
+}
+
+// d_rows[position[t, j]] = w[t, j] d_out[t]; d_w[t, j] = <d_out[t], rows[position[t, j]]>, 0
+// for an unused slot; either may be NULL
+template <int DT, bool VEC>
+__global__ __launch_bounds__(256) void expert_combine_grad_kernel(
+        const uint8_t* __restrict__ rows, const float* __restrict__ w, const int* __restrict__ position,
+        const int* __restrict__ offsets, const uint8_t* __restrict__ d_out, uint8_t* __restrict__ d_rows,
+        float* __restrict__ d_w, int R, int k, int E, int D) {
+    using P = Piece<DT, VEC>;
+    __shared__ float part[4];
+    const int t = blockIdx.x;
+    for (int j = 0; j < k; ++j) {
+        const int r = position[(size_t)t * k + j];
+        const float f = w[(size_t)t * k + j];
+        float dot = 0.0f;
+        if ((unsigned)r < (unsigned)R)
+            for (int i = threadIdx.x; i < D / P::N; i += 256) {
+                float v[P::N], g[P::N];
+                P::load(rows + (size_t)r * D * P::ES, i, v);
+                P::load(d_out + (size_t)t * D * P::ES, i, g);
+#pragma unroll
+                for (int n = 0; n < P::N; ++n) {
+                    dot = fmaf(v[n], g[n], dot);
+                    g[n] *= f;
+                }
+                if (d_rows != nullptr) P::store(d_rows + (size_t)r * D * P::ES, i, g);
+            }
+#pragma unroll
+        for (int d = 1; d < 64; d <<= 1) dot += __shfl_xor(dot, d);
+        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+        __syncthreads();
+        if (threadIdx.x == 0 && d_w != nullptr) d_w[(size_t)t * k + j] = (part[0] + part[1]) + (part[2] + part[3]);
+        __syncthreads();
+    }
+    if (d_rows != nullptr) zero_tail<DT, VEC>(d_rows, offsets, R, E, D);
+}
+
+int expert_max() { return SORT_MAX_E; }
+
+size_t expert_sort_bytes(int R, int E) { return (size_t)((R + SORT_SLOTS - 1) / SORT_SLOTS) * E * sizeof(int); }
+
+template <typename ID>
+static void sort_go(const void* ids, int* order, int* position, int* offsets, int* counts, int R, int E, hipStream_t st) {
+    const int runs = R > 0 ? (R + SORT_SLOTS - 1) / SORT_SLOTS : 1;
+    const ID* p = reinterpret_cast<const ID*>(ids);
+    hipLaunchKernelGGL((expert_count_kernel<ID>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, R, E);
+    hipLaunchKernelGGL((expert_place_kernel<ID>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, order, position, offsets, R,
+                       E, runs);
+}
+
+hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R, int E,
+                              hipStream_t st) {
+    if (id_bytes == 8) sort_go<long long>(ids, order, position, offsets, counts, R, E, st);
+    else sort_go<int>(ids, order, position, offsets, counts, R, E, st);
+    return hipGetLastError();
+}
+
+// f(type code, vector pieces) for the row type; vector pieces where rows are whole 16-byte pieces
+template <typename F>
+static void by_type(int dt, int D, F f) {
+    const bool vec = D % (dt == DT_F32 ? 4 : 8) == 0;
+    using std::integral_constant;
+    using T = std::true_type;
+    using N = std::false_type;
+    if (dt == DT_F32) vec ? f(integral_constant<int, DT_F32>{}, T{}) : f(integral_constant<int, DT_F32>{}, N{});
+    else if (dt == DT_BF16) vec ? f(integral_constant<int, DT_BF16>{}, T{}) : f(integral_constant<int, DT_BF16>{}, N{});
+    else vec ? f(integral_constant<int, DT_F16>{}, T{}) : f(integral_constant<int, DT_F16>{}, N{});
+}
+
+hipError_t expert_gather_launch(const void* x, int dt, const int* position, const int* offsets, void* rows, int T, int k, int E,
+                                int D, hipStream_t st) {
+    by_type(dt, D, [&](auto d, auto v) {
+        hipLaunchKernelGGL((expert_gather_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
+                           reinterpret_cast<const uint8_t*>(x), position, offsets, reinterpret_cast<uint8_t*>(rows), T * k, k, E,
+                           D);
+    });
+    return hipGetLastError();
+}
+
+hipError_t expert_combine_launch(const void* rows, int dt, const float* w, const int* position, void* out, int T, int k, int D,
+                                 hipStream_t st) {
+    by_type(dt, D, [&](auto d, auto v) {
+        hipLaunchKernelGGL((expert_combine_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
+                           reinterpret_cast<const uint8_t*>(rows), w, position, reinterpret_cast<uint8_t*>(out), T * k, k, D);
+    });
+    return hipGetLastError();
+}
+
+hipError_t expert_combine_grad_launch(const void* rows, int dt, const float* w, const int* position, const int* offsets,
+                                      const void* d_out, void* d_rows, float* d_w, int T, int k, int E, int D, hipStream_t st) {
+    by_type(dt, D, [&](auto d, auto v) {
+        hipLaunchKernelGGL((expert_combine_grad_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
+                           reinterpret_cast<const uint8_t*>(rows), w, position, offsets, reinterpret_cast<const uint8_t*>(d_out),
+                           reinterpret_cast<uint8_t*>(d_rows), d_w, T * k, k, E, D);
+    });
+    return hipGetLastError();
+}
+
+}  // namespace convrot

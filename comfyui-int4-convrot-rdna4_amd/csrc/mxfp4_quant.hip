@@ -1,0 +1,146 @@
+// Quantization of rows to microscaled 4-bit floats, with the block-Hadamard
+// rotation on the way, and back.
+//
+// Per 32 values: s = 2^(floor(log2 max|y|) - 2), code = E2M1 nearest to y / s
+// (ties to even, past 6 to 6), y = x or x rotated in groups of 16, 64 or 256.
+// Bound by memory: a value is read once (2 or 4 bytes) and leaves 17/32 bytes.
+// A lane holds 16 consecutive values, so a block is two neighbouring lanes, a
+// rotation group 1, 4 or 16 of them, and every exchange is a DPP operand of the
+// instruction that uses it: no LDS, no barrier.  Blocks and groups lie whole in
+// a row, so the matrix is walked as one array and rows do not matter, except
+// where the codes' rows are padded.
+
+#include "mxfp4.h"
+
+namespace convrot {
+
+// PAD: rows of `codes` / `scales` are padded to Kp values (Kp % 32 == 0), the padding codes 0 with scale byte 0.
+template <int DT, int G, bool PAD>
+__global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
+                                                          uint8_t* __restrict__ scales, long long units, int K, int Kp) {
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;       // 16 values of the (padded) matrix
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    if constexpr (PAD) {
+        const int upr = Kp / 16;
+        const long long row = u / upr;
+        const int k = (int)(u - row * upr) * 16;
+        if (u < units && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
+    } else {
+        if (u < units) load16<DT>(x + (size_t)u * 16 * ES, v);
+    }
+    rotate16<G>(v);
+    uint32_t sb;
+    const v2u_mx c = mx_encode16(v, sb);
+    if (u < units) {
+        *reinterpret_cast<v2u_mx*>(codes + (size_t)u * 8) = c;
+        if ((threadIdx.x & 1) == 0) scales[u >> 1] = (uint8_t)sb;
+    }
+}
+
+// Values of the codes, rotated back (the rotation is its own inverse), rounded once to the output type.
+template <int DT, int G>
+__global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __restrict__ codes,
+                                                            const uint8_t* __restrict__ scales, uint8_t* __restrict__ out,
+                                                            long long units) {
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;
+    v2u_mx c = {0u, 0u};
+    uint32_t sb = 127u;
+    if (u < units) {
+        c = *reinterpret_cast<const v2u_mx*>(codes + (size_t)u * 8);
+        sb = scales[u >> 1];
+    }
+    // code -> value / 2: sign, exponent and mantissa bits moved to their places in a float whose
+    // exponent 0 is a half unit (0 and 1 are 0 and .5: the mantissa bit counts 2^-2 there), times
+    // 2^126, which makes subnormal numbers of the moved bits normal ones.
+    const float scale = sb == 255u ? __builtin_nanf("") : sb == 0u ? 0x1p-127f : __uint_as_float(sb << 23);
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) {
+        const uint32_t n = (c[i >> 3] >> (4 * (i & 7))) & 15u;
+        const float m = __uint_as_float(((n & 8u) << 28) | ((n & 7u) << 22));
+        v[i] = (m * 0x1p126f) * scale;
+    }
+    rotate16<G>(v);
+    if (u >= units) return;
+    uint8_t* o = out + (size_t)u * 16 * ES;
+    if constexpr (DT == DT_F32) {
+#pragma unroll
+        for (int i = 0; i < 4; ++i)
+            reinterpret_cast<float4*>(o)[i] = make_float4(v[4 * i], v[4 * i + 1], v[4 * i + 2], v[4 * i + 3]);
+    } else {
+#pragma unroll
+        for (int i = 0; i < 2; ++i) {
+            v4u_mx w;
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const float a = v[8 * i + 2 * j], b = v[8 * i + 2 * j + 1];
+                w[j] = DT == DT_BF16 ? pack_bf16x2(a, b) : pack_f16x2(a, b);
+            }
+            reinterpret_cast<v4u_mx*>(o)[i] = w;
+        }
+    }
+}
+
+template <int DT, int G>
+static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, hipStream_t st) {
+    const long long units = (long long)M * (Kp / 16);
+    const dim3 grid((unsigned)((units + 255) / 256));
+    const auto xb = reinterpret_cast<const uint8_t*>(x);
+    const auto cb = reinterpret_cast<uint8_t*>(codes);
+    const auto sb = reinterpret_cast<uint8_t*>(scales);
+    if (Kp == K) hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, false>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp);
+    else hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, true>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp);
+}
+
+template <int DT>
+static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st) {
+    switch (G) {
+        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, st);
+        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, st);
+        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, st);
+        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, st);
+    }
+}
+
+// x [M, K] -> codes [M, Kp/2], scales [M, Kp/32]
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st) {
+    if (M == 0) return hipSuccess;
+    switch (dt) {
+        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, G, st); break;
+        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, G, st); break;
+        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, G, st); break;
+    }
+    return hipGetLastError();
+}
+
+template <int DT>
+static void dequant_group(const void* codes, const void* scales, void* out, long long units, int G, hipStream_t st) {
+    const dim3 grid((unsigned)((units + 255) / 256));
+    const auto cb = reinterpret_cast<const uint8_t*>(codes);
+    const auto sb = reinterpret_cast<const uint8_t*>(scales);
+    const auto ob = reinterpret_cast<uint8_t*>(out);
+    switch (G) {
+        case 0: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 0>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
+        case 16: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 16>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
+        case 64: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 64>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
+        default: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 256>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
+    }
+}
+
+hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
+                                hipStream_t st) {
+    if (M == 0) return hipSuccess;
+    const long long units = (long long)M * (K / 16);
+    switch (dt) {
+        case DT_F32: dequant_group<DT_F32>(codes, scales, out, units, G, st); break;
+        case DT_BF16: dequant_group<DT_BF16>(codes, scales, out, units, G, st); break;
+        default: dequant_group<DT_F16>(codes, scales, out, units, G, st); break;
+    }
+    return hipGetLastError();
+}
+
+}  // namespace convrot

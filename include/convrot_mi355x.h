@@ -403,6 +403,70 @@ int cr_max_quant_k(void);
 int cr_convrot_dequant(const void* q, int bits, const void* scale, void* out, int out_dtype, int N, int K, int G,
                        void* stream);
 
+/*
+ * Microscaled 4-bit floats (MXFP4).  No counterpart in the reference.
+ *
+ * A row of K values (K % 32 == 0) is K/2 bytes of E2M1 codes (bit 3 the sign,
+ * then two exponent bits and a mantissa bit: 0, .5, 1, 1.5, 2, 3, 4, 6; value 2j
+ * in the low half of byte j) and K/32 scale bytes, byte s standing for
+ * 2^(s - 127) and 255 for NaN.  Quantizing takes y = x, or x rotated by H_G where
+ * G is 16, 64 or 256 (0: not), in fp32, and per 32 values the scale
+ * 2^max(floor(log2 max|y|) - 2, -127) and the nearest codes of y / scale, ties to
+ * even, magnitudes past 6 to 6.  A block with a NaN or an infinity gets scale
+ * byte 255 and codes 0, a block of zeros scale byte 0.
+ *
+ * cr_mxfp4_quant: x [M, K] (in_dtype) -> codes [M, K/2], scales [M, K/32].
+ * cr_mxfp4_dequant: the codes' values, rotated back, [M, K] in out_dtype.
+ * cr_mxfp4_linear: out[m, n] = sum_k q(x)[m, k] W[n, k] + bias[n], x and out
+ *   [M, ..] of `dtype`, W codes [N, K/2] with scales [N, K/32] as cr_mxfp4_quant
+ *   writes them; products and sums in fp32, rounded once; bias NULL or of
+ *   bias_dtype.  workspace: >= cr_mxfp4_linear_workspace(M, K) bytes.
+ * Pointers 16-byte aligned; K <= 2^24.
+ */
+int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream);
+int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
+                     void* stream);
+size_t cr_mxfp4_linear_workspace(int M, int K);
+int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,
+                    void* out, int M, int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream);
+
+/*
+ * Expert routing.  No counterpart in the reference.
+ *
+ * Token t's slot j is number t k + j; it goes to expert ids[t, j], or to none
+ * where the id is outside [0, E).  cr_expert_sort (ids int32 or int64, id_bytes 4
+ * or 8; R = T k slots; E <= cr_max_experts()) writes the stable plan: order[R] (the
+ * slot of each sorted row, -1 past the last), position[R] (the sorted row of each
+ * slot, -1 for an unused one), offsets[E + 1] (expert e's rows are offsets[e] ..
+ * offsets[e + 1] - 1).  workspace: >= cr_expert_sort_workspace(R, E) bytes.
+ *
+ * cr_expert_gather: rows[position[t, j]] = x[t], rows past the last used one zero.
+ * cr_expert_combine: out[t] = sum_j weights[t, j] rows[position[t, j]] over the used
+ *   slots in order, in fp32 (weights NULL: 1; then it is the gather's gradient).
+ * cr_expert_combine_grad: d_rows[position[t, j]] = weights[t, j] d_out[t], zero past
+ *   the last used row; d_weights[t, j] = <d_out[t], rows[position[t, j]]>, zero for an
+ *   unused slot; either output may be NULL.
+ * cr_mxfp4_expert_linear: out[r] = q(x[source(r)]) W[e(r)]^T + bias[e(r)] for the R
+ *   sorted rows, zero past the last used one.  W codes [E, N, K/2], scales
+ *   [E, N, K/32], bias NULL or [E, N].  order NULL: x has the R sorted rows; else x has
+ *   the R / top_k tokens and source(r) = order[r] / top_k.  workspace: >=
+ *   cr_mxfp4_linear_workspace(rows of x, K) bytes.
+ * Rows of `dtype`, [.., D] or [.., K] contiguous; weights f32.
+ */
+int cr_max_experts(void);
+size_t cr_expert_sort_workspace(int R, int E);
+int cr_expert_sort(const void* ids, int id_bytes, int* order, int* position, int* offsets, int R, int E,
+                   void* workspace, size_t workspace_bytes, void* stream);
+int cr_expert_gather(const void* x, int dtype, const int* position, const int* offsets, void* rows, int T, int k, int E,
+                     int D, void* stream);
+int cr_expert_combine(const void* rows, int dtype, const float* weights, const int* position, void* out, int T, int k,
+                      int D, void* stream);
+int cr_expert_combine_grad(const void* rows, int dtype, const float* weights, const int* position, const int* offsets,
+                           const void* d_out, void* d_rows, float* d_weights, int T, int k, int E, int D, void* stream);
+int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k, const int* offsets, int E,
+                           const void* W, const void* wscales, const void* bias, int bias_dtype, void* out, int R,
+                           int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream);
+
 /* CR_ABI_VERSION of the header this library was built with. */
 int cr_abi_version(void);
 
