@@ -130,7 +130,7 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     b = None if bias is None else native._aligned(bias)
     M = _rows(x2.numel() // K)
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
-    nbytes = lib.cr_mxfp4_linear_workspace(M, K)
+    nbytes = lib.cr_mxfp4_linear_workspace(M, N, K, 1)
     st = native._stream(x.device)
     with native.on_device(x.device), native._call_lock(x.device, st):
         work = native._workspace(x.device, st, nbytes)
@@ -178,7 +178,7 @@ def mxfp4_expert_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.T
     w, ws = native._aligned(qweight), native._aligned(wscales)
     b = None if bias is None else native._aligned(bias)
     out = torch.empty((R, N), dtype=x.dtype, device=x.device)
-    nbytes = lib.cr_mxfp4_linear_workspace(x2.shape[0], K)
+    nbytes = lib.cr_mxfp4_linear_workspace(x2.shape[0], N, K, E)
     st = native._stream(x.device)
     with native.on_device(x.device), native._call_lock(x.device, st):
         work = native._workspace(x.device, st, nbytes)

@@ -84,7 +84,7 @@ _SIGNATURES = {
     "cr_convrot_dequant": ([_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp], _i),
     "cr_mxfp4_quant": ([_vp, _i, _vp, _vp, _i, _i, _i, _vp], _i),
     "cr_mxfp4_dequant": ([_vp, _vp, _vp, _i, _i, _i, _i, _vp], _i),
-    "cr_mxfp4_linear_workspace": ([_i, _i], ctypes.c_size_t),
+    "cr_mxfp4_linear_workspace": ([_i] * 4, ctypes.c_size_t),
     "cr_mxfp4_linear": ([_vp, _i, _vp, _vp, _vp, _i, _vp] + [_i] * 4 + [_vp, ctypes.c_size_t, _vp], _i),
     "cr_mxfp4_expert_linear": ([_vp, _i, _vp, _i, _vp, _i, _vp, _vp, _vp, _i, _vp] + [_i] * 4
                                + [_vp, ctypes.c_size_t, _vp], _i),

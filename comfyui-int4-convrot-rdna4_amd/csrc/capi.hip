@@ -47,7 +47,10 @@ hipError_t dequant_launch(const void* q, int bits, const float* s, void* out, in
                           hipStream_t st);
 hipError_t gemm_splitk_launch(const int8_t* Xp, const int8_t* Wp, const float* xs, const float* ws, float* accum,
                               int M, int N, int K, int nsplit, hipStream_t st);
-hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st);
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G,
+                              hipStream_t st);
+hipError_t mxfp4_pad_scales_launch(const void* src, void* dst, long long rows, int nb, int Ks, hipStream_t st);
+bool mxfp4_gemm_staged(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
 hipError_t mxfp4_gemm_launch(const MxProblem& p, hipStream_t st);
@@ -549,7 +552,8 @@ static int mx_args_ok(int dtype, int M, int K, int G) {
 
 API int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream) {
     if (!mx_args_ok(in_dtype, M, K, G)) return -1;
-    return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, K, G, reinterpret_cast<hipStream_t>(stream));
+    return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, K, K / convrot::MX_BLOCK, G,
+                                            reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
@@ -558,33 +562,44 @@ API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int o
     return (int)convrot::mxfp4_dequant_launch(codes, scales, out, out_dtype, M, K, G, reinterpret_cast<hipStream_t>(stream));
 }
 
-// Codes and scales of x, rows padded to a multiple of 128 values, after the counter region.
-struct MxPlan { size_t codes, scales, total; int Kp; };
-static MxPlan mx_plan(int M, int K) {
+// After the counter region: the codes and scales of x in padded rows, and the weight's scales in rows of Ks bytes
+// where they are not that already.
+struct MxPlan { size_t codes, scales, wscales, total; int Kp, Ks; };
+static MxPlan mx_plan(long long M, long long rows_w, int K) {
     MxPlan p;
     p.Kp = (K + 127) / 128 * 128;
+    p.Ks = (K / convrot::MX_BLOCK + 15) / 16 * 16;
     p.codes = kSplitCounterBytes;
-    p.scales = p.codes + (size_t)M * (p.Kp / 2);                      // 64 bytes or more a row: stays 16-byte aligned
-    p.total = p.scales + ((size_t)M * (p.Kp / 32) + 15) / 16 * 16;
+    p.scales = p.codes + (size_t)M * (p.Kp / 2);                      // 64 bytes or more a row: 16-byte aligned
+    p.wscales = p.scales + (size_t)M * p.Ks;
+    p.total = p.wscales + (p.Ks == K / convrot::MX_BLOCK ? 0 : (size_t)rows_w * p.Ks);
     return p;
 }
 
-// x [rows, K] quantized into the workspace, then the product; `p` but for the activation's operand
+// x [rows, K] quantized into the workspace, then the product; `p` but for the operands laid out there
 static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, void* workspace, size_t workspace_bytes,
                          hipStream_t st) {
-    const MxPlan plan = mx_plan(rows, p.K);
+    const long long rows_w = (long long)p.E * p.N;
+    const MxPlan plan = mx_plan(rows, rows_w, p.K);
     if (workspace == nullptr || workspace_bytes < plan.total) return -1;
     uint8_t* ws = reinterpret_cast<uint8_t*>(workspace);
     p.a = ws + plan.codes;
     p.as = ws + plan.scales;
     p.Kp = plan.Kp;
-    const hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, G, st);
+    p.Ks = plan.Ks;
+    p.wp = p.ws;
+    hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, p.Ks, G, st);
     if (e != hipSuccess) return (int)e;
+    if (p.Ks != p.K / convrot::MX_BLOCK && convrot::mxfp4_gemm_staged(p)) {
+        p.wp = ws + plan.wscales;
+        e = convrot::mxfp4_pad_scales_launch(p.ws, ws + plan.wscales, rows_w, p.K / convrot::MX_BLOCK, p.Ks, st);
+        if (e != hipSuccess) return (int)e;
+    }
     return (int)convrot::mxfp4_gemm_launch(p, st);
 }
 
-API size_t cr_mxfp4_linear_workspace(int M, int K) {
-    return M <= 0 || K <= 0 || K % convrot::MX_BLOCK != 0 ? 0 : mx_plan(M, K).total;
+API size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E) {
+    return M <= 0 || N <= 0 || E < 1 || K <= 0 || K % convrot::MX_BLOCK != 0 ? 0 : mx_plan(M, (long long)N * E, K).total;
 }
 
 API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,
@@ -596,7 +611,8 @@ API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wsc
     p.ws = reinterpret_cast<const uint8_t*>(wscales);
     p.bias = bias;
     p.out = out;
-    p.R = M; p.N = N; p.K = K; p.E = 1; p.top_k = 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    p.R = M; p.N = N; p.K = K; p.E = 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    convrot::mx_set_top_k(p, 1);
     return mx_linear_run(x, M, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 
@@ -614,7 +630,8 @@ API int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int t
     p.out = out;
     p.offsets = offsets;
     p.order = order;
-    p.R = R; p.N = N; p.K = K; p.E = E; p.top_k = order != nullptr ? top_k : 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    p.R = R; p.N = N; p.K = K; p.E = E; p.dt = dtype; p.bias_dt = bias_dtype;
+    convrot::mx_set_top_k(p, order != nullptr ? top_k : 1);
     return mx_linear_run(x, R / p.top_k, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
 

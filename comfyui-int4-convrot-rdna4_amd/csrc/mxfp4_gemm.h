@@ -8,17 +8,30 @@
 namespace convrot {
 
 // y[r, n] = sum_k a[row(r), k] w[e(r)][n, k] + bias[e(r)][n] for the R rows of the output.
-// a: codes [rows, Kp/2] and scales [rows, Kp/32], Kp = K rounded up to 128, the padding codes zero.
-// w: codes [E, N, K/2] and scales [E, N, K/32].  offsets NULL: E = 1 and row(r) = r.  Else rows
-// offsets[e] .. offsets[e + 1] - 1 are expert e's, those from offsets[E] on come out zero, and
-// row(r) = r, or order[r] / top_k where order is not NULL.
+// a: codes [rows, Kp/2], Kp = K rounded up to 128, the padding codes zero with scale byte 0; scales
+// [rows, Ks], Ks = K/32 rounded up to 16 (what is past Kp/32 is never used).
+// w: codes [E, N, K/2] and scales [E, N, K/32]; wp: the scales in rows of Ks bytes, the padding 0
+// (the scales themselves where Ks = K/32).
+// offsets NULL: E = 1 and row(r) = r.  Else rows offsets[e] .. offsets[e + 1] - 1 are expert e's, those from
+// offsets[E] on come out zero, and row(r) = r, or order[r] / top_k where order is not NULL.
 struct MxProblem {
-    const uint8_t *a, *as, *w, *ws;
+    const uint8_t *a, *as, *w, *ws, *wp;
     const void* bias;
     void* out;
     const int *offsets, *order;
-    int R, N, K, Kp, E, top_k, dt, bias_dt;
+    int R, N, K, Kp, Ks, E, top_k, dt, bias_dt;
+    unsigned k_mul;                                        // n / top_k = n k_mul >> k_shift for 0 <= n < 2^31
+    int k_shift;
 };
+
+// l = ceil(log2 d), m = ceil(2^(31 + l) / d): n m >> (31 + l) is n / d for every n < 2^31, and m < 2^32.
+inline void mx_set_top_k(MxProblem& p, int d) {
+    int l = 0;
+    while ((1ll << l) < d) ++l;
+    p.top_k = d;
+    p.k_shift = 31 + l;
+    p.k_mul = (unsigned)(((1ull << p.k_shift) + d - 1) / d);
+}
 
 // A tile of at most BM rows: rows m0 .. m1 - 1 of expert e, or rows to be zeroed (e = E).
 struct MxTile { int e, m0, m1; };
@@ -30,42 +43,49 @@ inline long long mx_row_tiles(int R, int E, bool ragged, int BM) {
     return R / BM + (E + 1LL < R ? E + 1LL : R);
 }
 
-// Row tile `t` of the grid, found by the whole wave from the experts' offsets:
-// lane l holds expert l of each run of 64, the tiles are counted with a prefix
-// sum over the lanes.  False: past the last tile.
+// Expert e's rows as the wave's lanes hold them, 64 experts a run; expert E is the rows past the last used one.
 template <int BM>
-__device__ __forceinline__ bool mx_tile(const MxProblem& p, int t, MxTile& tile) {
-    if (p.offsets == nullptr) {
-        tile = {0, t * BM, min(t * BM + BM, p.R)};
-        return tile.m0 < p.R;
-    }
-    const int lane = threadIdx.x & 63;
-    int base = 0;
-    for (int e0 = 0; e0 <= p.E; e0 += 64) {                // expert E: the rows past the last used one
-        const int e = e0 + lane;
-        const int r0 = e <= p.E ? min(max(p.offsets[e], 0), p.R) : p.R;
-        const int r1 = e < p.E ? min(max(p.offsets[e + 1], r0), p.R) : p.R;
-        const int n = (r1 - r0 + BM - 1) / BM;
-        int sum = n;
+struct MxRun {
+    int r0, r1, n, sum;                                    // rows, their tiles, tiles of this and the lanes before
+    __device__ __forceinline__ MxRun(const MxProblem& p, int e) {
+        r0 = e <= p.E ? min(max(p.offsets[e], 0), p.R) : p.R;
+        r1 = e < p.E ? min(max(p.offsets[e + 1], r0), p.R) : p.R;
+        sum = n = (r1 - r0 + BM - 1) / BM;
+        const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
             const int o = __shfl_up(sum, d);
             if (lane >= d) sum += o;
         }
-        const int first = base + sum - n;
-        const unsigned long long here = __ballot(t >= first && t < first + n);
+    }
+};
+
+// Row tiles that there are.
+template <int BM>
+__device__ __forceinline__ int mx_tile_count(const MxProblem& p) {
+    if (p.offsets == nullptr) return (p.R + BM - 1) / BM;
+    int count = 0;
+    for (int e0 = 0; e0 <= p.E; e0 += 64) count += __shfl(MxRun<BM>(p, e0 + (threadIdx.x & 63)).sum, 63);
+    return __builtin_amdgcn_readfirstlane(count);
+}
+
+// Row tile t, which there is.
+template <int BM>
+__device__ __forceinline__ MxTile mx_tile(const MxProblem& p, int t) {
+    if (p.offsets == nullptr) return {0, t * BM, min(t * BM + BM, p.R)};
+    int base = 0;
+    for (int e0 = 0; e0 <= p.E; e0 += 64) {
+        const MxRun<BM> run(p, e0 + (threadIdx.x & 63));
+        const int first = base + run.sum - run.n;
+        const unsigned long long here = __ballot(t >= first && t < first + run.n);
         if (here) {
             const int l = __builtin_ctzll(here);
-            const int m0 = __shfl(r0 + (t - first) * BM, l);
-            tile = {e0 + l, m0, min(m0 + BM, __shfl(r1, l))};
-            tile.e = __builtin_amdgcn_readfirstlane(tile.e);
-            tile.m0 = __builtin_amdgcn_readfirstlane(tile.m0);
-            tile.m1 = __builtin_amdgcn_readfirstlane(tile.m1);
-            return true;
+            const int m0 = __builtin_amdgcn_readfirstlane(__shfl(run.r0 + (t - first) * BM, l));
+            return {e0 + l, m0, __builtin_amdgcn_readfirstlane(min(m0 + BM, __shfl(run.r1, l)))};
         }
-        base += __shfl(sum, 63);
+        base += __shfl(run.sum, 63);
     }
-    return false;
+    return {p.E, p.R, p.R};
 }
 
 __device__ __forceinline__ float mx_read(const void* p, int dt, size_t i) {
@@ -91,7 +111,9 @@ __device__ __forceinline__ void mx_store4(void* out, int dt, size_t i, const flo
 
 // Row of `a` that output row r takes.
 __device__ __forceinline__ int mx_source_row(const MxProblem& p, int r) {
-    return p.order != nullptr ? min(max(p.order[r], 0), p.R - 1) / p.top_k : r;
+    if (p.order == nullptr) return r;
+    const unsigned slot = (unsigned)min(max(p.order[r], 0), p.R - 1);
+    return (int)((unsigned long long)slot * p.k_mul >> p.k_shift);
 }
 
 // Zeros in rows m0 .. m1 - 1, columns n0 .. n1 - 1 (threads of a workgroup).

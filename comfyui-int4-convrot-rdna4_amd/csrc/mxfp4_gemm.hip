@@ -20,8 +20,8 @@ __device__ __forceinline__ v8i_mx mx_operand(v4u_mx c) {
 // 64 x 64 outputs by four waves of 32 x 32, operands from memory to registers.
 __global__ __launch_bounds__(256) void mxfp4_gemm_direct_kernel(MxProblem p, int tiles_n) {
     constexpr int BM = 64, BN = 64;
-    MxTile t;
-    if (!mx_tile<BM>(p, blockIdx.x / tiles_n, t)) return;
+    if ((int)(blockIdx.x / tiles_n) >= mx_tile_count<BM>(p)) return;
+    const MxTile t = mx_tile<BM>(p, blockIdx.x / tiles_n);
     const int n0 = (blockIdx.x % tiles_n) * BN;
     if (t.e == p.E && p.offsets != nullptr) return mx_zero(p, t.m0, t.m1, n0, min(n0 + BN, p.N));
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
@@ -31,7 +31,7 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_direct_kernel(MxProblem p, int
     const size_t ar = (size_t)mx_source_row(p, min(r, t.m1 - 1));
     const size_t wr = (size_t)t.e * p.N + min(n, p.N - 1);
     const uint8_t* a = p.a + ar * (p.Kp / 2);
-    const uint8_t* as = p.as + ar * (p.Kp / 32);
+    const uint8_t* as = p.as + ar * p.Ks;
     const uint8_t* w = p.w + wr * (p.K / 2);
     const uint8_t* ws = p.ws + wr * (p.K / 32);
     v16f_mx acc = {0};
@@ -60,8 +60,12 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_direct_kernel(MxProblem p, int
     }
 }
 
+bool mxfp4_gemm_staged(const MxProblem& p);
+hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st);
+
 hipError_t mxfp4_gemm_launch(const MxProblem& p, hipStream_t st) {
     if (p.R == 0 || p.N == 0) return hipSuccess;
+    if (mxfp4_gemm_staged(p)) return mxfp4_gemm_staged_launch(p, st);
     const int tiles_n = (p.N + 63) / 64;
     const long long grid = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 64) * tiles_n;
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;

@@ -14,19 +14,22 @@
 
 namespace convrot {
 
-// PAD: rows of `codes` / `scales` are padded to Kp values (Kp % 32 == 0), the padding codes 0 with scale byte 0.
+// PAD: rows of `codes` are padded to Kp values (Kp % 32 == 0), the padding codes 0 with scale byte 0, and rows
+// of `scales` have Ks >= Kp/32 bytes, the first Kp/32 of them written.
 template <int DT, int G, bool PAD>
 __global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
-                                                          uint8_t* __restrict__ scales, long long units, int K, int Kp) {
+                                                          uint8_t* __restrict__ scales, long long units, int K, int Kp, int Ks) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     const long long u = (long long)blockIdx.x * 256 + threadIdx.x;       // 16 values of the (padded) matrix
     float v[16];
+    size_t block = (size_t)u >> 1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.0f;
     if constexpr (PAD) {
         const int upr = Kp / 16;
         const long long row = u / upr;
         const int k = (int)(u - row * upr) * 16;
+        block = (size_t)row * Ks + k / 32;
         if (u < units && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
     } else {
         if (u < units) load16<DT>(x + (size_t)u * 16 * ES, v);
@@ -36,7 +39,7 @@ __global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restr
     const v2u_mx c = mx_encode16(v, sb);
     if (u < units) {
         *reinterpret_cast<v2u_mx*>(codes + (size_t)u * 8) = c;
-        if ((threadIdx.x & 1) == 0) scales[u >> 1] = (uint8_t)sb;
+        if ((threadIdx.x & 1) == 0) scales[block] = (uint8_t)sb;
     }
 }
 
@@ -86,34 +89,59 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
 }
 
 template <int DT, int G>
-static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, hipStream_t st) {
+static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, hipStream_t st) {
     const long long units = (long long)M * (Kp / 16);
     const dim3 grid((unsigned)((units + 255) / 256));
     const auto xb = reinterpret_cast<const uint8_t*>(x);
     const auto cb = reinterpret_cast<uint8_t*>(codes);
     const auto sb = reinterpret_cast<uint8_t*>(scales);
-    if (Kp == K) hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, false>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp);
-    else hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, true>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp);
+    if (Kp == K && Ks == K / 32) hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, false>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp, Ks);
+    else hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, true>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp, Ks);
 }
 
 template <int DT>
-static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st) {
+static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, hipStream_t st) {
     switch (G) {
-        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, st);
-        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, st);
-        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, st);
-        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, st);
+        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, Ks, st);
+        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, Ks, st);
+        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, Ks, st);
+        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, Ks, st);
     }
 }
 
-// x [M, K] -> codes [M, Kp/2], scales [M, Kp/32]
-hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int G, hipStream_t st) {
+// x [M, K] -> codes [M, Kp/2], scales [M, Ks]
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G,
+                              hipStream_t st) {
     if (M == 0) return hipSuccess;
     switch (dt) {
-        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, G, st); break;
-        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, G, st); break;
-        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, G, st); break;
+        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, Ks, G, st); break;
+        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, Ks, G, st); break;
+        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, Ks, G, st); break;
     }
+    return hipGetLastError();
+}
+
+// Scale rows of K/32 bytes -> rows of Ks (a multiple of 16), the padding 0: 16 bytes a thread.
+__global__ __launch_bounds__(256) void mxfp4_pad_scales_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
+                                                               long long pieces, int nb, int Ks) {
+    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
+    if (i >= pieces) return;
+    const int per = Ks / 16;
+    const long long row = i / per;
+    const int b0 = (int)(i - row * per) * 16;
+    const uint8_t* s = src + (size_t)row * nb + b0;
+    v4u_mx w = {0u, 0u, 0u, 0u};
+#pragma unroll
+    for (int j = 0; j < 16; ++j)
+        if (b0 + j < nb) w[j >> 2] |= (uint32_t)s[j] << (8 * (j & 3));
+    reinterpret_cast<v4u_mx*>(dst)[i] = w;
+}
+
+hipError_t mxfp4_pad_scales_launch(const void* src, void* dst, long long rows, int nb, int Ks, hipStream_t st) {
+    const long long pieces = rows * (Ks / 16);
+    if (pieces == 0) return hipSuccess;
+    hipLaunchKernelGGL(mxfp4_pad_scales_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st,
+                       reinterpret_cast<const uint8_t*>(src), reinterpret_cast<uint8_t*>(dst), pieces, nb, Ks);
     return hipGetLastError();
 }
 

@@ -420,13 +420,13 @@ int cr_convrot_dequant(const void* q, int bits, const void* scale, void* out, in
  * cr_mxfp4_linear: out[m, n] = sum_k q(x)[m, k] W[n, k] + bias[n], x and out
  *   [M, ..] of `dtype`, W codes [N, K/2] with scales [N, K/32] as cr_mxfp4_quant
  *   writes them; products and sums in fp32, rounded once; bias NULL or of
- *   bias_dtype.  workspace: >= cr_mxfp4_linear_workspace(M, K) bytes.
+ *   bias_dtype.  workspace: >= cr_mxfp4_linear_workspace(M, N, K, 1) bytes.
  * Pointers 16-byte aligned; K <= 2^24.
  */
 int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream);
 int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
                      void* stream);
-size_t cr_mxfp4_linear_workspace(int M, int K);
+size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E);
 int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,
                     void* out, int M, int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream);
 
@@ -450,7 +450,7 @@ int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales
  *   sorted rows, zero past the last used one.  W codes [E, N, K/2], scales
  *   [E, N, K/32], bias NULL or [E, N].  order NULL: x has the R sorted rows; else x has
  *   the R / top_k tokens and source(r) = order[r] / top_k.  workspace: >=
- *   cr_mxfp4_linear_workspace(rows of x, K) bytes.
+ *   cr_mxfp4_linear_workspace(rows of x, N, K, E) bytes.
  * Rows of `dtype`, [.., D] or [.., K] contiguous; weights f32.
  */
 int cr_max_experts(void);

@@ -161,8 +161,8 @@ def test_library_refuses(native):
     assert lib.cr_expert_gather(n, 1, n, n, n, 4, 0, 4, 8, n) == -1                      # k
     assert lib.cr_expert_combine(n, 1, n, n, n, 1 << 20, 1 << 12, 8, n) == -1            # slots past 2^31
     assert lib.cr_expert_combine_grad(n, 1, n, n, n, n, n, n, 4, 2, 4, 8, n) == -1       # no weights
-    assert lib.cr_mxfp4_linear_workspace(3, 1600) >= 3 * (1664 // 2 + 1664 // 32)
-    assert lib.cr_mxfp4_linear_workspace(0, 64) == 0
+    assert lib.cr_mxfp4_linear_workspace(3, 8, 1600, 1) >= 3 * (1664 // 2 + 1664 // 32)
+    assert lib.cr_mxfp4_linear_workspace(0, 8, 64, 1) == 0
 
 
 def test_names_are_public(q):
