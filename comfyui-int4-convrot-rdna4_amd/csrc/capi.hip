@@ -48,8 +48,8 @@ hipError_t dequant_launch(const void* q, int bits, const float* s, void* out, in
 hipError_t gemm_splitk_launch(const int8_t* Xp, const int8_t* Wp, const float* xs, const float* ws, float* accum,
                               int M, int N, int K, int nsplit, hipStream_t st);
 hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G,
-                              hipStream_t st);
-hipError_t mxfp4_pad_scales_launch(const void* src, void* dst, long long rows, int nb, int Ks, hipStream_t st);
+                              int layout, hipStream_t st);
+hipError_t mxfp4_tile_scales_launch(const void* src, void* dst, int E, int N, int nb, int Ks, hipStream_t st);
 bool mxfp4_gemm_staged(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
@@ -553,7 +553,7 @@ static int mx_args_ok(int dtype, int M, int K, int G) {
 API int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream) {
     if (!mx_args_ok(in_dtype, M, K, G)) return -1;
     return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, K, K / convrot::MX_BLOCK, G,
-                                            reinterpret_cast<hipStream_t>(stream));
+                                            convrot::MX_PLAIN, reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
@@ -562,17 +562,17 @@ API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int o
     return (int)convrot::mxfp4_dequant_launch(codes, scales, out, out_dtype, M, K, G, reinterpret_cast<hipStream_t>(stream));
 }
 
-// After the counter region: the codes and scales of x in padded rows, and the weight's scales in rows of Ks bytes
-// where they are not that already.
+// After the counter region: the codes and scales of x, rows padded, and the weight's scales in the order of staged
+// tiles.
 struct MxPlan { size_t codes, scales, wscales, total; int Kp, Ks; };
 static MxPlan mx_plan(long long M, long long rows_w, int K) {
     MxPlan p;
-    p.Kp = (K + 127) / 128 * 128;
+    p.Kp = (K + 255) / 256 * 256;
     p.Ks = (K / convrot::MX_BLOCK + 15) / 16 * 16;
     p.codes = kSplitCounterBytes;
-    p.scales = p.codes + (size_t)M * (p.Kp / 2);                      // 64 bytes or more a row: 16-byte aligned
+    p.scales = p.codes + (size_t)M * (p.Kp / 2);                      // 128 bytes or more a row: 16-byte aligned
     p.wscales = p.scales + (size_t)M * p.Ks;
-    p.total = p.wscales + (p.Ks == K / convrot::MX_BLOCK ? 0 : (size_t)rows_w * p.Ks);
+    p.total = p.wscales + (size_t)rows_w * p.Ks;
     return p;
 }
 
@@ -587,12 +587,14 @@ static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, v
     p.as = ws + plan.scales;
     p.Kp = plan.Kp;
     p.Ks = plan.Ks;
-    p.wp = p.ws;
-    hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, p.Ks, G, st);
+    p.as_rows = rows;
+    p.wp = ws + plan.wscales;
+    const bool staged = convrot::mxfp4_gemm_staged(p);
+    hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, p.Ks, G,
+                                               staged ? convrot::MX_TILES : convrot::MX_ROWS, st);
     if (e != hipSuccess) return (int)e;
-    if (p.Ks != p.K / convrot::MX_BLOCK && convrot::mxfp4_gemm_staged(p)) {
-        p.wp = ws + plan.wscales;
-        e = convrot::mxfp4_pad_scales_launch(p.ws, ws + plan.wscales, rows_w, p.K / convrot::MX_BLOCK, p.Ks, st);
+    if (staged) {
+        e = convrot::mxfp4_tile_scales_launch(p.ws, ws + plan.wscales, p.E, p.N, p.K / convrot::MX_BLOCK, p.Ks, st);
         if (e != hipSuccess) return (int)e;
     }
     return (int)convrot::mxfp4_gemm_launch(p, st);

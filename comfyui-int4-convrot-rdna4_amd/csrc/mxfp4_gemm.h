@@ -8,10 +8,10 @@
 namespace convrot {
 
 // y[r, n] = sum_k a[row(r), k] w[e(r)][n, k] + bias[e(r)][n] for the R rows of the output.
-// a: codes [rows, Kp/2], Kp = K rounded up to 128, the padding codes zero with scale byte 0; scales
-// [rows, Ks], Ks = K/32 rounded up to 16 (what is past Kp/32 is never used).
-// w: codes [E, N, K/2] and scales [E, N, K/32]; wp: the scales in rows of Ks bytes, the padding 0
-// (the scales themselves where Ks = K/32).
+// a: codes [as_rows, Kp/2], Kp = K rounded up to 256, the padding codes zero; w: codes [E, N, K/2] and scales
+// [E, N, K/32].  Scales for staged tiles: as [Ks/16, as_rows, 16] and wp [E, Ks/16, N, 16], Ks = K/32 rounded up
+// to 16, 512 k after the other, the bytes of a row in the order of mx_scale_place, the padding 0.  For the others
+// as is [as_rows, Ks] and wp is not there.
 // offsets NULL: E = 1 and row(r) = r.  Else rows offsets[e] .. offsets[e + 1] - 1 are expert e's, those from
 // offsets[E] on come out zero, and row(r) = r, or order[r] / top_k where order is not NULL.
 struct MxProblem {
@@ -19,7 +19,7 @@ struct MxProblem {
     const void* bias;
     void* out;
     const int *offsets, *order;
-    int R, N, K, Kp, Ks, E, top_k, dt, bias_dt;
+    int R, N, K, Kp, Ks, as_rows, E, top_k, dt, bias_dt;
     unsigned k_mul;                                        // n / top_k = n k_mul >> k_shift for 0 <= n < 2^31
     int k_shift;
 };
@@ -32,6 +32,13 @@ inline void mx_set_top_k(MxProblem& p, int d) {
     p.k_shift = 31 + l;
     p.k_mul = (unsigned)(((1ull << p.k_shift) + d - 1) / d);
 }
+
+// Where mxfp4_quant_launch puts codes and scales.
+enum : int { MX_PLAIN = 0, MX_ROWS = 1, MX_TILES = 2 };
+
+// Place of block b (0 .. 15) of 512 k: a lane of half h of a wave takes blocks 2 s + h of a stage of 256 k, s = 0 .. 3,
+// whose bytes are one word.
+__host__ __device__ constexpr int mx_scale_place(int b) { return (b & 8) | (b & 1) << 2 | (b >> 1 & 3); }
 
 // A tile of at most BM rows: rows m0 .. m1 - 1 of expert e, or rows to be zeroed (e = E).
 struct MxTile { int e, m0, m1; };
@@ -109,9 +116,8 @@ __device__ __forceinline__ void mx_store4(void* out, int dt, size_t i, const flo
     }
 }
 
-// Row of `a` that output row r takes.
+// Row of `a` that output row r takes where there is an order.
 __device__ __forceinline__ int mx_source_row(const MxProblem& p, int r) {
-    if (p.order == nullptr) return r;
     const unsigned slot = (unsigned)min(max(p.order[r], 0), p.R - 1);
     return (int)((unsigned long long)slot * p.k_mul >> p.k_shift);
 }

@@ -28,7 +28,7 @@ __global__ __launch_bounds__(256) void mxfp4_gemm_direct_kernel(MxProblem p, int
     const int r = t.m0 + (wave >> 1) * 32 + (lane & 31), half = lane >> 5;
     const int n = n0 + (wave & 1) * 32 + (lane & 31);
     // rows and columns past the edge repeat the last one; they are not stored
-    const size_t ar = (size_t)mx_source_row(p, min(r, t.m1 - 1));
+    const size_t ar = (size_t)(p.order != nullptr ? mx_source_row(p, min(r, t.m1 - 1)) : min(r, t.m1 - 1));
     const size_t wr = (size_t)t.e * p.N + min(n, p.N - 1);
     const uint8_t* a = p.a + ar * (p.Kp / 2);
     const uint8_t* as = p.as + ar * p.Ks;

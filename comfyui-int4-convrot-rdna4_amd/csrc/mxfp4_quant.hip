@@ -10,37 +10,54 @@
 // a row, so the matrix is walked as one array and rows do not matter, except
 // where the codes' rows are padded.
 
-#include "mxfp4.h"
+#include "mxfp4_gemm.h"
 
 namespace convrot {
 
-// PAD: rows of `codes` are padded to Kp values (Kp % 32 == 0), the padding codes 0 with scale byte 0, and rows
-// of `scales` have Ks >= Kp/32 bytes, the first Kp/32 of them written.
-template <int DT, int G, bool PAD>
+template <int DT, int G>
 __global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
-                                                          uint8_t* __restrict__ scales, long long units, int K, int Kp, int Ks) {
+                                                          uint8_t* __restrict__ scales, long long units) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
-    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;       // 16 values of the (padded) matrix
+    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;       // 16 values of the matrix
     float v[16];
-    size_t block = (size_t)u >> 1;
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    if constexpr (PAD) {
-        const int upr = Kp / 16;
-        const long long row = u / upr;
-        const int k = (int)(u - row * upr) * 16;
-        block = (size_t)row * Ks + k / 32;
-        if (u < units && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
-    } else {
-        if (u < units) load16<DT>(x + (size_t)u * 16 * ES, v);
-    }
+    if (u < units) load16<DT>(x + (size_t)u * 16 * ES, v);
     rotate16<G>(v);
     uint32_t sb;
     const v2u_mx c = mx_encode16(v, sb);
     if (u < units) {
         *reinterpret_cast<v2u_mx*>(codes + (size_t)u * 8) = c;
-        if ((threadIdx.x & 1) == 0) scales[block] = (uint8_t)sb;
+        if ((threadIdx.x & 1) == 0) scales[u >> 1] = (uint8_t)sb;
     }
+}
+
+// The activation of a product: rows of codes padded to Kp values (a multiple of 256) with codes 0, scales in rows of
+// Ks bytes or (TILES) in the order of staged tiles (mxfp4_gemm.h), 16 bytes of 512 k a row either way.  A workgroup
+// takes 512 k of 8 rows, so that its scales leave as one run of 128 bytes (a byte a block, as above, 8192 x 8192: 34 us).
+template <int DT, int G, bool TILES>
+__global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
+                                                               uint8_t* __restrict__ scales, int M, int K, int Kp, int Ks) {
+    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    __shared__ __attribute__((aligned(16))) uint8_t sc[8][16];
+    const int per = Ks / 16;
+    const int ss = blockIdx.x % per, row0 = (int)(blockIdx.x / per) * 8;
+    const int r = threadIdx.x >> 5, l = threadIdx.x & 31;
+    const int row = row0 + r, k = ss * 512 + l * 16;
+    float v[16];
+#pragma unroll
+    for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+    if (row < M && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
+    rotate16<G>(v);
+    uint32_t sb;
+    const v2u_mx c = mx_encode16(v, sb);
+    if (row < M && k < Kp) *reinterpret_cast<v2u_mx*>(codes + (size_t)row * (Kp / 2) + k / 2) = c;
+    if ((l & 1) == 0) sc[r][TILES ? mx_scale_place(l >> 1) : l >> 1] = (uint8_t)sb;
+    __syncthreads();
+    const int w = row0 + threadIdx.x;
+    if (threadIdx.x < 8 && w < M)
+        *reinterpret_cast<v4u_mx*>(scales + (TILES ? ((size_t)ss * M + w) * 16 : (size_t)w * Ks + ss * 16)) =
+                *reinterpret_cast<const v4u_mx*>(sc[threadIdx.x]);
 }
 
 // Values of the codes, rotated back (the rotation is its own inverse), rounded once to the output type.
@@ -89,59 +106,71 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
 }
 
 template <int DT, int G>
-static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, hipStream_t st) {
-    const long long units = (long long)M * (Kp / 16);
-    const dim3 grid((unsigned)((units + 255) / 256));
+static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int layout, hipStream_t st) {
     const auto xb = reinterpret_cast<const uint8_t*>(x);
     const auto cb = reinterpret_cast<uint8_t*>(codes);
     const auto sb = reinterpret_cast<uint8_t*>(scales);
-    if (Kp == K && Ks == K / 32) hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, false>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp, Ks);
-    else hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G, true>), grid, dim3(256), 0, st, xb, cb, sb, units, K, Kp, Ks);
+    const long long units = (long long)M * (K / 16);
+    const dim3 rows((unsigned)((M + 7LL) / 8 * (Ks / 16)));
+    if (layout == MX_PLAIN)
+        hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, xb, cb, sb, units);
+    else if (layout == MX_TILES)
+        hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, G, true>), rows, dim3(256), 0, st, xb, cb, sb, M, K, Kp, Ks);
+    else
+        hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, G, false>), rows, dim3(256), 0, st, xb, cb, sb, M, K, Kp, Ks);
 }
 
 template <int DT>
-static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, hipStream_t st) {
+static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, int layout,
+                        hipStream_t st) {
     switch (G) {
-        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, Ks, st);
-        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, Ks, st);
-        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, Ks, st);
-        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, Ks, st);
+        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, Ks, layout, st);
+        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, Ks, layout, st);
+        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, Ks, layout, st);
+        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, Ks, layout, st);
     }
 }
 
-// x [M, K] -> codes [M, Kp/2], scales [M, Ks]
-hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G,
+// x [M, K] -> codes and scales: MX_PLAIN the public form (Kp, Ks unused), MX_ROWS and MX_TILES a product's operand
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, int layout,
                               hipStream_t st) {
     if (M == 0) return hipSuccess;
     switch (dt) {
-        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, Ks, G, st); break;
-        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, Ks, G, st); break;
-        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, Ks, G, st); break;
+        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
+        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
+        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
     }
     return hipGetLastError();
 }
 
-// Scale rows of K/32 bytes -> rows of Ks (a multiple of 16), the padding 0: 16 bytes a thread.
-__global__ __launch_bounds__(256) void mxfp4_pad_scales_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
-                                                               long long pieces, int nb, int Ks) {
+// Scales [E, N, nb] -> [E, Ks/16, N, 16], 16 bytes a thread (piece i: 512 k number i / N % (Ks/16) of a row).
+__global__ __launch_bounds__(256) void mxfp4_tile_scales_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
+                                                                long long pieces, int N, int nb, int Ks) {
     const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
     if (i >= pieces) return;
-    const int per = Ks / 16;
-    const long long row = i / per;
-    const int b0 = (int)(i - row * per) * 16;
-    const uint8_t* s = src + (size_t)row * nb + b0;
+    const long long run = i / N;                           // e Ks/16 + 512 k number
+    const int n = (int)(i - run * N), per = Ks / 16;
+    const long long e = run / per;
+    const int b0 = (int)(run - e * per) * 16;
+    const uint8_t* s = src + (size_t)(e * N + n) * nb + b0;
     v4u_mx w = {0u, 0u, 0u, 0u};
+    if (nb % 16 == 0) {
+        const v4u_mx r = *reinterpret_cast<const v4u_mx*>(s);
 #pragma unroll
-    for (int j = 0; j < 16; ++j)
-        if (b0 + j < nb) w[j >> 2] |= (uint32_t)s[j] << (8 * (j & 3));
+        for (int j = 0; j < 16; ++j) w[mx_scale_place(j) >> 2] |= (r[j >> 2] >> (8 * (j & 3)) & 255u) << (8 * (mx_scale_place(j) & 3));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (b0 + j < nb) w[mx_scale_place(j) >> 2] |= (uint32_t)s[j] << (8 * (mx_scale_place(j) & 3));
+    }
     reinterpret_cast<v4u_mx*>(dst)[i] = w;
 }
 
-hipError_t mxfp4_pad_scales_launch(const void* src, void* dst, long long rows, int nb, int Ks, hipStream_t st) {
-    const long long pieces = rows * (Ks / 16);
+hipError_t mxfp4_tile_scales_launch(const void* src, void* dst, int E, int N, int nb, int Ks, hipStream_t st) {
+    const long long pieces = (long long)E * N * (Ks / 16);
     if (pieces == 0) return hipSuccess;
-    hipLaunchKernelGGL(mxfp4_pad_scales_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st,
-                       reinterpret_cast<const uint8_t*>(src), reinterpret_cast<uint8_t*>(dst), pieces, nb, Ks);
+    hipLaunchKernelGGL(mxfp4_tile_scales_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st,
+                       reinterpret_cast<const uint8_t*>(src), reinterpret_cast<uint8_t*>(dst), pieces, N, nb, Ks);
     return hipGetLastError();
 }
 
