@@ -53,7 +53,10 @@ hipError_t mxfp4_tile_scales_launch(const void* src, void* dst, int E, int N, in
 bool mxfp4_gemm_staged(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
-hipError_t mxfp4_gemm_launch(const MxProblem& p, hipStream_t st);
+hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st);
+bool mxfp4_gemm_fused(const MxProblem& p);
+hipError_t mxfp4_gemm_fused_launch(const MxProblem& p, const void* x, int G, hipStream_t st);
+hipError_t mxfp4_gemm_few_launch(const MxProblem& p, hipStream_t st);
 int expert_max();
 size_t expert_sort_bytes(int R, int E);
 hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R,
@@ -589,15 +592,15 @@ static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, v
     p.Ks = plan.Ks;
     p.as_rows = rows;
     p.wp = ws + plan.wscales;
+    if (convrot::mxfp4_gemm_fused(p)) return (int)convrot::mxfp4_gemm_fused_launch(p, x, G, st);
     const bool staged = convrot::mxfp4_gemm_staged(p);
     hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, p.Ks, G,
                                                staged ? convrot::MX_TILES : convrot::MX_ROWS, st);
     if (e != hipSuccess) return (int)e;
-    if (staged) {
-        e = convrot::mxfp4_tile_scales_launch(p.ws, ws + plan.wscales, p.E, p.N, p.K / convrot::MX_BLOCK, p.Ks, st);
-        if (e != hipSuccess) return (int)e;
-    }
-    return (int)convrot::mxfp4_gemm_launch(p, st);
+    if (!staged) return (int)convrot::mxfp4_gemm_few_launch(p, st);
+    e = convrot::mxfp4_tile_scales_launch(p.ws, ws + plan.wscales, p.E, p.N, p.K / convrot::MX_BLOCK, p.Ks, st);
+    if (e != hipSuccess) return (int)e;
+    return (int)convrot::mxfp4_gemm_staged_launch(p, st);
 }
 
 API size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E) {

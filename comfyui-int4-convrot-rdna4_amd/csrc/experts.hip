@@ -15,7 +15,7 @@
 namespace convrot {
 
 constexpr int SORT_THREADS = 256, SORT_WAVES = 4;
-constexpr int SORT_SLOTS = 4096;           // slots per workgroup
+constexpr int SORT_SLOTS = 2048;           // slots of a workgroup's run
 constexpr int SORT_MAX_E = 1024;
 
 template <typename ID>
@@ -43,34 +43,43 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_count_kernel(const ID* __
 
 // Workgroup b places its run: expert e's first row there is offsets[e] plus the
 // counts of the runs before.  Each wave takes a quarter of the run in order; the
-// lanes that go to one expert find each other by the bits of its number.
-template <typename ID>
+// lanes that go to one expert find each other by the bits of its number.  A
+// single run needs no counts from elsewhere (ONE): one launch.
+template <typename ID, bool ONE>
 __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __restrict__ ids,
                                                                     const int* __restrict__ counts, int* __restrict__ order,
                                                                     int* __restrict__ position, int* __restrict__ offsets,
                                                                     int R, int E, int runs) {
-    __shared__ int total[SORT_MAX_E], next[SORT_WAVES][SORT_MAX_E];
-    __shared__ int wave_sum[SORT_WAVES], used;
+    __shared__ int first_row[SORT_MAX_E], next[SORT_WAVES][SORT_MAX_E];
+    __shared__ int wave_sum[SORT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int s0 = blockIdx.x * SORT_SLOTS;
-    constexpr int SPAN = SORT_SLOTS / SORT_WAVES;
-    for (int e = tid; e < SORT_WAVES * SORT_MAX_E; e += SORT_THREADS) (&next[0][0])[e] = 0;
+    const int s0 = blockIdx.x * SORT_SLOTS, here = min(R - s0, SORT_SLOTS);
+    const int span = ((here + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;      // slots of a wave, whole wavefronts
+    const int w0 = s0 + wave * span, w1 = min(w0 + span, s0 + here);
+    for (int e = tid; e < E; e += SORT_THREADS)
+        for (int v = 0; v < SORT_WAVES; ++v) next[v][e] = 0;
     __syncthreads();
-    for (int i = lane; i < SPAN; i += 64) {
-        const int e = expert_of(ids, s0 + wave * SPAN + i, R, E);
-        if (e >= 0) atomicAdd(&next[wave][e], 1);
+    for (int s = w0 + lane; s < w1; s += 64) {
+        const int e = expert_of(ids, s, R, E);
+        if (e >= 0) atomicAdd(&next[wave][e], 1);          // integers: the order does not matter
     }
-    // totals of all runs, and of the runs before this one
-    int carry = 0;
+    __syncthreads();
+    int used = 0;
     for (int e0 = 0; e0 < E; e0 += SORT_THREADS) {
         const int e = e0 + tid;
-        int all = 0, before = 0;
-        if (e < E)
-            for (int b = 0; b < runs; ++b) {
-                const int c = counts[(size_t)b * E + e];
-                before += b < (int)blockIdx.x ? c : 0;
-                all += c;
+        int all = 0, before = 0;                           // of all runs, and of those before this one
+        if (e < E) {
+            if constexpr (ONE) {
+                for (int v = 0; v < SORT_WAVES; ++v) all += next[v][e];
+            } else {
+#pragma unroll 8
+                for (int b = 0; b < runs; ++b) {
+                    const int c = counts[(size_t)b * E + e];
+                    before += b < (int)blockIdx.x ? c : 0;
+                    all += c;
+                }
             }
+        }
         int sum = all;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -79,24 +88,21 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
         }
         if (lane == 63) wave_sum[wave] = sum;
         __syncthreads();
-        int first = carry + sum - all;
+        int first = used + sum - all;
         for (int v = 0; v < SORT_WAVES; ++v) {
             if (v < wave) first += wave_sum[v];
-            carry += wave_sum[v];
+            used += wave_sum[v];
         }
         if (e < E) {
             if (blockIdx.x == 0) offsets[e] = first;
-            total[e] = first + before;
+            first_row[e] = first + before;
         }
         __syncthreads();
     }
-    if (tid == 0) {
-        used = carry;
-        if (blockIdx.x == 0) offsets[E] = carry;
-    }
-    // each wave's first row of each expert
+    if (tid == 0 && blockIdx.x == 0) offsets[E] = used;
+    // each wave's first row of each expert (read by the threads that wrote first_row)
     for (int e = tid; e < E; e += SORT_THREADS) {
-        int at = total[e];
+        int at = first_row[e];
         for (int v = 0; v < SORT_WAVES; ++v) {
             const int c = next[v][e];
             next[v][e] = at;
@@ -104,9 +110,9 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
         }
     }
     __syncthreads();
-    for (int i = lane; i < SPAN; i += 64) {
-        const int s = s0 + wave * SPAN + i;
-        const int e = expert_of(ids, s, R, E);
+    for (int s1 = w0; s1 < w1; s1 += 64) {
+        const int s = s1 + lane;
+        const int e = s < w1 ? expert_of(ids, s, R, E) : -1;
         unsigned long long same = __ballot(e >= 0);
         for (int bit = 0; (E - 1) >> bit; ++bit) {
             const bool one = (e >> bit) & 1;
@@ -118,11 +124,11 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
         wave_sync();
         if (e >= 0 && (same >> lane) == 1ull) next[wave][e] = row + 1;      // the last of them
         wave_sync();
-        if (s < R) position[s] = row;
+        if (s < w1) position[s] = row;
         if (row >= 0) order[row] = s;
     }
-    for (int i = tid; i < SORT_SLOTS; i += SORT_THREADS)
-        if (s0 + i < R && s0 + i >= used) order[s0 + i] = -1;
+    for (int i = tid; i < here; i += SORT_THREADS)
+        if (s0 + i >= used) order[s0 + i] = -1;
 }
 
 // Rows by the plan (a row number outside it is taken for an unused slot).  A workgroup takes a token and its threads 16 bytes (or one
@@ -264,9 +270,14 @@ template <typename ID>
 static void sort_go(const void* ids, int* order, int* position, int* offsets, int* counts, int R, int E, hipStream_t st) {
     const int runs = R > 0 ? (R + SORT_SLOTS - 1) / SORT_SLOTS : 1;
     const ID* p = reinterpret_cast<const ID*>(ids);
+    if (runs == 1) {
+        hipLaunchKernelGGL((expert_place_kernel<ID, true>), dim3(1), dim3(SORT_THREADS), 0, st, p, counts, order, position,
+                           offsets, R, E, runs);
+        return;
+    }
     hipLaunchKernelGGL((expert_count_kernel<ID>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, R, E);
-    hipLaunchKernelGGL((expert_place_kernel<ID>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, order, position, offsets, R,
-                       E, runs);
+    hipLaunchKernelGGL((expert_place_kernel<ID, false>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, order, position,
+                       offsets, R, E, runs);
 }
 
 hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R, int E,

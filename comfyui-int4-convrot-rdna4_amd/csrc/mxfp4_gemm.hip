@@ -1,76 +1,303 @@
-// The product of MXFP4 rows with MXFP4 weights, for one weight matrix or one per expert.
+// The product of MXFP4 rows with MXFP4 weights where there are few rows: operands from
+// memory to registers, k split over the waves of a workgroup (mxfp4_gemm.h has the
+// operands; mxfp4_staged.hip the kernel for many rows).
 //
-// v_mfma_scale_f32_32x32x64_f8f6f4 multiplies 4-bit floats and applies both
-// operands' block scales itself: lane l supplies row l % 32, the 32 values of
-// block l / 32 of the 64 (16 bytes) and that block's scale byte.
+// v_mfma_scale_f32_16x16x128_f8f6f4 multiplies 4-bit floats and applies both operands'
+// block scales itself: lane l supplies row l % 16, the 32 values of block l / 16 of the
+// 128 (16 bytes) and that block's scale byte.  The weight's rows are its first operand,
+// so a lane's four results are neighbouring columns of one output row.
+//
+// Bound by the weight's bytes (a few rows) or by the copies of both operands from L2.
+// Eight waves share 16 NF columns by 16 MF rows, each a run of k, so that a CU has
+// some 100 KB of loads in flight and a grid of one row tile still fills the card; their
+// sums meet in LDS, added in wave order.  With FUSE the workgroup rotates and quantizes
+// its rows itself, while its first weights are on the way, which saves a launch and a
+// round trip of the codes.
 
+#include "gemm_common.h"
 #include "mxfp4_gemm.h"
 
 namespace convrot {
 
 typedef int v8i_mx __attribute__((ext_vector_type(8)));
-typedef float v16f_mx __attribute__((ext_vector_type(16)));
+typedef float v4f_mx __attribute__((ext_vector_type(4)));
 
-constexpr int MX_FP4 = 4;                  // operand format code of E2M1
+constexpr int FEW_WAVES = 8;
 
 __device__ __forceinline__ v8i_mx mx_operand(v4u_mx c) {
     return (v8i_mx){(int)c.x, (int)c.y, (int)c.z, (int)c.w, 0, 0, 0, 0};
 }
 
-// 64 x 64 outputs by four waves of 32 x 32, operands from memory to registers.
-__global__ __launch_bounds__(256) void mxfp4_gemm_direct_kernel(MxProblem p, int tiles_n) {
-    constexpr int BM = 64, BN = 64;
-    if ((int)(blockIdx.x / tiles_n) >= mx_tile_count<BM>(p)) return;
-    const MxTile t = mx_tile<BM>(p, blockIdx.x / tiles_n);
-    const int n0 = (blockIdx.x % tiles_n) * BN;
-    if (t.e == p.E && p.offsets != nullptr) return mx_zero(p, t.m0, t.m1, n0, min(n0 + BN, p.N));
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int r = t.m0 + (wave >> 1) * 32 + (lane & 31), half = lane >> 5;
-    const int n = n0 + (wave & 1) * 32 + (lane & 31);
-    // rows and columns past the edge repeat the last one; they are not stored
-    const size_t ar = (size_t)(p.order != nullptr ? mx_source_row(p, min(r, t.m1 - 1)) : min(r, t.m1 - 1));
-    const size_t wr = (size_t)t.e * p.N + min(n, p.N - 1);
-    const uint8_t* a = p.a + ar * (p.Kp / 2);
-    const uint8_t* as = p.as + ar * p.Ks;
-    const uint8_t* w = p.w + wr * (p.K / 2);
-    const uint8_t* ws = p.ws + wr * (p.K / 32);
-    v16f_mx acc = {0};
-    for (int k = 0; k < p.K; k += 64) {
-        const int b = k / 32 + half;                      // past K: the activation's padding (zero) against block b - 1
-        const int bw = min(b, p.K / 32 - 1);
-        const v4u_mx ca = *reinterpret_cast<const v4u_mx*>(a + (size_t)b * 16);
-        const v4u_mx cw = *reinterpret_cast<const v4u_mx*>(w + (size_t)bw * 16);
-        const int sw = b == bw ? ws[bw] : 127;
-        acc = __builtin_amdgcn_mfma_scale_f32_32x32x64_f8f6f4(mx_operand(cw), mx_operand(ca), acc, MX_FP4, MX_FP4, 0, sw, 0,
-                                                              (int)as[b]);
-    }
-    // lane: output row m = lane % 32, columns 8 (i / 4) + 4 half + i % 4
-    if (r >= t.m1) return;
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        const int c = n0 + (wave & 1) * 32 + 8 * g + 4 * half;
-        if (c >= p.N) continue;
-        float v[4];
-#pragma unroll
-        for (int j = 0; j < 4; ++j) {
-            v[j] = acc[4 * g + j];
-            if (p.bias != nullptr && c + j < p.N) v[j] += mx_read(p.bias, p.bias_dt, (size_t)t.e * p.N + c + j);
+// The 16 values of unit u (K / 16 of them a row) of the tile's rows
+template <int DT>
+__device__ __forceinline__ void few_load(const MxProblem& p, const uint8_t* x, const MxTile& t, int u, float (&v)[16]) {
+    const int per = p.K / 16, r = u / per, k = (u - r * per) * 16;
+    const size_t row = p.order != nullptr ? mx_source_row(p, t.m0 + r) : t.m0 + r;
+    load16<DT>(x + (row * p.K + k) * (DT == DT_F32 ? 4 : 2), v);
+}
+
+// The scale bytes of the tile's columns and rows in LDS, 16 bytes a thread: a byte a lane from memory instead costs a
+// third of the time (1 x 5120 -> 13824 12.6 us, 8.2 with none at all).
+__device__ __forceinline__ void few_copy16(const uint8_t* src, uint8_t* dst, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += 64 * FEW_WAVES * 16) {
+        if (i + 16 <= bytes) {
+            v4u_mx w;
+            __builtin_memcpy(&w, src + i, 16);             // any alignment
+            *reinterpret_cast<v4u_mx*>(dst + i) = w;
+        } else {
+            for (int j = i; j < bytes; ++j) dst[j] = src[j];
         }
-        mx_store4(p.out, p.dt, (size_t)r * p.N + c, v, min(4, p.N - c), p.N % 4 == 0);
     }
 }
 
-bool mxfp4_gemm_staged(const MxProblem& p);
-hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st);
+constexpr int few_pad(int bytes) { return (bytes + 15) & ~15; }
 
-hipError_t mxfp4_gemm_launch(const MxProblem& p, hipStream_t st) {
-    if (p.R == 0 || p.N == 0) return hipSuccess;
-    if (mxfp4_gemm_staged(p)) return mxfp4_gemm_staged_launch(p, st);
-    const int tiles_n = (p.N + 63) / 64;
-    const long long grid = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 64) * tiles_n;
+// Widest rows whose scales are held in LDS; past it they are read from memory.
+constexpr int FEW_MAX_K = 32768;
+
+// DT, G: of x, with FUSE.
+template <int DT, int G, int MF, int NF, bool FUSE>
+__global__ __launch_bounds__(64 * FEW_WAVES) void mxfp4_gemm_few_kernel(MxProblem p, const uint8_t* __restrict__ x) {
+    constexpr int BM = 16 * MF, BN = 16 * NF, THREADS = 64 * FEW_WAVES;
+    extern __shared__ __attribute__((aligned(16))) uint8_t lds_few[];
+    const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
+    const int tiles_m = mx_tile_count<BM>(p), tiles_n = (p.N + BN - 1) / BN;
+    if ((int)blockIdx.x >= tiles_m * tiles_n) return;
+    int tm, tn;
+    tile_of_block(blockIdx.x, tiles_m, tiles_n, tiles_m, tm, tn);   // an XCD's row tiles of the same columns together
+    const MxTile t = mx_tile<BM>(p, tm);
+    const int n0 = tn * BN;
+    if (t.e == p.E && p.offsets != nullptr) return mx_zero(p, t.m0, t.m1, n0, min(n0 + BN, p.N));
+    const int rows = t.m1 - t.m0;
+
+    // x first: its values are needed before the weight's, and loads come back in order
+    float v[16];
+    const int units = rows * (p.K / 16);
+    if constexpr (FUSE) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+        if (tid < units) few_load<DT>(p, x, t, tid, v);
+    }
+
+    // Steps of 128 k; this wave's are pairs (whole lines) of them, first .. last - 1.
+    const int l16 = lane & 15, g = lane >> 4;
+    const int nb = p.K / 32, steps = (p.K + 127) / 128, pairs = (steps + 1) / 2;
+    const int first = wave * pairs / FEW_WAVES, last = (wave + 1) * pairs / FEW_WAVES;
+    const uint8_t *w[NF], *ws[NF], *a[MF], *as[MF];
+#pragma unroll
+    for (int j = 0; j < NF; ++j) {                         // columns and rows past the edge repeat the last
+        const size_t r = (size_t)t.e * p.N + min(n0 + j * 16 + l16, p.N - 1);
+        w[j] = p.w + r * (p.K / 2);
+        ws[j] = p.ws + r * nb;
+    }
+    // LDS: the columns' scales [BN, nb], the rows' scales [rows, srow], with FUSE the rows' codes [rows, stride]
+    const bool near = p.K <= FEW_MAX_K;
+    const int stride = p.Kp / 2, srow = FUSE ? p.Kp / 32 : p.Ks;
+    uint8_t* lds_ws = lds_few;
+    uint8_t* lds_s = lds_few + few_pad(BN * nb);
+    uint8_t* lds_c = lds_s + few_pad(rows * srow);
+    int lrow[MF];
+#pragma unroll
+    for (int i = 0; i < MF; ++i) {
+        lrow[i] = min(i * 16 + l16, rows - 1);
+        if constexpr (!FUSE) {
+            const size_t r = p.order != nullptr ? mx_source_row(p, t.m0 + lrow[i]) : t.m0 + lrow[i];
+            a[i] = p.a + r * stride;
+            as[i] = p.as + r * p.Ks;
+        }
+    }
+    struct Step { v4u_mx w[NF], a[MF]; };                  // codes of block 4 st + g
+    auto load_w = [&](Step& s, int st) __attribute__((always_inline)) {
+        const int blk = st * 4 + g;
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            s.w[j] = *reinterpret_cast<const v4u_mx*>(w[j] + (size_t)min(blk, nb - 1) * 16);   // past K: times codes 0
+        }
+    };
+    auto load_a = [&](Step& s, int st) __attribute__((always_inline)) {
+        const int blk = st * 4 + g;
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            if constexpr (FUSE) {
+                s.a[i] = *reinterpret_cast<const v4u_mx*>(lds_c + lrow[i] * stride + blk * 16);
+            } else {
+                s.a[i] = *reinterpret_cast<const v4u_mx*>(a[i] + (size_t)blk * 16);
+            }
+        }
+    };
+    Step s[2][2];
+    if (first < last) {
+        load_w(s[0][0], 2 * first);
+        if (2 * first + 1 < steps) load_w(s[0][1], 2 * first + 1);
+        if constexpr (!FUSE) {
+            load_a(s[0][0], 2 * first);
+            if (2 * first + 1 < steps) load_a(s[0][1], 2 * first + 1);
+        }
+    }
+    if constexpr (FUSE) {
+        for (int u = tid; u < units; u += THREADS) {           // whole blocks and groups: no lane of one is missing
+            if (u >= THREADS) {
+#pragma unroll
+                for (int i = 0; i < 16; ++i) v[i] = 0.0f;
+                if (u < units) few_load<DT>(p, x, t, u, v);
+            }
+            rotate16<G>(v);
+            uint32_t sb;
+            const v2u_mx c = mx_encode16(v, sb);
+            const int per = p.K / 16, r = u / per, k16 = u - r * per;
+            if (u < units) {
+                *reinterpret_cast<v2u_mx*>(lds_c + r * stride + k16 * 8) = c;
+                if ((k16 & 1) == 0) lds_s[r * srow + k16 / 2] = (uint8_t)sb;
+            }
+        }
+        const int pad = (p.Kp - p.K) / 32;                 // blocks of zeros behind each row
+        for (int i = tid; i < rows * pad; i += THREADS) {
+            const int r = i / pad, blk = nb + i - r * pad;
+            *reinterpret_cast<v4u_mx*>(lds_c + r * stride + blk * 16) = (v4u_mx){0u, 0u, 0u, 0u};
+            lds_s[r * srow + blk] = 0;
+        }
+    } else if (near) {
+        const int per = srow / 16;
+        for (int i = tid; i < rows * per; i += THREADS) {
+            const int r = i / per;
+            const size_t row = p.order != nullptr ? mx_source_row(p, t.m0 + r) : t.m0 + r;
+            reinterpret_cast<v4u_mx*>(lds_s)[i] = reinterpret_cast<const v4u_mx*>(p.as + row * srow)[i - r * per];
+        }
+    }
+    const int cols = min(BN, p.N - n0);
+    if (near) few_copy16(p.ws + ((size_t)t.e * p.N + n0) * nb, lds_ws, cols * nb);
+    __syncthreads();
+
+    v4f_mx acc[NF][MF];
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int i = 0; i < MF; ++i) acc[j][i] = (v4f_mx){0.0f, 0.0f, 0.0f, 0.0f};
+    auto multiply = [&](Step& s, int st) __attribute__((always_inline)) {
+        if constexpr (FUSE) load_a(s, st);
+        const int blk = st * 4 + g, bw = min(blk, nb - 1);
+        int sw[NF], sa[MF];
+#pragma unroll
+        for (int j = 0; j < NF; ++j) {
+            sw[j] = near ? lds_ws[min(j * 16 + l16, cols - 1) * nb + bw] : ws[j][bw];
+            if (blk >= nb) sw[j] = 127;                    // past K: the last scale may be NaN
+        }
+#pragma unroll
+        for (int i = 0; i < MF; ++i) {
+            if constexpr (FUSE) sa[i] = lds_s[lrow[i] * srow + blk];
+            else sa[i] = near ? lds_s[lrow[i] * srow + blk] : as[i][blk];
+        }
+#pragma unroll
+        for (int j = 0; j < NF; ++j)
+#pragma unroll
+            for (int i = 0; i < MF; ++i)
+                acc[j][i] = __builtin_amdgcn_mfma_scale_f32_16x16x128_f8f6f4(mx_operand(s.w[j]), mx_operand(s.a[i]), acc[j][i],
+                                                                             4, 4, 0, sw[j], 0, sa[i]);
+    };
+    auto pair = [&](int pr, int q) __attribute__((always_inline)) {
+        if (pr + 1 < last) {
+#pragma unroll
+            for (int h = 0; h < 2; ++h)
+                if (2 * pr + 2 + h < steps) {
+                    load_w(s[1 - q][h], 2 * pr + 2 + h);
+                    if constexpr (!FUSE) load_a(s[1 - q][h], 2 * pr + 2 + h);
+                }
+        }
+        multiply(s[q][0], 2 * pr);
+        if (2 * pr + 1 < steps) multiply(s[q][1], 2 * pr + 1);
+    };
+    for (int pr = first; pr < last; pr += 2) {
+        pair(pr, 0);
+        if (pr + 1 < last) pair(pr + 1, 1);
+    }
+
+    // the waves' sums, added in wave order
+    __syncthreads();                                       // no wave reads codes or scales any more
+    float4* part = reinterpret_cast<float4*>(lds_few);
+    constexpr int Q = NF * MF * 64;                        // groups of four columns
+#pragma unroll
+    for (int j = 0; j < NF; ++j)
+#pragma unroll
+        for (int i = 0; i < MF; ++i)
+            part[wave * Q + (j * MF + i) * 64 + lane] = make_float4(acc[j][i][0], acc[j][i][1], acc[j][i][2], acc[j][i][3]);
+    __syncthreads();
+    for (int q = tid; q < Q; q += THREADS) {
+        float4 o = part[q];
+#pragma unroll
+        for (int k = 1; k < FEW_WAVES; ++k) {
+            const float4 b = part[k * Q + q];
+            o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
+        }
+        const int f = q >> 6, l = q & 63;
+        const int m = t.m0 + f % MF * 16 + (l & 15), n = n0 + f / MF * 16 + (l >> 4) * 4;
+        if (m >= t.m1 || n >= p.N) continue;
+        float r[4] = {o.x, o.y, o.z, o.w};
+        if (p.bias != nullptr) {
+#pragma unroll
+            for (int j = 0; j < 4; ++j)
+                if (n + j < p.N) r[j] += mx_read(p.bias, p.bias_dt, (size_t)t.e * p.N + n + j);
+        }
+        mx_store4(p.out, p.dt, (size_t)m * p.N + n, r, min(4, p.N - n), p.N % 4 == 0);
+    }
+}
+
+template <int DT, int G, int MF, int NF, bool FUSE>
+static hipError_t few_go(const MxProblem& p, const void* x, hipStream_t st) {
+    static std::atomic<bool> attr[kMaxDev];
+    const long long grid = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 16 * MF) * ((p.N + 16 * NF - 1) / (16 * NF));
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL(mxfp4_gemm_direct_kernel, dim3((unsigned)grid), dim3(256), 0, st, p, tiles_n);
+    const int sums = FEW_WAVES * NF * MF * 1024;
+    const int rows = p.R < 16 * MF ? p.R : 16 * MF;
+    const int nb = p.K / 32;
+    const int held = p.K > FEW_MAX_K ? 0 : few_pad(16 * NF * nb) + few_pad(rows * (FUSE ? p.Kp / 32 : p.Ks)) + (FUSE ? rows * p.Kp / 2 : 0);
+    const int lds = held > sums ? held : sums;
+    int dev = 0;
+    hipError_t e = current_device(&dev);
+    if (e != hipSuccess) return e;
+    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&mxfp4_gemm_few_kernel<DT, G, MF, NF, FUSE>), 160 << 10);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((mxfp4_gemm_few_kernel<DT, G, MF, NF, FUSE>), dim3((unsigned)grid), dim3(64 * FEW_WAVES), lds, st, p,
+                       reinterpret_cast<const uint8_t*>(x));
     return hipGetLastError();
+}
+
+// Rows that each workgroup quantizes itself: their values are few, and their codes fit its LDS.
+bool mxfp4_gemm_fused(const MxProblem& p) {
+    const long long values = (long long)(p.R < 16 ? p.R : 16) * p.Kp;
+    return p.R <= 8 && p.K <= FEW_MAX_K && values <= (64 << 10);
+}
+
+template <int DT, int G>
+static hipError_t fused_go(const MxProblem& p, const void* x, hipStream_t st) {
+    const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 16) * ((p.N + 31) / 32);
+    return tiles >= 256 ? few_go<DT, G, 1, 2, true>(p, x, st) : few_go<DT, G, 1, 1, true>(p, x, st);
+}
+
+template <int DT>
+static hipError_t fused_group(const MxProblem& p, const void* x, int G, hipStream_t st) {
+    switch (G) {
+        case 0: return fused_go<DT, 0>(p, x, st);
+        case 16: return fused_go<DT, 16>(p, x, st);
+        case 64: return fused_go<DT, 64>(p, x, st);
+        default: return fused_go<DT, 256>(p, x, st);
+    }
+}
+
+// x as it came, where mxfp4_gemm_fused says so
+hipError_t mxfp4_gemm_fused_launch(const MxProblem& p, const void* x, int G, hipStream_t st) {
+    switch (p.dt) {
+        case DT_F32: return fused_group<DT_F32>(p, x, G, st);
+        case DT_BF16: return fused_group<DT_BF16>(p, x, G, st);
+        default: return fused_group<DT_F16>(p, x, G, st);
+    }
+}
+
+// x quantized with scales in rows.  Row tiles as high as an expert's rows are many on average.
+hipError_t mxfp4_gemm_few_launch(const MxProblem& p, hipStream_t st) {
+    const int rows = p.offsets != nullptr ? (p.R + p.E - 1) / p.E : p.R;
+    if (rows <= (p.offsets != nullptr ? 8 : 16)) return few_go<0, 0, 1, 2, false>(p, nullptr, st);
+    if (rows <= (p.offsets != nullptr ? 24 : 32)) return few_go<0, 0, 2, 2, false>(p, nullptr, st);
+    return few_go<0, 0, 4, 2, false>(p, nullptr, st);
 }
 
 }  // namespace convrot
