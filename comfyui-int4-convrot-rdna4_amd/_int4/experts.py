@@ -54,6 +54,11 @@ def max_experts() -> int:
 def sort_tokens_by_expert(expert_ids: torch.Tensor, num_experts: int) -> ExpertPlan:
     """The plan of expert_ids [T, k] (int32 or int64): a stable counting sort of the
     slots by expert, without a host synchronization."""
+    if expert_ids.is_cuda:
+        host = native.host_or_none()
+        p = None if host is None else host.expert_sort(expert_ids, num_experts)
+        if p is not None:
+            return ExpertPlan(*p)
     if expert_ids.dim() != 2 or expert_ids.shape[1] < 1:
         raise ValueError(f"expert_ids must be [T, k], got shape {tuple(expert_ids.shape)}")
     if expert_ids.dtype not in (torch.int32, torch.int64):
@@ -158,6 +163,11 @@ def gather_expert_rows(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     """x [T, D] -> rows [T k, D] in the plan's order (row r is token order[r] // k);
     rows past the last used one are zero.  Differentiable: a token's gradient is
     the sum of its rows', in fp32, rounded once."""
+    if x.is_cuda:
+        host = native.host_or_none()
+        rows = None if host is None else host.expert_gather(x, plan.order, plan.position, plan.offsets)
+        if rows is not None:
+            return rows
     _check_dtype(x, "x")
     plan.check()
     if x.dim() != 2 or x.shape[0] != plan.position.shape[0]:
@@ -173,6 +183,11 @@ def combine_expert_rows(rows: torch.Tensor, weights: torch.Tensor, plan: ExpertP
     rows [T k, D] in the plan's order, weights [T, k] of any of the three types,
     out [T, D] in the rows' type, summed in fp32 and rounded once.  A token without
     a used slot gets zeros.  Differentiable in the rows and the weights."""
+    if rows.is_cuda:
+        host = native.host_or_none()
+        out = None if host is None else host.expert_combine(rows, weights, plan.order, plan.position, plan.offsets)
+        if out is not None:
+            return out
     _check_dtype(rows, "rows")
     _check_dtype(weights, "weights")
     plan.check()

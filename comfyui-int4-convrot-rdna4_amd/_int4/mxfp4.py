@@ -60,6 +60,11 @@ def quantize_mxfp4(x: torch.Tensor, convrot_groupsize: int | None = None) -> tup
     the scale is 2^(floor(log2 max) - 2), not below 2^-127, and the codes are the
     nearest E2M1 values of y / scale, ties to even, magnitudes past 6 to 6.  A
     block that holds a NaN or an infinity is NaN as a whole (scale byte 255)."""
+    if x.is_cuda:
+        host = native.host_or_none()
+        q = None if host is None else host.mx_quantize(x, convrot_groupsize)
+        if q is not None:
+            return q
     dt = _check_dtype(x, "x")
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -85,6 +90,12 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, convrot_groupsiz
     """The values of codes [..., K/2] with scales [..., K/32], rotated back to the
     original basis where a group size is given: [..., K] in ``output_dtype``,
     rounded once, on the codes' device."""
+    if codes.is_cuda and output_dtype in native._IN_DTYPE_CODE:
+        host = native.host_or_none()
+        x = None if host is None else host.mx_dequantize(codes, scales, convrot_groupsize,
+                                                         native._IN_DTYPE_CODE[output_dtype])
+        if x is not None:
+            return x
     if output_dtype not in native._IN_DTYPE_CODE:
         raise ValueError(f"output_dtype must be float32, bfloat16 or float16, got {output_dtype}")
     _check_operand(codes, scales, codes.shape[:-1], codes.shape[-1] * 2 if codes.dim() else 0, "codes")
@@ -110,6 +121,11 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     qweight uint8 [N, K/2], wscales uint8 [N, K/32].  Products and sums in fp32;
     the output [..., N] has x's type and is rounded once.  bias [N] is float32,
     bfloat16 or float16."""
+    if x.is_cuda:
+        host = native.host_or_none()
+        y = None if host is None else host.mx_linear(x, qweight, wscales, bias, convrot_groupsize)
+        if y is not None:
+            return y
     dt = _check_dtype(x, "x")
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -153,6 +169,12 @@ def mxfp4_expert_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.T
     ``sorted_rows``, the T k rows [T k, K] already in the plan's order.  Row r of
     the output is x_r W_e^T + bias[e] for its expert e; rows past the last used
     one are zero.  Types and rounding as in :func:`mxfp4_linear`; bias is [E, N]."""
+    if x.is_cuda:
+        host = native.host_or_none()
+        y = None if host is None else host.mx_expert_linear(x, qweight, wscales, plan.order, plan.position, plan.offsets,
+                                                            bias, convrot_groupsize, sorted_rows)
+        if y is not None:
+            return y
     dt = _check_dtype(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be 2-D, got shape {tuple(x.shape)}")

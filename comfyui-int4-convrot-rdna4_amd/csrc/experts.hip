@@ -15,14 +15,22 @@
 namespace convrot {
 
 constexpr int SORT_THREADS = 256, SORT_WAVES = 4;
-constexpr int SORT_SLOTS = 2048;           // slots of a workgroup's run
+constexpr int SORT_EACH = 8;               // slots of a lane
+constexpr int SORT_SLOTS = 64 * SORT_EACH * SORT_WAVES;     // slots of a workgroup's run
 constexpr int SORT_MAX_E = 1024;
 
+// The experts of a wave's slots w0 + 64 i + lane (-1: none), loaded together.
 template <typename ID>
-__device__ __forceinline__ int expert_of(const ID* ids, int s, int R, int E) {
-    if (s >= R) return -1;
-    const ID id = ids[s];
-    return id >= 0 && id < (ID)E ? (int)id : -1;
+__device__ __forceinline__ void experts_of(const ID* ids, int w0, int R, int E, int (&e)[SORT_EACH]) {
+    ID id[SORT_EACH];
+    const int lane = threadIdx.x & 63;
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i) {
+        const long long s = (long long)w0 + 64 * i + lane;
+        id[i] = s < R ? ids[s] : (ID)-1;
+    }
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i) e[i] = id[i] >= 0 && id[i] < (ID)E ? (int)id[i] : -1;
 }
 
 // counts[b, e]: slots of workgroup b's run that go to expert e
@@ -30,51 +38,68 @@ template <typename ID>
 __global__ __launch_bounds__(SORT_THREADS) void expert_count_kernel(const ID* __restrict__ ids, int* __restrict__ counts,
                                                                     int R, int E) {
     __shared__ int n[SORT_MAX_E];
-    for (int e = threadIdx.x; e < E; e += SORT_THREADS) n[e] = 0;
+    int e[SORT_EACH];
+    experts_of(ids, blockIdx.x * SORT_SLOTS + (threadIdx.x >> 6) * (SORT_SLOTS / SORT_WAVES), R, E, e);
+    for (int i = threadIdx.x; i < E; i += SORT_THREADS) n[i] = 0;
     __syncthreads();
-    const int s0 = blockIdx.x * SORT_SLOTS;
-    for (int i = threadIdx.x; i < SORT_SLOTS && s0 + i < R; i += SORT_THREADS) {
-        const int e = expert_of(ids, s0 + i, R, E);
-        if (e >= 0) atomicAdd(&n[e], 1);                   // integers: the order does not matter
-    }
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i)
+        if (e[i] >= 0) atomicAdd(&n[e[i]], 1);             // integers: the order does not matter
     __syncthreads();
-    for (int e = threadIdx.x; e < E; e += SORT_THREADS) counts[(size_t)blockIdx.x * E + e] = n[e];
+    for (int i = threadIdx.x; i < E; i += SORT_THREADS) counts[(size_t)blockIdx.x * E + i] = n[i];
 }
 
 // Workgroup b places its run: expert e's first row there is offsets[e] plus the
-// counts of the runs before.  Each wave takes a quarter of the run in order; the
-// lanes that go to one expert find each other by the bits of its number.  A
-// single run needs no counts from elsewhere (ONE): one launch.
+// counts of the runs before.  Each wave takes a quarter of the run, in order, 64
+// slots at a time; the lanes that go to one expert find each other by the bits of
+// its number, so that one of them counts for all, and their order is the slots'.
+// A single run needs no counts from elsewhere (ONE): one launch.  A few slots take
+// 2.6 us, 2000 of 32 experts 4, bound by the chain of loads, ballots and LDS.
 template <typename ID, bool ONE>
 __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __restrict__ ids,
                                                                     const int* __restrict__ counts, int* __restrict__ order,
                                                                     int* __restrict__ position, int* __restrict__ offsets,
                                                                     int R, int E, int runs) {
-    __shared__ int first_row[SORT_MAX_E], next[SORT_WAVES][SORT_MAX_E];
+    __shared__ int next[SORT_WAVES][SORT_MAX_E];
     __shared__ int wave_sum[SORT_WAVES];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int s0 = blockIdx.x * SORT_SLOTS, here = min(R - s0, SORT_SLOTS);
-    const int span = ((here + SORT_WAVES - 1) / SORT_WAVES + 63) / 64 * 64;      // slots of a wave, whole wavefronts
-    const int w0 = s0 + wave * span, w1 = min(w0 + span, s0 + here);
-    for (int e = tid; e < E; e += SORT_THREADS)
-        for (int v = 0; v < SORT_WAVES; ++v) next[v][e] = 0;
+    const int w0 = s0 + wave * (SORT_SLOTS / SORT_WAVES);
+    int e[SORT_EACH], rank[SORT_EACH], many[SORT_EACH];    // lanes of the same expert before this one; all, of the last
+    experts_of(ids, w0, R, E, e);
+    for (int i = tid; i < E; i += SORT_THREADS)
+        for (int v = 0; v < SORT_WAVES; ++v) next[v][i] = 0;
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i) {
+        if (w0 + 64 * i >= R) break;                       // nothing past here
+        unsigned long long same = __ballot(e[i] >= 0);
+        for (int bit = 0; (E - 1) >> bit; ++bit) {
+            const bool one = (e[i] >> bit) & 1;
+            const unsigned long long m = __ballot(one);
+            same &= one ? m : ~m;
+        }
+        rank[i] = __popcll(same & ((1ull << lane) - 1));
+        many[i] = e[i] >= 0 && (same >> lane) == 1ull ? rank[i] + 1 : 0;
+    }
     __syncthreads();
-    for (int s = w0 + lane; s < w1; s += 64) {
-        const int e = expert_of(ids, s, R, E);
-        if (e >= 0) atomicAdd(&next[wave][e], 1);          // integers: the order does not matter
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i) {
+        if (w0 + 64 * i >= R) break;
+        if (many[i]) next[wave][e[i]] += many[i];          // one lane an expert
+        wave_sync();
     }
     __syncthreads();
     int used = 0;
     for (int e0 = 0; e0 < E; e0 += SORT_THREADS) {
-        const int e = e0 + tid;
+        const int x = e0 + tid;
         int all = 0, before = 0;                           // of all runs, and of those before this one
-        if (e < E) {
+        if (x < E) {
             if constexpr (ONE) {
-                for (int v = 0; v < SORT_WAVES; ++v) all += next[v][e];
+                for (int v = 0; v < SORT_WAVES; ++v) all += next[v][x];
             } else {
 #pragma unroll 8
                 for (int b = 0; b < runs; ++b) {
-                    const int c = counts[(size_t)b * E + e];
+                    const int c = counts[(size_t)b * E + x];
                     before += b < (int)blockIdx.x ? c : 0;
                     all += c;
                 }
@@ -93,38 +118,28 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
             if (v < wave) first += wave_sum[v];
             used += wave_sum[v];
         }
-        if (e < E) {
-            if (blockIdx.x == 0) offsets[e] = first;
-            first_row[e] = first + before;
+        if (x < E) {
+            if (blockIdx.x == 0) offsets[x] = first;
+            int at = first + before;                       // each wave's first row of the expert
+            for (int v = 0; v < SORT_WAVES; ++v) {
+                const int c = next[v][x];
+                next[v][x] = at;
+                at += c;
+            }
         }
         __syncthreads();
     }
     if (tid == 0 && blockIdx.x == 0) offsets[E] = used;
-    // each wave's first row of each expert (read by the threads that wrote first_row)
-    for (int e = tid; e < E; e += SORT_THREADS) {
-        int at = first_row[e];
-        for (int v = 0; v < SORT_WAVES; ++v) {
-            const int c = next[v][e];
-            next[v][e] = at;
-            at += c;
-        }
-    }
-    __syncthreads();
-    for (int s1 = w0; s1 < w1; s1 += 64) {
-        const int s = s1 + lane;
-        const int e = s < w1 ? expert_of(ids, s, R, E) : -1;
-        unsigned long long same = __ballot(e >= 0);
-        for (int bit = 0; (E - 1) >> bit; ++bit) {
-            const bool one = (e >> bit) & 1;
-            const unsigned long long m = __ballot(one);
-            same &= one ? m : ~m;
-        }
+#pragma unroll
+    for (int i = 0; i < SORT_EACH; ++i) {
+        if (w0 + 64 * i >= R) break;
+        const int s = w0 + 64 * i + lane;
         int row = -1;
-        if (e >= 0) row = next[wave][e] + __popcll(same & ((1ull << lane) - 1));
+        if (e[i] >= 0) row = next[wave][e[i]] + rank[i];
         wave_sync();
-        if (e >= 0 && (same >> lane) == 1ull) next[wave][e] = row + 1;      // the last of them
+        if (many[i]) next[wave][e[i]] = row + 1;           // the last of them
         wave_sync();
-        if (s < w1) position[s] = row;
+        if (s < R) position[s] = row;
         if (row >= 0) order[row] = s;
     }
     for (int i = tid; i < here; i += SORT_THREADS)

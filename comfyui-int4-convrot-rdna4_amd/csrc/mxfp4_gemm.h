@@ -122,13 +122,18 @@ __device__ __forceinline__ int mx_source_row(const MxProblem& p, int r) {
     return (int)((unsigned long long)slot * p.k_mul >> p.k_shift);
 }
 
-// Zeros in rows m0 .. m1 - 1, columns n0 .. n1 - 1 (threads of a workgroup).
+// Zeros in rows m0 .. m1 - 1, columns n0 .. n1 - 1 (n0 a multiple of 16), by the threads of a workgroup: a wave a row at a
+// time, 16 bytes a lane where rows are whole pieces of that.
 __device__ __forceinline__ void mx_zero(const MxProblem& p, int m0, int m1, int n0, int n1) {
-    const int n = n1 - n0;
-    for (long long i = threadIdx.x; i < (long long)(m1 - m0) * n; i += blockDim.x) {
-        const size_t o = (size_t)(m0 + i / n) * p.N + n0 + i % n;
-        if (p.dt == DT_F32) reinterpret_cast<float*>(p.out)[o] = 0.0f;
-        else reinterpret_cast<uint16_t*>(p.out)[o] = 0;
+    const int es = p.dt == DT_F32 ? 4 : 2, lane = threadIdx.x & 63;
+    for (int m = m0 + (threadIdx.x >> 6); m < m1; m += blockDim.x >> 6) {
+        uint8_t* row = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + n0) * es;
+        const int bytes = (n1 - n0) * es;
+        if ((size_t)p.N * es % 16 == 0) {
+            for (int i = lane * 16; i < bytes; i += 1024) *reinterpret_cast<v4u_mx*>(row + i) = (v4u_mx){0u, 0u, 0u, 0u};
+        } else {
+            for (int i = lane * 2; i < bytes; i += 128) *reinterpret_cast<uint16_t*>(row + i) = 0;
+        }
     }
 }
 
