@@ -47,9 +47,8 @@ hipError_t dequant_launch(const void* q, int bits, const float* s, void* out, in
                           hipStream_t st);
 hipError_t gemm_splitk_launch(const int8_t* Xp, const int8_t* Wp, const float* xs, const float* ws, float* accum,
                               int M, int N, int K, int nsplit, hipStream_t st);
-hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G,
-                              int layout, hipStream_t st);
-hipError_t mxfp4_tile_scales_launch(const void* src, void* dst, int E, int N, int nb, int Ks, hipStream_t st);
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int G, hipStream_t st);
+hipError_t mxfp4_operands_launch(const void* x, int G, const MxProblem& p, bool tiles, hipStream_t st);
 bool mxfp4_gemm_staged(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
@@ -555,8 +554,7 @@ static int mx_args_ok(int dtype, int M, int K, int G) {
 
 API int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream) {
     if (!mx_args_ok(in_dtype, M, K, G)) return -1;
-    return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, K, K / convrot::MX_BLOCK, G,
-                                            convrot::MX_PLAIN, reinterpret_cast<hipStream_t>(stream));
+    return (int)convrot::mxfp4_quant_launch(x, in_dtype, codes, scales, M, K, G, reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
@@ -594,13 +592,9 @@ static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, v
     p.wp = ws + plan.wscales;
     if (convrot::mxfp4_gemm_fused(p)) return (int)convrot::mxfp4_gemm_fused_launch(p, x, G, st);
     const bool staged = convrot::mxfp4_gemm_staged(p);
-    hipError_t e = convrot::mxfp4_quant_launch(x, p.dt, ws + plan.codes, ws + plan.scales, rows, p.K, p.Kp, p.Ks, G,
-                                               staged ? convrot::MX_TILES : convrot::MX_ROWS, st);
+    const hipError_t e = convrot::mxfp4_operands_launch(x, G, p, staged, st);
     if (e != hipSuccess) return (int)e;
-    if (!staged) return (int)convrot::mxfp4_gemm_few_launch(p, st);
-    e = convrot::mxfp4_tile_scales_launch(p.ws, ws + plan.wscales, p.E, p.N, p.K / convrot::MX_BLOCK, p.Ks, st);
-    if (e != hipSuccess) return (int)e;
-    return (int)convrot::mxfp4_gemm_staged_launch(p, st);
+    return (int)(staged ? convrot::mxfp4_gemm_staged_launch(p, st) : convrot::mxfp4_gemm_few_launch(p, st));
 }
 
 API size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E) {

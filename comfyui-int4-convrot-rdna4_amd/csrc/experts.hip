@@ -146,8 +146,8 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
         if (s0 + i >= used) order[s0 + i] = -1;
 }
 
-// Rows by the plan (a row number outside it is taken for an unused slot).  A workgroup takes a token and its threads 16 bytes (or one
-// element) of the row each.
+// Rows by the plan (a row number outside it is taken for an unused slot), 16
+// bytes or one element of a row a thread.
 template <int DT>
 struct RowVec {                              // 16 bytes of a row as floats
     static constexpr int N = DT == DT_F32 ? 4 : 8;
@@ -201,77 +201,115 @@ __device__ __forceinline__ void zero_tail(uint8_t* rows, const int* offsets, int
         for (int i = threadIdx.x; i < D / P::N; i += blockDim.x) P::store(rows + (size_t)r * D * P::ES, i, z);
 }
 
+// A workgroup takes 256 pieces of one token's row; a token's slots are read four at a time, their rows together.
+constexpr int ROW_SLOTS = 4;
+
+// Rows position[t, j0 .. j0 + 3] (-1: none) and with W their weights
+__device__ __forceinline__ void slots_of(const int* position, const float* w, long long t, int j0, int k, int R, int (&r)[ROW_SLOTS],
+                                         float (&f)[ROW_SLOTS]) {
+#pragma unroll
+    for (int j = 0; j < ROW_SLOTS; ++j) {
+        const bool there = j0 + j < k;
+        const int p = there ? position[t * k + j0 + j] : -1;
+        r[j] = (unsigned)p < (unsigned)R ? p : -1;
+        f[j] = there && w != nullptr ? w[t * k + j0 + j] : 1.0f;
+    }
+}
+
 // gathered[position[t, j]] = x[t]
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_gather_kernel(const uint8_t* __restrict__ x, const int* __restrict__ position,
                                                             const int* __restrict__ offsets, uint8_t* __restrict__ rows, int R,
-                                                            int k, int E, int D) {
+                                                            int k, int E, int D, int parts) {
     using P = Piece<DT, VEC>;
-    const int t = blockIdx.x;
-    for (int i = threadIdx.x; i < D / P::N; i += 256) {
+    const long long t = blockIdx.x / parts;
+    const int i = (blockIdx.x % parts) * 256 + threadIdx.x;
+    if (i < D / P::N) {
         float v[P::N];
         P::load(x + (size_t)t * D * P::ES, i, v);
         for (int j = 0; j < k; ++j) {
-            const int r = position[(size_t)t * k + j];
+            const int r = position[t * k + j];
             if ((unsigned)r < (unsigned)R) P::store(rows + (size_t)r * D * P::ES, i, v);
         }
     }
     zero_tail<DT, VEC>(rows, offsets, R, E, D);
 }
 
-// out[t] = sum_j w[t, j] rows[position[t, j]] (w NULL: 1)
+// out[t] = sum_j w[t, j] rows[position[t, j]] (w NULL: 1).  Bound by reading the rows: 8192 x 4 rows of 4096 bf16 88 us
+// with a row at a time.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const uint8_t* __restrict__ rows, const float* __restrict__ w,
                                                              const int* __restrict__ position, uint8_t* __restrict__ out, int R,
-                                                             int k, int D) {
+                                                             int k, int D, int parts) {
     using P = Piece<DT, VEC>;
-    const int t = blockIdx.x;
-    for (int i = threadIdx.x; i < D / P::N; i += 256) {
-        float s[P::N] = {};
-        for (int j = 0; j < k; ++j) {
-            const int r = position[(size_t)t * k + j];
-            if ((unsigned)r >= (unsigned)R) continue;
-            const float f = w != nullptr ? w[(size_t)t * k + j] : 1.0f;
-            float v[P::N];
-            P::load(rows + (size_t)r * D * P::ES, i, v);
+    const long long t = blockIdx.x / parts;
+    const int i = (blockIdx.x % parts) * 256 + threadIdx.x;
+    if (i >= D / P::N) return;
+    float s[P::N] = {};
+    for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
+        int r[ROW_SLOTS];
+        float f[ROW_SLOTS], v[ROW_SLOTS][P::N];
+        slots_of(position, w, t, j0, k, R, r, f);
 #pragma unroll
-            for (int n = 0; n < P::N; ++n) s[n] = fmaf(f, v[n], s[n]);
-        }
-        P::store(out + (size_t)t * D * P::ES, i, s);
+        for (int j = 0; j < ROW_SLOTS; ++j)
+            if (r[j] >= 0) P::load(rows + (size_t)r[j] * D * P::ES, i, v[j]);
+#pragma unroll
+        for (int j = 0; j < ROW_SLOTS; ++j)
+            if (r[j] >= 0) {
+#pragma unroll
+                for (int n = 0; n < P::N; ++n) s[n] = fmaf(f[j], v[j][n], s[n]);
+            }
     }
+    P::store(out + (size_t)t * D * P::ES, i, s);
 }
 
 // d_rows[position[t, j]] = w[t, j] d_out[t]; d_w[t, j] = <d_out[t], rows[position[t, j]]>, 0
-// for an unused slot; either may be NULL
+// for an unused slot; either may be NULL.  A workgroup takes a token whole: the
+// products of a slot are added over its threads in a fixed order.
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
         const uint8_t* __restrict__ rows, const float* __restrict__ w, const int* __restrict__ position,
         const int* __restrict__ offsets, const uint8_t* __restrict__ d_out, uint8_t* __restrict__ d_rows,
         float* __restrict__ d_w, int R, int k, int E, int D) {
     using P = Piece<DT, VEC>;
-    __shared__ float part[4];
-    const int t = blockIdx.x;
-    for (int j = 0; j < k; ++j) {
-        const int r = position[(size_t)t * k + j];
-        const float f = w[(size_t)t * k + j];
-        float dot = 0.0f;
-        if ((unsigned)r < (unsigned)R)
-            for (int i = threadIdx.x; i < D / P::N; i += 256) {
-                float v[P::N], g[P::N];
-                P::load(rows + (size_t)r * D * P::ES, i, v);
-                P::load(d_out + (size_t)t * D * P::ES, i, g);
+    __shared__ float part[4][ROW_SLOTS];
+    const long long t = blockIdx.x;
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
+        int r[ROW_SLOTS];
+        float f[ROW_SLOTS], dot[ROW_SLOTS] = {};
+        slots_of(position, w, t, j0, k, R, r, f);
+        for (int i = threadIdx.x; i < D / P::N; i += 256) {
+            float g[P::N], v[ROW_SLOTS][P::N];
+            P::load(d_out + (size_t)t * D * P::ES, i, g);
+            if (d_w != nullptr) {
 #pragma unroll
-                for (int n = 0; n < P::N; ++n) {
-                    dot = fmaf(v[n], g[n], dot);
-                    g[n] *= f;
-                }
-                if (d_rows != nullptr) P::store(d_rows + (size_t)r * D * P::ES, i, g);
+                for (int j = 0; j < ROW_SLOTS; ++j)
+                    if (r[j] >= 0) P::load(rows + (size_t)r[j] * D * P::ES, i, v[j]);
             }
 #pragma unroll
-        for (int d = 1; d < 64; d <<= 1) dot += __shfl_xor(dot, d);
-        if ((threadIdx.x & 63) == 0) part[threadIdx.x >> 6] = dot;
+            for (int j = 0; j < ROW_SLOTS; ++j) {
+                if (r[j] < 0) continue;
+                float d[P::N];
+#pragma unroll
+                for (int n = 0; n < P::N; ++n) {
+                    if (d_w != nullptr) dot[j] = fmaf(v[j][n], g[n], dot[j]);
+                    d[n] = f[j] * g[n];
+                }
+                if (d_rows != nullptr) P::store(d_rows + (size_t)r[j] * D * P::ES, i, d);
+            }
+        }
+        if (d_w == nullptr) continue;
+#pragma unroll
+        for (int j = 0; j < ROW_SLOTS; ++j) {
+#pragma unroll
+            for (int d = 1; d < 64; d <<= 1) dot[j] += __shfl_xor(dot[j], d);
+            if (lane == 0) part[wave][j] = dot[j];
+        }
         __syncthreads();
-        if (threadIdx.x == 0 && d_w != nullptr) d_w[(size_t)t * k + j] = (part[0] + part[1]) + (part[2] + part[3]);
+        if (threadIdx.x < ROW_SLOTS && j0 + (int)threadIdx.x < k)
+            d_w[t * k + j0 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) +
+                                            (part[2][threadIdx.x] + part[3][threadIdx.x]);
         __syncthreads();
     }
     if (d_rows != nullptr) zero_tail<DT, VEC>(d_rows, offsets, R, E, D);
@@ -314,23 +352,36 @@ static void by_type(int dt, int D, F f) {
     else vec ? f(integral_constant<int, DT_F16>{}, T{}) : f(integral_constant<int, DT_F16>{}, N{});
 }
 
+// workgroups of 256 pieces that a row takes
+template <int DT, bool VEC>
+static long long row_parts(int D) { return (D / Piece<DT, VEC>::N + 255) / 256; }
+
 hipError_t expert_gather_launch(const void* x, int dt, const int* position, const int* offsets, void* rows, int T, int k, int E,
                                 int D, hipStream_t st) {
+    bool fits = true;
     by_type(dt, D, [&](auto d, auto v) {
-        hipLaunchKernelGGL((expert_gather_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
-                           reinterpret_cast<const uint8_t*>(x), position, offsets, reinterpret_cast<uint8_t*>(rows), T * k, k, E,
-                           D);
+        const long long parts = row_parts<decltype(d)::value, decltype(v)::value>(D);
+        fits = T * parts <= 0x7fffffffLL;
+        if (fits)
+            hipLaunchKernelGGL((expert_gather_kernel<decltype(d)::value, decltype(v)::value>), dim3((unsigned)(T * parts)),
+                               dim3(256), 0, st, reinterpret_cast<const uint8_t*>(x), position, offsets,
+                               reinterpret_cast<uint8_t*>(rows), T * k, k, E, D, (int)parts);
     });
-    return hipGetLastError();
+    return fits ? hipGetLastError() : hipErrorInvalidValue;
 }
 
 hipError_t expert_combine_launch(const void* rows, int dt, const float* w, const int* position, void* out, int T, int k, int D,
                                  hipStream_t st) {
+    bool fits = true;
     by_type(dt, D, [&](auto d, auto v) {
-        hipLaunchKernelGGL((expert_combine_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
-                           reinterpret_cast<const uint8_t*>(rows), w, position, reinterpret_cast<uint8_t*>(out), T * k, k, D);
+        const long long parts = row_parts<decltype(d)::value, decltype(v)::value>(D);
+        fits = T * parts <= 0x7fffffffLL;
+        if (fits)
+            hipLaunchKernelGGL((expert_combine_kernel<decltype(d)::value, decltype(v)::value>), dim3((unsigned)(T * parts)),
+                               dim3(256), 0, st, reinterpret_cast<const uint8_t*>(rows), w, position,
+                               reinterpret_cast<uint8_t*>(out), T * k, k, D, (int)parts);
     });
-    return hipGetLastError();
+    return fits ? hipGetLastError() : hipErrorInvalidValue;
 }
 
 hipError_t expert_combine_grad_launch(const void* rows, int dt, const float* w, const int* position, const int* offsets,

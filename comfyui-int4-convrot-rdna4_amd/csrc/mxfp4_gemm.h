@@ -33,9 +33,6 @@ inline void mx_set_top_k(MxProblem& p, int d) {
     p.k_mul = (unsigned)(((1ull << p.k_shift) + d - 1) / d);
 }
 
-// Where mxfp4_quant_launch puts codes and scales.
-enum : int { MX_PLAIN = 0, MX_ROWS = 1, MX_TILES = 2 };
-
 // Place of block b (0 .. 15) of 512 k: a lane of half h of a wave takes blocks 2 s + h of a stage of 256 k, s = 0 .. 3,
 // whose bytes are one word.
 __host__ __device__ constexpr int mx_scale_place(int b) { return (b & 8) | (b & 1) << 2 | (b >> 1 & 3); }

@@ -12,6 +12,8 @@
 
 #include "mxfp4_gemm.h"
 
+#include <type_traits>
+
 namespace convrot {
 
 template <int DT, int G>
@@ -32,14 +34,43 @@ __global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restr
     }
 }
 
+// 16 scale bytes of weight row n of expert e (piece i: 512 k number i / N % (Ks/16)) into the order of staged tiles:
+// [E, N, nb] -> [E, Ks/16, N, 16].
+struct MxTileScales { const uint8_t* src; uint8_t* dst; long long pieces; int N, nb; };
+
+__device__ __forceinline__ void tile_scales(const MxTileScales& w, long long i, int Ks) {
+    if (i >= w.pieces) return;
+    const long long run = i / w.N;                         // e Ks/16 + 512 k number
+    const int n = (int)(i - run * w.N), per = Ks / 16;
+    const long long e = run / per;
+    const int b0 = (int)(run - e * per) * 16;
+    const uint8_t* s = w.src + (size_t)(e * w.N + n) * w.nb + b0;
+    v4u_mx o = {0u, 0u, 0u, 0u};
+    if (w.nb % 16 == 0) {
+        const v4u_mx r = *reinterpret_cast<const v4u_mx*>(s);
+#pragma unroll
+        for (int j = 0; j < 16; ++j) o[mx_scale_place(j) >> 2] |= (r[j >> 2] >> (8 * (j & 3)) & 255u) << (8 * (mx_scale_place(j) & 3));
+    } else {
+#pragma unroll
+        for (int j = 0; j < 16; ++j)
+            if (b0 + j < w.nb) o[mx_scale_place(j) >> 2] |= (uint32_t)s[j] << (8 * (mx_scale_place(j) & 3));
+    }
+    reinterpret_cast<v4u_mx*>(w.dst)[i] = o;
+}
+
 // The activation of a product: rows of codes padded to Kp values (a multiple of 256) with codes 0, scales in rows of
 // Ks bytes or (TILES) in the order of staged tiles (mxfp4_gemm.h), 16 bytes of 512 k a row either way.  A workgroup
-// takes 512 k of 8 rows, so that its scales leave as one run of 128 bytes (a byte a block, as above, 8192 x 8192: 34 us).
+// takes 512 k of 8 rows, so that its scales leave as one run of 128 bytes.  The grid's last workgroups lay out the
+// weight's scales for staged tiles: a launch of its own for them took 3.5 us more.
 template <int DT, int G, bool TILES>
 __global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
-                                                               uint8_t* __restrict__ scales, int M, int K, int Kp, int Ks) {
+                                                               uint8_t* __restrict__ scales, int M, int K, int Kp, int Ks,
+                                                               unsigned blocks, MxTileScales w) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     __shared__ __attribute__((aligned(16))) uint8_t sc[8][16];
+    if constexpr (TILES) {
+        if (blockIdx.x >= blocks) return tile_scales(w, (long long)(blockIdx.x - blocks) * 256 + threadIdx.x, Ks);
+    }
     const int per = Ks / 16;
     const int ss = blockIdx.x % per, row0 = (int)(blockIdx.x / per) * 8;
     const int r = threadIdx.x >> 5, l = threadIdx.x & 31;
@@ -54,9 +85,9 @@ __global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __
     if (row < M && k < Kp) *reinterpret_cast<v2u_mx*>(codes + (size_t)row * (Kp / 2) + k / 2) = c;
     if ((l & 1) == 0) sc[r][TILES ? mx_scale_place(l >> 1) : l >> 1] = (uint8_t)sb;
     __syncthreads();
-    const int w = row0 + threadIdx.x;
-    if (threadIdx.x < 8 && w < M)
-        *reinterpret_cast<v4u_mx*>(scales + (TILES ? ((size_t)ss * M + w) * 16 : (size_t)w * Ks + ss * 16)) =
+    const int m = row0 + threadIdx.x;
+    if (threadIdx.x < 8 && m < M)
+        *reinterpret_cast<v4u_mx*>(scales + (TILES ? ((size_t)ss * M + m) * 16 : (size_t)m * Ks + ss * 16)) =
                 *reinterpret_cast<const v4u_mx*>(sc[threadIdx.x]);
 }
 
@@ -106,71 +137,56 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
 }
 
 template <int DT, int G>
-static void quant_go(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int layout, hipStream_t st) {
-    const auto xb = reinterpret_cast<const uint8_t*>(x);
-    const auto cb = reinterpret_cast<uint8_t*>(codes);
-    const auto sb = reinterpret_cast<uint8_t*>(scales);
+static void quant_go(const void* x, void* codes, void* scales, int M, int K, hipStream_t st) {
     const long long units = (long long)M * (K / 16);
-    const dim3 rows((unsigned)((M + 7LL) / 8 * (Ks / 16)));
-    if (layout == MX_PLAIN)
-        hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st, xb, cb, sb, units);
-    else if (layout == MX_TILES)
-        hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, G, true>), rows, dim3(256), 0, st, xb, cb, sb, M, K, Kp, Ks);
-    else
-        hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, G, false>), rows, dim3(256), 0, st, xb, cb, sb, M, K, Kp, Ks);
+    hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st,
+                       reinterpret_cast<const uint8_t*>(x), reinterpret_cast<uint8_t*>(codes), reinterpret_cast<uint8_t*>(scales),
+                       units);
 }
 
-template <int DT>
-static void quant_group(const void* x, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, int layout,
-                        hipStream_t st) {
-    switch (G) {
-        case 0: return quant_go<DT, 0>(x, codes, scales, M, K, Kp, Ks, layout, st);
-        case 16: return quant_go<DT, 16>(x, codes, scales, M, K, Kp, Ks, layout, st);
-        case 64: return quant_go<DT, 64>(x, codes, scales, M, K, Kp, Ks, layout, st);
-        default: return quant_go<DT, 256>(x, codes, scales, M, K, Kp, Ks, layout, st);
-    }
-}
-
-// x [M, K] -> codes and scales: MX_PLAIN the public form (Kp, Ks unused), MX_ROWS and MX_TILES a product's operand
-hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int Kp, int Ks, int G, int layout,
-                              hipStream_t st) {
-    if (M == 0) return hipSuccess;
+// f(type code, group) as compile-time constants
+template <typename F>
+static void by_type_and_group(int dt, int G, F f) {
+    using std::integral_constant;
+    auto group = [&](auto d) {
+        switch (G) {
+            case 0: return f(d, integral_constant<int, 0>{});
+            case 16: return f(d, integral_constant<int, 16>{});
+            case 64: return f(d, integral_constant<int, 64>{});
+            default: return f(d, integral_constant<int, 256>{});
+        }
+    };
     switch (dt) {
-        case DT_F32: quant_group<DT_F32>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
-        case DT_BF16: quant_group<DT_BF16>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
-        default: quant_group<DT_F16>(x, codes, scales, M, K, Kp, Ks, G, layout, st); break;
+        case DT_F32: return group(integral_constant<int, DT_F32>{});
+        case DT_BF16: return group(integral_constant<int, DT_BF16>{});
+        default: return group(integral_constant<int, DT_F16>{});
     }
+}
+
+// x [M, K] -> codes [M, K/2], scales [M, K/32]
+hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int G, hipStream_t st) {
+    if (M == 0) return hipSuccess;
+    by_type_and_group(dt, G, [&](auto d, auto g) { quant_go<decltype(d)::value, decltype(g)::value>(x, codes, scales, M, K, st); });
     return hipGetLastError();
 }
 
-// Scales [E, N, nb] -> [E, Ks/16, N, 16], 16 bytes a thread (piece i: 512 k number i / N % (Ks/16) of a row).
-__global__ __launch_bounds__(256) void mxfp4_tile_scales_kernel(const uint8_t* __restrict__ src, uint8_t* __restrict__ dst,
-                                                                long long pieces, int N, int nb, int Ks) {
-    const long long i = (long long)blockIdx.x * 256 + threadIdx.x;
-    if (i >= pieces) return;
-    const long long run = i / N;                           // e Ks/16 + 512 k number
-    const int n = (int)(i - run * N), per = Ks / 16;
-    const long long e = run / per;
-    const int b0 = (int)(run - e * per) * 16;
-    const uint8_t* s = src + (size_t)(e * N + n) * nb + b0;
-    v4u_mx w = {0u, 0u, 0u, 0u};
-    if (nb % 16 == 0) {
-        const v4u_mx r = *reinterpret_cast<const v4u_mx*>(s);
-#pragma unroll
-        for (int j = 0; j < 16; ++j) w[mx_scale_place(j) >> 2] |= (r[j >> 2] >> (8 * (j & 3)) & 255u) << (8 * (mx_scale_place(j) & 3));
-    } else {
-#pragma unroll
-        for (int j = 0; j < 16; ++j)
-            if (b0 + j < nb) w[mx_scale_place(j) >> 2] |= (uint32_t)s[j] << (8 * (mx_scale_place(j) & 3));
-    }
-    reinterpret_cast<v4u_mx*>(dst)[i] = w;
-}
-
-hipError_t mxfp4_tile_scales_launch(const void* src, void* dst, int E, int N, int nb, int Ks, hipStream_t st) {
-    const long long pieces = (long long)E * N * (Ks / 16);
-    if (pieces == 0) return hipSuccess;
-    hipLaunchKernelGGL(mxfp4_tile_scales_kernel, dim3((unsigned)((pieces + 255) / 256)), dim3(256), 0, st,
-                       reinterpret_cast<const uint8_t*>(src), reinterpret_cast<uint8_t*>(dst), pieces, N, nb, Ks);
+// x [rows, K] as the operand p.a, p.as of a product; with `tiles` in the order of staged tiles, and p.ws as p.wp
+hipError_t mxfp4_operands_launch(const void* x, int G, const MxProblem& p, bool tiles, hipStream_t st) {
+    const unsigned blocks = (unsigned)((p.as_rows + 7LL) / 8 * (p.Ks / 16));
+    MxTileScales w{p.ws, const_cast<uint8_t*>(p.wp), (long long)p.E * p.N * (p.Ks / 16), p.N, p.K / 32};
+    const long long grid = tiles ? blocks + (w.pieces + 255) / 256 : blocks;
+    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
+    by_type_and_group(p.dt, G, [&](auto d, auto g) {
+        constexpr int DT = decltype(d)::value, GG = decltype(g)::value;
+        const auto xb = reinterpret_cast<const uint8_t*>(x);
+        const auto cb = const_cast<uint8_t*>(p.a), sb = const_cast<uint8_t*>(p.as);
+        if (tiles)
+            hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, true>), dim3((unsigned)grid), dim3(256), 0, st, xb, cb, sb,
+                               p.as_rows, p.K, p.Kp, p.Ks, blocks, w);
+        else
+            hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, false>), dim3((unsigned)grid), dim3(256), 0, st, xb, cb, sb,
+                               p.as_rows, p.K, p.Kp, p.Ks, blocks, w);
+    });
     return hipGetLastError();
 }
 

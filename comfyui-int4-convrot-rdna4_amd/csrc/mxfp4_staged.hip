@@ -312,16 +312,28 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     }
 }
 
-// 0: not this kernel; else the wave's fragments 16 FM + FN.
+// The kernel of a product: 0 the one for few rows (mxfp4_gemm.hip), else the tile, 256 or 128 a side.
+//
+// Few rows run there up to 32, and up to one round of its workgroups of 64 x 32 outputs where there is one weight
+// (512 K, us: 4096 columns 64 rows 15.9, staged 20.2; 192 rows 25.7 and 20.6; 2048 columns of K 8192 256 rows 24 and 31);
+// experts' few rows leave most of such a workgroup idle (64 rows of 32 experts 35.9 and 35.1).
+// Tiles: rounds of the CUs times what a tile takes, measured at K 1600 to 8192: 256 a side, one a CU, 8 + 1.65 us a
+// stage of 256 k; 128 a side, two a CU, 7 + 0.83 us (13824 columns of K 5120: 512 rows 44.5 and 34.3 us, 1024 rows 52.2
+// and 58, 8192 rows 308 and 346; 2048 columns of K 8192: 4096 rows 70.4 and 64.8).
 static int staged_shape(const MxProblem& p) {
-    if (p.R <= 64) return 0;
-    // the tokens' rows are addressed by 32-bit offsets from the first
-    if (p.order != nullptr && (size_t)(p.R / p.top_k) * (p.Kp / 2) >= (size_t(1) << 32)) return 0;
     const bool ragged = p.offsets != nullptr;
-    auto tiles = [&](int bm, int bn) { return mx_row_tiles(p.R, p.E, ragged, bm) * ((p.N + bn - 1) / bn); };
-    if (tiles(256, 256) >= 200) return 0x44;
-    if (tiles(128, 256) >= 200) return 0x24;
-    return 0x22;
+    if (p.R <= 32) return 0;
+    if (!ragged && (p.R + 63LL) / 64 * ((p.N + 31) / 32) <= 256) return 0;
+    // the tokens' rows are addressed by 32-bit offsets from the first
+    if (p.order != nullptr && (size_t)p.as_rows * (p.Kp / 2) >= (size_t(1) << 32)) return 0;
+    auto cost = [&](int side, int at_once, double fixed, double stage) {
+        // half a tile more for each expert that has rows
+        const double rows = ragged ? (double)p.R / side + 0.5 * (p.E < p.R ? p.E : p.R) : (double)((p.R + side - 1) / side);
+        const double tiles = rows * ((p.N + side - 1) / side);
+        const long long rounds = (long long)(tiles / at_once) + (tiles > (double)at_once * (long long)(tiles / at_once));
+        return rounds * (fixed + stage * ((p.K + 255) / 256));
+    };
+    return cost(256, 256, 8.0, 1.65) < cost(128, 512, 7.0, 0.83) ? 256 : 128;
 }
 
 bool mxfp4_gemm_staged(const MxProblem& p) { return staged_shape(p) != 0; }
@@ -345,11 +357,7 @@ static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
 
 template <int DT>
 static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
-    switch (staged_shape(p)) {
-        case 0x44: return staged_go<DT, 4, 4>(p, st);
-        case 0x24: return staged_go<DT, 2, 4>(p, st);
-        default: return staged_go<DT, 2, 2>(p, st);
-    }
+    return staged_shape(p) == 256 ? staged_go<DT, 4, 4>(p, st) : staged_go<DT, 2, 2>(p, st);
 }
 
 hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st) {
