@@ -279,30 +279,37 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
                     }
                 }
                 wave_sync();
+                // eight pieces read together: one by one, each store waited for its own read (11100 cycles a 256 x 256 tile)
+                constexpr int EIGHT = PR * (32 / ROWS) < 8 ? PR * (32 / ROWS) : 8;
 #pragma unroll
-                for (int x = x0; x < x0 + PR; ++x) {
-                    const int c = x / FM, i = x % FM;
-                    const int col = c0 + c * CP + unit * (16 / ES);
+                for (int y0 = 0; y0 < PR * (32 / ROWS); y0 += EIGHT) {
+                    v4u_mx w[EIGHT];
 #pragma unroll
-                    for (int r = 0; r < 32; r += ROWS) {
-                        const int row = r + prow, m = m0 + i * 32 + row;
-                        const v4u_mx w = *reinterpret_cast<const v4u_mx*>(scr + (x - x0) * 32 * RB + row * RB +
-                                                                          ((unit ^ (row & (U - 1))) << 4));
+                    for (int y = 0; y < EIGHT; ++y) {
+                        const int x = (y0 + y) / (32 / ROWS), row = (y0 + y) % (32 / ROWS) * ROWS + prow;
+                        w[y] = *reinterpret_cast<const v4u_mx*>(scr + x * 32 * RB + row * RB + ((unit ^ (row & (U - 1))) << 4));
+                    }
+                    __builtin_amdgcn_sched_barrier(0);
+#pragma unroll
+                    for (int y = 0; y < EIGHT; ++y) {
+                        const int x = x0 + (y0 + y) / (32 / ROWS), row = (y0 + y) % (32 / ROWS) * ROWS + prow;
+                        const int m = m0 + x % FM * 32 + row, col = c0 + x / FM * CP + unit * (16 / ES);
                         uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + col) * ES;
                         // not kept in L2, where the next tiles' operands are
-                        if constexpr (!EDGE) __builtin_nontemporal_store(w, reinterpret_cast<v4u_mx*>(o));
+                        if constexpr (!EDGE) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
                         else if (m < m1 && col < p.N) {
-                            if (vec) __builtin_nontemporal_store(w, reinterpret_cast<v4u_mx*>(o));
+                            if (vec) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
                             else {
 #pragma unroll
                                 for (int e = 0; e < 16 / ES; ++e)
                                     if (col + e < p.N) {
-                                        if constexpr (DT == DT_F32) reinterpret_cast<uint32_t*>(o)[e] = w[e];
-                                        else reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(w[e / 2] >> (16 * (e & 1)));
+                                        if constexpr (DT == DT_F32) reinterpret_cast<uint32_t*>(o)[e] = w[y][e];
+                                        else reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(w[y][e / 2] >> (16 * (e & 1)));
                                     }
                             }
                         }
                     }
+                    __builtin_amdgcn_sched_barrier(0);
                 }
                 wave_sync();
             }
