@@ -24,17 +24,18 @@ namespace convrot {
 typedef int v8i_mx __attribute__((ext_vector_type(8)));
 typedef float v16f_mx __attribute__((ext_vector_type(16)));
 
-template <int FM_, int FN_>
+template <int FM_, int FN_, int SLOTS_>
 struct Staged {
     static constexpr int FM = FM_, FN = FN_;               // 32-row fragments of a wave
+    static constexpr int SLOTS = SLOTS_;                   // stages in LDS: 2 or 4
     static constexpr int BM = 64 * FM, BN = 64 * FN;
     static constexpr int THREADS = 256;
     static constexpr int STAGE = (BM + BN) * 128;          // codes of 256 k
     static constexpr int SCALES = (BM + BN) * 16;          // scale bytes of 512 k
-    static constexpr int RING = 2 * STAGE;
-    static constexpr int LDS = RING + 2 * SCALES;
+    static constexpr int RING = SLOTS * STAGE;
+    static constexpr int LDS = RING + SLOTS * SCALES;      // scales of two stages each: what is read and what is copied
     static constexpr int L = 2 * (FM + FN);                // copies of a wave and stage (1 KB each)
-    static constexpr int D3 = (L + 2) / 3, D0 = D3, D1 = L - D3 - D0;   // issued in phase 3 of the stage before, 0 and 1
+    static constexpr int D3 = (L + 2) / 3, D0 = D3, D1 = L - D3 - D0;   // issued in phase 3 of a stage, 0 and 1 of the next
     static constexpr int NS = (FM + FN + 3) / 4;           // copies of scales of a wave and 512 k
 };
 
@@ -42,9 +43,9 @@ struct Staged {
 // lanes that an LDS read serves at a time, 16 rows of one chunk, touch every bank once.
 __device__ __forceinline__ uint32_t staged_off(int row, int chunk) { return row * 128 + ((chunk ^ (row >> 1 & 7)) << 4); }
 
-template <int DT, int FM, int FN>
+template <int DT, int FM, int FN, int SLOTS>
 __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, int gm_max) {
-    using S = Staged<FM, FN>;
+    using S = Staged<FM, FN, SLOTS>;
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_mx[];
     const int tid = threadIdx.x, lane = tid & 63;
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
@@ -113,7 +114,7 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
 #pragma unroll
         for (int j = 0; j < S::NS; ++j) {
             const int i = min(wave * S::NS + j, FM + FN - 1);
-            dma16_sv(lds0 + S::RING + (ss & 1) * S::SCALES + i * 1024,
+            dma16_sv(lds0 + S::RING + ss % SLOTS * S::SCALES + i * 1024,
                      i < FM ? AS + (size_t)ss * a_step : WS + (size_t)ss * w_step, soff[j]);
         }
     };
@@ -155,35 +156,39 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     using T = std::true_type;
     using N = std::false_type;
 
-    // Two slots: stage st sits in slot st % 2.  A stage is four phases of 64 k; while phase s multiplies, the fragments
-    // of the next one are read.  Before phase 3 every wave waits for its copies of stage st + 1 and for its reads of
-    // stage st, and passes the barrier: stage st + 1 is there, and no wave reads stage st's slot any more.  Stage st + 2
-    // is copied into it in phase 3 and in phases 0 and 1 of stage st + 1; its last copies have phase 2 to arrive in.
-    // The scales of 512 k come with the first of the two stages before.
-    // more1, more2: stages st + 1, st + 2 are there (known when compiling the steady loop); START: the first stage.
-    auto stage = [&](int st, auto place, auto start, bool more1, bool more2) __attribute__((always_inline)) {
-        constexpr int q = decltype(place)::value;          // st % 2
-        constexpr uint32_t here = q * S::STAGE, next = (1 - q) * S::STAGE;
-        const uint32_t sc_next = ((st + 1) >> 1 & 1) * S::SCALES + (1 - q) * 8;
+    // Stage st sits in slot st % SLOTS.  A stage is four phases of 64 k; while phase s multiplies, the fragments of the
+    // next one are read.  Before phase 3 every wave waits for its copies of stage st + 1 and for its reads of stage st,
+    // and passes the barrier: stage st + 1 is there, and no wave reads stage st's slot any more.  Stage st + SLOTS is
+    // copied into it in phase 3 and in phases 0 and 1 of stage st + 1.  With two slots its last copies have phase 2 to
+    // arrive in, which two workgroups on a CU, or the long phases of a 256 x 256 tile, hide; four slots give them two
+    // stages more.  The scales of 512 k come SLOTS stages ahead.
+    // STEADY: stages st + SLOTS and below are all there; START: the first stage.
+    auto stage = [&](int st, auto place, auto start, auto steady) __attribute__((always_inline)) {
+        constexpr int q = decltype(place)::value;          // st % SLOTS
+        constexpr bool STEADY = decltype(steady)::value;
+        constexpr uint32_t here = q * S::STAGE, next = (q + 1) % SLOTS * S::STAGE;
+        const bool late = STEADY || st + SLOTS < nst, early = STEADY || st + SLOTS - 1 < nst;
+        const uint32_t sc_next = ((st + 1) >> 1) % SLOTS * S::SCALES + ((q + 1) & 1) * 8;
         auto phase = [&](auto step, auto zero) __attribute__((always_inline)) {
             constexpr int s = decltype(step)::value;
             constexpr int n = s == 3 ? S::D3 : s == 0 ? S::D0 : s == 1 ? S::D1 : 0;      // copies of this phase
             constexpr int first = s == 3 ? 0 : s == 0 ? S::D3 : S::D3 + S::D0;
-            if (s == 0 && q == 0 && more2) dma_scales((st >> 1) + 1);
+            if (s == 0 && q % 2 == 0 && late) dma_scales((st + SLOTS) >> 1);
 #pragma unroll
             for (int x = 0; x < X; ++x) {
-                mfma_one(F[s & 1], C[q], step, zero, x);
+                mfma_one(F[s & 1], C[q & 1], step, zero, x);
                 __builtin_amdgcn_sched_barrier(0);
                 if (x < Y) {
                     if (s < 3) read_frag(F[(s + 1) & 1], here, (s + 1) & 3, x);
                     else {
                         read_frag(F[0], next, 0, x);
-                        read_scale(C[1 - q], sc_next, x);
+                        read_scale(C[(q + 1) & 1], sc_next, x);
                     }
                 }
-                if (s == 3 ? more2 : more1) {
+                if (s == 3 ? late : early) {
 #pragma unroll
-                    for (int j = x * n / X; j < (x + 1) * n / X; ++j) dma_codes(s == 3 ? st + 2 : st + 1, s == 3 ? q : 1 - q, first + j);
+                    for (int j = x * n / X; j < (x + 1) * n / X; ++j)
+                        dma_codes(s == 3 ? st + SLOTS : st + SLOTS - 1, s == 3 ? q : (q + SLOTS - 1) % SLOTS, first + j);
                 }
                 __builtin_amdgcn_sched_barrier(0);
             }
@@ -191,13 +196,17 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         phase(std::integral_constant<int, 0>{}, start);
         phase(std::integral_constant<int, 1>{}, N{});
         phase(std::integral_constant<int, 2>{}, N{});
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & 0xc07f);  // and no LDS read of this wave outstanding
+        // vmcnt counts in order of issue.  After stage st + 1's copies came those of stages st + 2 .. st + SLOTS - 1, and
+        // the scales issued in the even one of this stage and the one before.  0xc07f: no LDS read of this wave either.
+        constexpr int AHEAD = (SLOTS - 2) * S::L;
+        if (SLOTS > 2 && (q % 2 == 0 ? late : early))
+            __builtin_amdgcn_s_waitcnt(vmcnt_imm(AHEAD + S::NS) & 0xc07f);
+        else if (SLOTS > 2 && early) __builtin_amdgcn_s_waitcnt(vmcnt_imm(AHEAD) & 0xc07f);
+        else __builtin_amdgcn_s_waitcnt(vmcnt_imm(0) & 0xc07f);
         __builtin_amdgcn_s_barrier();
         __builtin_amdgcn_sched_barrier(0);
         phase(std::integral_constant<int, 3>{}, N{});
     };
-    using Q0 = std::integral_constant<int, 0>;
-    using Q1 = std::integral_constant<int, 1>;
 
     // LDS traffic of this wave done, and every wave here (vmcnt as it is: copies and stores stay in flight)
     auto lds_barrier = [&]() __attribute__((always_inline)) {
@@ -214,13 +223,19 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     constexpr int U = RB / 16, ROWS = 64 / U;              // 16-byte units of a row, rows of a wave's store
     static_assert(PR >= 1 && PIECES % PR == 0, "whole pieces");
 
-    dma_scales(0);
 #pragma unroll
-    for (int j = 0; j < S::L; ++j) dma_codes(0, 0, j);
-    if (nst > 1) {
+    for (int ss = 0; ss < SLOTS / 2; ++ss)
+        if (2 * ss < nst) dma_scales(ss);
 #pragma unroll
-        for (int j = 0; j < S::D3; ++j) dma_codes(1, 1, j);
-        __builtin_amdgcn_s_waitcnt(vmcnt_imm(S::D3));      // stage 0 and its scales are there
+    for (int st = 0; st < SLOTS - 1; ++st)
+        if (st < nst) {
+#pragma unroll
+            for (int j = 0; j < S::L; ++j) dma_codes(st, st, j);
+        }
+    if (SLOTS - 1 < nst) {
+#pragma unroll
+        for (int j = 0; j < S::D3; ++j) dma_codes(SLOTS - 1, SLOTS - 1, j);
+        __builtin_amdgcn_s_waitcnt(vmcnt_imm((SLOTS - 2) * S::L + S::D3));      // stage 0 and its scales are there
     } else {
         __builtin_amdgcn_s_waitcnt(vmcnt_imm(0));
     }
@@ -230,15 +245,28 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         read_frag(F[0], 0, 0, r);
         read_scale(C[0], 0, r);
     }
-    stage(0, Q0{}, T{}, nst > 1, nst > 2);
+    auto place = [](auto i) { return std::integral_constant<int, decltype(i)::value % SLOTS>{}; };
+    using I1 = std::integral_constant<int, 1>;
+    using I2 = std::integral_constant<int, 2>;
+    using I3 = std::integral_constant<int, 3>;
+    using I4 = std::integral_constant<int, 4>;
+    stage(0, std::integral_constant<int, 0>{}, T{}, N{});
     int st = 1;
-    for (; st + 3 < nst; st += 2) {
-        stage(st, Q1{}, N{}, true, true);
-        stage(st + 1, Q0{}, N{}, true, true);
+    for (; st + 2 * SLOTS - 1 < nst; st += SLOTS) {
+        stage(st, place(I1{}), N{}, T{});
+        stage(st + 1, place(I2{}), N{}, T{});
+        if constexpr (SLOTS == 4) {
+            stage(st + 2, place(I3{}), N{}, T{});
+            stage(st + 3, place(I4{}), N{}, T{});
+        }
     }
-    for (; st < nst; st += 2) {
-        stage(st, Q1{}, N{}, st + 1 < nst, st + 2 < nst);
-        if (st + 1 < nst) stage(st + 1, Q0{}, N{}, st + 2 < nst, st + 3 < nst);
+    for (; st < nst; st += SLOTS) {
+        stage(st, place(I1{}), N{}, N{});
+        if (st + 1 < nst) stage(st + 1, place(I2{}), N{}, N{});
+        if constexpr (SLOTS == 4) {
+            if (st + 2 < nst) stage(st + 2, place(I3{}), N{}, N{});
+            if (st + 3 < nst) stage(st + 3, place(I4{}), N{}, N{});
+        }
     }
     lds_barrier();                                         // no wave reads the ring or the scales any more
     float* biases = reinterpret_cast<float*>(lds_mx + S::RING);
@@ -345,26 +373,29 @@ static int staged_shape(const MxProblem& p) {
 
 bool mxfp4_gemm_staged(const MxProblem& p) { return staged_shape(p) != 0; }
 
-template <int DT, int FM, int FN>
+template <int DT, int FM, int FN, int SLOTS>
 static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
-    using S = Staged<FM, FN>;
+    using S = Staged<FM, FN, SLOTS>;
     static std::atomic<bool> attr[kMaxDev];
     int dev = 0;
     hipError_t e = current_device(&dev);
     if (e != hipSuccess) return e;
-    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&mxfp4_gemm_staged_kernel<DT, FM, FN>), S::LDS);
+    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&mxfp4_gemm_staged_kernel<DT, FM, FN, SLOTS>), S::LDS);
     if (e != hipSuccess) return e;
     const long long rows = mx_row_tiles(p.R, p.E, p.offsets != nullptr, S::BM);
     long long grid = rows * ((p.N + S::BN - 1) / S::BN);
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((mxfp4_gemm_staged_kernel<DT, FM, FN>), dim3((unsigned)grid), dim3(S::THREADS), S::LDS, st, p,
+    hipLaunchKernelGGL((mxfp4_gemm_staged_kernel<DT, FM, FN, SLOTS>), dim3((unsigned)grid), dim3(S::THREADS), S::LDS, st, p,
                        tile_group_rows((int)rows));
     return hipGetLastError();
 }
 
 template <int DT>
 static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
-    return staged_shape(p) == 256 ? staged_go<DT, 4, 4>(p, st) : staged_go<DT, 2, 2>(p, st);
+    if (staged_shape(p) == 256) return staged_go<DT, 4, 4, 2>(p, st);
+    // one tile a CU or fewer: nothing but its own copies hides a stage's latency
+    const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 128) * ((p.N + 127) / 128);
+    return tiles <= 256 ? staged_go<DT, 2, 2, 4>(p, st) : staged_go<DT, 2, 2, 2>(p, st);
 }
 
 hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st) {

@@ -190,6 +190,27 @@ def test_expert_linear_exact(backend, gpu, T, k, E, N, K, rows):
         assert torch.equal(y.cpu(), torch.from_numpy(want).float().to(dtype))
 
 
+@pytest.mark.parametrize("rows", [False, True], ids=["tokens", "sorted"])
+@pytest.mark.parametrize("T,k,E,N,K", [(2048, 2, 8, 4096, 288), (1500, 3, 70, 1000, 544)])
+def test_expert_linear_exact_large(backend, gpu, T, k, E, N, K, rows):
+    """Several rounds of tiles: 256 a side with eight experts, 128 with seventy."""
+    say("experts", T, k, E, N, K, rows)
+    ids = choice(T, k, E, seed=T + N, skew=0.5)
+    order, _, offsets = mx.plan(ids, E)
+    x, wc, ws = exact_operands(T * k if rows else T, N, K, seed=T + K, E=E)
+    plan = backend.sort_tokens_by_expert(torch.from_numpy(ids).cuda(), E)
+    xt = torch.from_numpy(x).cuda()
+    a = xt if rows else xt[torch.from_numpy(np.maximum(order, 0) // k).cuda().long()]
+    want = torch.zeros(T * k, N, dtype=torch.float64, device="cuda")
+    for e in range(E):
+        r = slice(offsets[e], offsets[e + 1])
+        want[r] = a[r] @ torch.from_numpy(mx.dequantize(wc[e], ws[e])).cuda().T
+    w, s = torch.from_numpy(wc).cuda(), torch.from_numpy(ws).cuda()
+    for dtype in DTYPES:
+        y = backend.mxfp4_expert_linear(xt.to(dtype), w, s, plan, sorted_rows=rows)
+        assert torch.equal(y, want.float().to(dtype))
+
+
 @pytest.mark.parametrize("ids", ["unused", "one expert", "no tokens"])
 def test_expert_linear_extremes(backend, gpu, ids):
     E, N, K, k = 6, 72, 96, 2

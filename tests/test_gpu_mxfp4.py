@@ -191,6 +191,24 @@ def test_linear_exact(backend, gpu, M, N, K):
         assert torch.equal(y.cpu(), torch.from_numpy(want + bias).float().to(dtype))
 
 
+# grids of more than one round of 128 x 128 tiles, and of 256 x 256 tiles; whole tiles, edges, and N that is no multiple
+# of a 16-byte piece
+LARGE_SHAPES = [(2100, 2304, 608), (2048, 2304, 1600), (3900, 4001, 352), (4096, 4096, 512), (4096, 4096, 1312)]
+
+
+@pytest.mark.parametrize("M,N,K", LARGE_SHAPES)
+def test_linear_exact_large(backend, gpu, M, N, K):
+    say("linear", M, N, K)
+    x, wc, ws = exact_operands(M, N, K, seed=M + N + K)
+    bias = torch.from_numpy(np.random.RandomState(1).randint(-64, 64, N) / 8.0).cuda()
+    w, s = torch.from_numpy(wc).cuda(), torch.from_numpy(ws).cuda()
+    xt = torch.from_numpy(x).cuda()
+    want = xt @ torch.from_numpy(mx.dequantize(wc, ws)).cuda().T + bias         # float64
+    for dtype in DTYPES:
+        y = backend.mxfp4_linear(xt.to(dtype), w, s, bias.to(dtype))
+        assert torch.equal(y, want.float().to(dtype))
+
+
 @pytest.mark.parametrize("dtype", DTYPES)
 @pytest.mark.parametrize("M,N,K,G", [(1, 777, 5120, 256), (7, 512, 1600, 64), (48, 300, 2304, 256), (130, 512, 512, 16),
                                      (300, 640, 1088, None), (520, 1111, 1600, 64)])
