@@ -12,7 +12,7 @@ fp32, without atomics: the same inputs give the same bits.
 """
 from __future__ import annotations
 
-import dataclasses
+from typing import NamedTuple
 
 import torch
 
@@ -20,8 +20,7 @@ from . import native
 from .mxfp4 import _check_dtype, _same_device
 
 
-@dataclasses.dataclass(frozen=True)
-class ExpertPlan:
+class ExpertPlan(NamedTuple):
     """Where each slot's row goes.  ``order`` int32 [T k]: the slot of each sorted
     row, -1 past the last used one.  ``position`` int32 [T, k]: the sorted row of
     each slot, -1 for an unused one.  ``offsets`` int32 [E + 1]: expert e has the

@@ -14,19 +14,19 @@
 
 namespace convrot {
 
-constexpr int SORT_THREADS = 256, SORT_WAVES = 4;
-constexpr int SORT_EACH = 8;               // slots of a lane
-constexpr int SORT_SLOTS = 64 * SORT_EACH * SORT_WAVES;     // slots of a workgroup's run
+constexpr int SORT_EACH = 4;               // slots of a lane
+constexpr int SORT_FEW = 4, SORT_MANY = 16;                 // waves of a workgroup: of a plan that fits them, of others
+constexpr int sort_slots(int waves) { return 64 * SORT_EACH * waves; }      // slots of its run
 constexpr int SORT_MAX_E = 1024;
 
 // The experts of a wave's slots w0 + 64 i + lane (-1: none), loaded together.
 template <typename ID>
-__device__ __forceinline__ void experts_of(const ID* ids, int w0, int R, int E, int (&e)[SORT_EACH]) {
+__device__ __forceinline__ void experts_of(const ID* ids, long long w0, int R, int E, int (&e)[SORT_EACH]) {
     ID id[SORT_EACH];
     const int lane = threadIdx.x & 63;
 #pragma unroll
     for (int i = 0; i < SORT_EACH; ++i) {
-        const long long s = (long long)w0 + 64 * i + lane;
+        const long long s = w0 + 64 * i + lane;
         id[i] = s < R ? ids[s] : (ID)-1;
     }
 #pragma unroll
@@ -35,40 +35,42 @@ __device__ __forceinline__ void experts_of(const ID* ids, int w0, int R, int E, 
 
 // counts[b, e]: slots of workgroup b's run that go to expert e
 template <typename ID>
-__global__ __launch_bounds__(SORT_THREADS) void expert_count_kernel(const ID* __restrict__ ids, int* __restrict__ counts,
+__global__ __launch_bounds__(64 * SORT_MANY) void expert_count_kernel(const ID* __restrict__ ids, int* __restrict__ counts,
                                                                     int R, int E) {
     __shared__ int n[SORT_MAX_E];
     int e[SORT_EACH];
-    experts_of(ids, blockIdx.x * SORT_SLOTS + (threadIdx.x >> 6) * (SORT_SLOTS / SORT_WAVES), R, E, e);
-    for (int i = threadIdx.x; i < E; i += SORT_THREADS) n[i] = 0;
+    experts_of(ids, (blockIdx.x * (long long)SORT_MANY + (threadIdx.x >> 6)) * (64 * SORT_EACH), R, E, e);
+    for (int i = threadIdx.x; i < E; i += 64 * SORT_MANY) n[i] = 0;
     __syncthreads();
 #pragma unroll
     for (int i = 0; i < SORT_EACH; ++i)
         if (e[i] >= 0) atomicAdd(&n[e[i]], 1);             // integers: the order does not matter
     __syncthreads();
-    for (int i = threadIdx.x; i < E; i += SORT_THREADS) counts[(size_t)blockIdx.x * E + i] = n[i];
+    for (int i = threadIdx.x; i < E; i += 64 * SORT_MANY) counts[(size_t)blockIdx.x * E + i] = n[i];
 }
 
 // Workgroup b places its run: expert e's first row there is offsets[e] plus the
-// counts of the runs before.  Each wave takes a quarter of the run, in order, 64
+// counts of the runs before.  Each wave takes a part of the run, in order, 64
 // slots at a time; the lanes that go to one expert find each other by the bits of
 // its number, so that one of them counts for all, and their order is the slots'.
-// A single run needs no counts from elsewhere (ONE): one launch.  A few slots take
-// 2.6 us, 2000 of 32 experts 4, bound by the chain of loads, ballots and LDS.
-template <typename ID, bool ONE>
-__global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __restrict__ ids,
+// A single run needs no counts from elsewhere (ONE): one launch.  Bound by the
+// chain of loads, ballots and LDS, so a wave has few slots: 2000 slots of 32
+// experts 5.3 us (7.4 with four waves of 512), 64 slots 2.7 (3.4 with sixteen waves).
+template <typename ID, bool ONE, int WAVES>
+__global__ __launch_bounds__(64 * WAVES) void expert_place_kernel(const ID* __restrict__ ids,
                                                                     const int* __restrict__ counts, int* __restrict__ order,
                                                                     int* __restrict__ position, int* __restrict__ offsets,
                                                                     int R, int E, int runs) {
-    __shared__ int next[SORT_WAVES][SORT_MAX_E];
-    __shared__ int wave_sum[SORT_WAVES];
+    extern __shared__ int lds_sort[];                      // next[wave][e], then wave_sum
+    int* next = lds_sort;
+    int* wave_sum = lds_sort + WAVES * E;
+    constexpr int THREADS = 64 * WAVES;
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int s0 = blockIdx.x * SORT_SLOTS, here = min(R - s0, SORT_SLOTS);
-    const int w0 = s0 + wave * (SORT_SLOTS / SORT_WAVES);
+    const long long s0 = blockIdx.x * (long long)sort_slots(WAVES), w0 = s0 + wave * (64 * SORT_EACH);
     int e[SORT_EACH], rank[SORT_EACH], many[SORT_EACH];    // lanes of the same expert before this one; all, of the last
     experts_of(ids, w0, R, E, e);
-    for (int i = tid; i < E; i += SORT_THREADS)
-        for (int v = 0; v < SORT_WAVES; ++v) next[v][i] = 0;
+    for (int i = tid; i < WAVES * E; i += THREADS) next[i] = 0;
+    next += wave * E;                                      // this wave's
 #pragma unroll
     for (int i = 0; i < SORT_EACH; ++i) {
         if (w0 + 64 * i >= R) break;                       // nothing past here
@@ -85,17 +87,17 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
 #pragma unroll
     for (int i = 0; i < SORT_EACH; ++i) {
         if (w0 + 64 * i >= R) break;
-        if (many[i]) next[wave][e[i]] += many[i];          // one lane an expert
+        if (many[i]) next[e[i]] += many[i];          // one lane an expert
         wave_sync();
     }
     __syncthreads();
     int used = 0;
-    for (int e0 = 0; e0 < E; e0 += SORT_THREADS) {
+    for (int e0 = 0; e0 < E; e0 += THREADS) {
         const int x = e0 + tid;
         int all = 0, before = 0;                           // of all runs, and of those before this one
         if (x < E) {
             if constexpr (ONE) {
-                for (int v = 0; v < SORT_WAVES; ++v) all += next[v][x];
+                for (int v = 0; v < WAVES; ++v) all += lds_sort[v * E + x];
             } else {
 #pragma unroll 8
                 for (int b = 0; b < runs; ++b) {
@@ -114,16 +116,16 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
         if (lane == 63) wave_sum[wave] = sum;
         __syncthreads();
         int first = used + sum - all;
-        for (int v = 0; v < SORT_WAVES; ++v) {
+        for (int v = 0; v < WAVES; ++v) {
             if (v < wave) first += wave_sum[v];
             used += wave_sum[v];
         }
         if (x < E) {
             if (blockIdx.x == 0) offsets[x] = first;
             int at = first + before;                       // each wave's first row of the expert
-            for (int v = 0; v < SORT_WAVES; ++v) {
-                const int c = next[v][x];
-                next[v][x] = at;
+            for (int v = 0; v < WAVES; ++v) {
+                const int c = lds_sort[v * E + x];
+                lds_sort[v * E + x] = at;
                 at += c;
             }
         }
@@ -133,17 +135,17 @@ __global__ __launch_bounds__(SORT_THREADS) void expert_place_kernel(const ID* __
 #pragma unroll
     for (int i = 0; i < SORT_EACH; ++i) {
         if (w0 + 64 * i >= R) break;
-        const int s = w0 + 64 * i + lane;
+        const long long s = w0 + 64 * i + lane;
         int row = -1;
-        if (e[i] >= 0) row = next[wave][e[i]] + rank[i];
+        if (e[i] >= 0) row = next[e[i]] + rank[i];
         wave_sync();
-        if (many[i]) next[wave][e[i]] = row + 1;           // the last of them
+        if (many[i]) next[e[i]] = row + 1;           // the last of them
         wave_sync();
         if (s < R) position[s] = row;
-        if (row >= 0) order[row] = s;
+        if (row >= 0) order[row] = (int)s;
     }
-    for (int i = tid; i < here; i += SORT_THREADS)
-        if (s0 + i >= used) order[s0 + i] = -1;
+    for (int i = tid; i < sort_slots(WAVES); i += THREADS)
+        if (s0 + i < R && s0 + i >= used) order[s0 + i] = -1;
 }
 
 // Rows by the plan (a row number outside it is taken for an unused slot), 16
@@ -317,27 +319,42 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
 
 int expert_max() { return SORT_MAX_E; }
 
-size_t expert_sort_bytes(int R, int E) { return (size_t)((R + SORT_SLOTS - 1) / SORT_SLOTS) * E * sizeof(int); }
+static int sort_runs(int R) {
+    return R <= sort_slots(SORT_FEW) ? 1 : (int)((R + (long long)sort_slots(SORT_MANY) - 1) / sort_slots(SORT_MANY));
+}
+
+size_t expert_sort_bytes(int R, int E) { return (size_t)sort_runs(R) * E * sizeof(int); }
+
+template <typename ID, bool ONE, int WAVES>
+static hipError_t place_go(const ID* ids, const int* counts, int* order, int* position, int* offsets, int R, int E, int runs,
+                           hipStream_t st) {
+    static std::atomic<bool> attr[kMaxDev];
+    constexpr int MOST = WAVES * (SORT_MAX_E + 1) * (int)sizeof(int);
+    int dev = 0;
+    hipError_t e = current_device(&dev);
+    if (e != hipSuccess) return e;
+    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&expert_place_kernel<ID, ONE, WAVES>), MOST);
+    if (e != hipSuccess) return e;
+    hipLaunchKernelGGL((expert_place_kernel<ID, ONE, WAVES>), dim3(runs), dim3(64 * WAVES), WAVES * (E + 1) * sizeof(int), st,
+                       ids, counts, order, position, offsets, R, E, runs);
+    return hipGetLastError();
+}
 
 template <typename ID>
-static void sort_go(const void* ids, int* order, int* position, int* offsets, int* counts, int R, int E, hipStream_t st) {
-    const int runs = R > 0 ? (R + SORT_SLOTS - 1) / SORT_SLOTS : 1;
+static hipError_t sort_go(const void* ids, int* order, int* position, int* offsets, int* counts, int R, int E, hipStream_t st) {
+    const int runs = sort_runs(R);
     const ID* p = reinterpret_cast<const ID*>(ids);
-    if (runs == 1) {
-        hipLaunchKernelGGL((expert_place_kernel<ID, true>), dim3(1), dim3(SORT_THREADS), 0, st, p, counts, order, position,
-                           offsets, R, E, runs);
-        return;
-    }
-    hipLaunchKernelGGL((expert_count_kernel<ID>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, R, E);
-    hipLaunchKernelGGL((expert_place_kernel<ID, false>), dim3(runs), dim3(SORT_THREADS), 0, st, p, counts, order, position,
-                       offsets, R, E, runs);
+    if (R <= sort_slots(SORT_FEW)) return place_go<ID, true, SORT_FEW>(p, counts, order, position, offsets, R, E, runs, st);
+    if (runs == 1) return place_go<ID, true, SORT_MANY>(p, counts, order, position, offsets, R, E, runs, st);
+    hipLaunchKernelGGL((expert_count_kernel<ID>), dim3(runs), dim3(64 * SORT_MANY), 0, st, p, counts, R, E);
+    const hipError_t e = hipGetLastError();
+    return e != hipSuccess ? e : place_go<ID, false, SORT_MANY>(p, counts, order, position, offsets, R, E, runs, st);
 }
 
 hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R, int E,
                               hipStream_t st) {
-    if (id_bytes == 8) sort_go<long long>(ids, order, position, offsets, counts, R, E, st);
-    else sort_go<int>(ids, order, position, offsets, counts, R, E, st);
-    return hipGetLastError();
+    return id_bytes == 8 ? sort_go<long long>(ids, order, position, offsets, counts, R, E, st)
+                         : sort_go<int>(ids, order, position, offsets, counts, R, E, st);
 }
 
 // f(type code, vector pieces) for the row type; vector pieces where rows are whole 16-byte pieces
