@@ -86,6 +86,11 @@ def sort_tokens_by_expert(expert_ids: torch.Tensor, num_experts: int) -> ExpertP
     return ExpertPlan(order, position, offsets)
 
 
+def _no_tangent(what, *ts):
+    if native.has_tangent(*ts):
+        raise RuntimeError(f"{what} has no forward-mode gradient")
+
+
 def _gather(x, plan):
     lib = native.load_library()
     (T, k), D, E = plan.position.shape, x.shape[1], plan.num_experts
@@ -172,6 +177,7 @@ def gather_expert_rows(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     if x.dim() != 2 or x.shape[0] != plan.position.shape[0]:
         raise ValueError(f"x of shape {tuple(x.shape)} does not fit a plan of {plan.position.shape[0]} tokens")
     _same_device(x, plan.order)
+    _no_tangent("gather_expert_rows", x)
     if torch.is_grad_enabled() and x.requires_grad:
         return _Gather.apply(x, plan)
     return _gather(x, plan)
@@ -196,6 +202,7 @@ def combine_expert_rows(rows: torch.Tensor, weights: torch.Tensor, plan: ExpertP
     if tuple(weights.shape) != (T, k):
         raise ValueError(f"weights of shape {tuple(weights.shape)} do not fit: {(T, k)} expected")
     _same_device(rows, weights, plan.order)
+    _no_tangent("combine_expert_rows", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _Combine.apply(rows, weights, plan)
     return _combine(rows, native._aligned(weights.to(torch.float32)), plan)

@@ -42,7 +42,7 @@ def _check_dtype(t: torch.Tensor, what: str) -> int:
 
 
 def _no_grad(what: str, *ts) -> None:
-    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts):
+    if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in ts) or native.has_tangent(*ts):
         raise RuntimeError(f"{what} has no gradient: call it under torch.no_grad() or on detached tensors")
 
 

@@ -124,7 +124,9 @@ def load_library():
             raise RuntimeError(f"{os.path.basename(path)} has ABI version {ver()}, these bindings need "
                                f"{ABI_VERSION}; rebuild it with the package's _int4/build.py")
         for name, (args, res) in _SIGNATURES.items():
-            fn = getattr(lib, name)
+            fn = getattr(lib, name, None)
+            if fn is None:
+                raise RuntimeError(f"{os.path.basename(path)} has no {name}; rebuild it with the package's _int4/build.py")
             fn.argtypes = args
             fn.restype = res
         _lib = lib
@@ -132,6 +134,8 @@ def load_library():
 
 
 _host = None
+_HOST_FUNCTIONS = ("w4a4", "w8a8", "mx_quantize", "mx_dequantize", "mx_linear", "mx_expert_linear", "expert_sort",
+                   "expert_gather", "expert_combine")
 
 
 def host_module():
@@ -152,6 +156,9 @@ def host_module():
                     raise RuntimeError(f"{os.path.basename(path)} was built for ABI version "
                                        f"{getattr(mod, 'ABI_VERSION', None)}, these bindings need {ABI_VERSION}; "
                                        "rebuild it with the package's _int4/build.py")
+                if not all(hasattr(mod, name) for name in _HOST_FUNCTIONS):
+                    raise RuntimeError(f"{os.path.basename(path)} is older than these bindings; rebuild it with the "
+                                       "package's _int4/build.py")
                 _host = mod
     return _host
 
@@ -227,6 +234,12 @@ def on_device(device):
     the current device."""
     index = device.index
     return _same if index is None or index == torch.cuda.current_device() else torch.cuda.device(index)
+
+
+def has_tangent(*ts) -> bool:
+    """Whether a tensor carries a forward-mode gradient, which a kernel call would drop."""
+    return torch.autograd.forward_ad._current_level >= 0 and any(
+        t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
 # One reusable workspace per (device, stream): calls on a stream run in stream

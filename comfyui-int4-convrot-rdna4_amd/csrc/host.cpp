@@ -213,11 +213,11 @@ PyObject* w8a8(PyObject*, PyObject* const* a, Py_ssize_t n) {
 // linear through Python and ctypes, 9.9 here, where the kernel takes 9.5.
 // ---------------------------------------------------------------------------
 
-// A tensor for these paths: exactly torch.Tensor or Parameter, plain, on the current device.
+// A tensor for these paths: exactly torch.Tensor or Parameter, plain, on the current device, without a forward gradient.
 bool operand(PyObject* o, at::Tensor* t, c10::Device* dev, bool first = false) {
     if (!THPVariable_CheckExact(o)) return false;
     *t = THPVariable_Unpack(o);
-    if (!t->is_cuda()) return false;
+    if (!t->is_cuda() || t->_fw_grad(0).defined()) return false;
     if (first) {
         if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
         *dev = t->device();

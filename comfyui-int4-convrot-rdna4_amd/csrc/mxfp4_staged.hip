@@ -60,7 +60,7 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     const int nst = (p.K + 255) / 256;
     // a chunk past a row: its last one (past K the codes of A are 0)
     const uint32_t last_a = p.Kp / 2 - 16, last_w = p.K / 2 - 16;
-    const uint32_t a_step = p.as_rows * 16u, w_step = p.N * 16u;         // scales: from 512 k to the next
+    const size_t a_step = (size_t)p.as_rows * 16, w_step = (size_t)p.N * 16;      // scales: from 512 k to the next
     // whether copy j is of A: the same for all of a wave's where A's rows are whole waves'
     auto is_a = [&](int j) __attribute__((always_inline)) {
         return (wave * S::L + ((S::BM / 8) % S::L == 0 ? 0 : j)) * 8 < S::BM;
@@ -115,7 +115,7 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         for (int j = 0; j < S::NS; ++j) {
             const int i = min(wave * S::NS + j, FM + FN - 1);
             dma16_sv(lds0 + S::RING + ss % SLOTS * S::SCALES + i * 1024,
-                     i < FM ? AS + (size_t)ss * a_step : WS + (size_t)ss * w_step, soff[j]);
+                     i < FM ? AS + ss * a_step : WS + ss * w_step, soff[j]);
         }
     };
     v16f_mx acc[FM][FN];

@@ -252,3 +252,53 @@ def test_experts_in_a_graph(backend, gpu):
         graph.replay()
         torch.cuda.synchronize()
         assert torch.equal(out, layer(new, xt.roll(seed, 0)))
+
+
+def test_rows_past_32_bits(backend, gpu):
+    """Sorted rows of more than 2^32 bytes: gather, combine and their gradients on the last rows."""
+    T, k, D = 150000, 2, 8192
+    ids = torch.full((T, k), -1, dtype=torch.int64)
+    ids[:, 0] = 0
+    ids[-3:, 1] = 1
+    plan = backend.sort_tokens_by_expert(ids.cuda(), 2)
+    x = torch.zeros(T, D, dtype=torch.bfloat16, device="cuda")
+    x[-3:] = torch.randn(3, D, generator=torch.Generator().manual_seed(0)).to(torch.bfloat16).cuda()
+    rows = backend.gather_expert_rows(x, plan)
+    assert rows.numel() * 2 > 2 ** 32 and plan.offsets.tolist() == [0, T, T + 3]
+    assert torch.equal(rows[T:T + 3], x[-3:]) and torch.equal(rows[T - 3:T], x[-3:]) and int(rows[T + 3:].count_nonzero()) == 0
+    w = torch.ones(T, k, device="cuda")
+    out = backend.combine_expert_rows(rows, w, plan)
+    assert torch.equal(out[-3:], (2 * x[-3:].float()).to(torch.bfloat16)) and int(out[:-3].count_nonzero()) == 0
+    rows.requires_grad_()
+    (d_rows,) = torch.autograd.grad(backend.combine_expert_rows(rows, w, plan), rows, x)
+    assert torch.equal(d_rows[T:T + 3], x[-3:]) and int(d_rows[T + 3:].count_nonzero()) == 0
+
+
+def test_differentiating_twice_raises(backend, gpu):
+    ids, plan, x, rows, w = routed(backend, 6, 2, 3, 16, torch.float32, seed=1)
+    x, rows, w = (t.cuda().requires_grad_() for t in (x, rows, w))
+    for out, wrt in ((backend.gather_expert_rows(x, plan), x), (backend.combine_expert_rows(rows, w, plan), w)):
+        g = torch.randn_like(out).requires_grad_()
+        (first,) = torch.autograd.grad(out, wrt, g, create_graph=True)
+        with pytest.raises(RuntimeError, match="twice|once_differentiable"):
+            first.sum().backward()
+
+
+def test_python_path_gives_the_same(backend, native, gpu, monkeypatch):
+    """Without the host module the same calls run through Python: the same bits, forward and backward."""
+    ids, plan, x, rows, w = routed(backend, 30, 3, 5, 264, torch.bfloat16, seed=2)
+    x, rows, w = (t.cuda().requires_grad_() for t in (x, rows, w))
+    wc, ws = backend.quantize_mxfp4(torch.randn(5, 40, 264 // 8 * 8 - 8, device="cuda", generator=torch.Generator("cuda").manual_seed(1)))
+    a = x.detach()[:, :256].contiguous()
+
+    def calls():
+        p = backend.sort_tokens_by_expert(torch.from_numpy(ids).cuda(), 5)
+        g, c = backend.gather_expert_rows(x, p), backend.combine_expert_rows(rows, w, p)
+        grads = torch.autograd.grad((g, c), (x, rows, w), (torch.ones_like(g), torch.ones_like(c)))
+        codes = backend.quantize_mxfp4(a, 64)
+        return [*p, g, c, *grads, *codes, backend.dequantize_mxfp4(*codes, 64), backend.mxfp4_linear(a, wc[0], ws[0]),
+                backend.mxfp4_expert_linear(a, wc, ws, p)]
+
+    first = calls()
+    monkeypatch.setattr(native, "host_or_none", lambda: None)
+    assert all(torch.equal(p, q) for p, q in zip(first, calls()))

@@ -272,3 +272,48 @@ def test_linear_forms(backend, gpu):
         torch.cuda.synchronize()
         assert torch.equal(y, want.roll(i, 0))
         assert torch.equal(backend.mxfp4_linear(xt, w, s), want)      # the eager call between replays
+
+
+def test_forward_mode_is_refused(backend, gpu):
+    x, wc, ws = exact_operands(4, 32, 64, seed=2)
+    xt, w, s = torch.from_numpy(x).float().cuda(), torch.from_numpy(wc).cuda(), torch.from_numpy(ws).cuda()
+    with torch.autograd.forward_ad.dual_level():
+        dual = torch.autograd.forward_ad.make_dual(xt, torch.ones_like(xt))
+        with pytest.raises(RuntimeError, match="no gradient"):
+            backend.mxfp4_linear(dual, w, s)
+        with pytest.raises(RuntimeError, match="no gradient"):
+            backend.quantize_mxfp4(dual)
+        assert backend.mxfp4_linear(xt, w, s).shape == (4, 32)
+
+
+def test_gradients_are_refused_on_the_gpu(backend, gpu):
+    x = torch.zeros(4, 64, device="cuda", requires_grad=True)
+    w, s = torch.zeros(8, 32, dtype=torch.uint8, device="cuda"), torch.zeros(8, 2, dtype=torch.uint8, device="cuda")
+    with pytest.raises(RuntimeError, match="no gradient"):
+        backend.mxfp4_linear(x, w, s)
+    with pytest.raises(RuntimeError, match="no gradient"):
+        backend.quantize_mxfp4(x)
+    with torch.no_grad():
+        assert backend.mxfp4_linear(x, w, s).shape == (4, 8)
+
+
+def test_offsets_past_32_bits(backend, gpu):
+    """An input and an output of more than 2^32 bytes and 2^31 values: the last rows as a small call gives them."""
+    M, K, N = 80000, 64, 27008
+    x, wc, ws = exact_operands(256, N, K, seed=4)
+    w, s = torch.from_numpy(wc).cuda(), torch.from_numpy(ws).cuda()
+    xt = torch.from_numpy(x).to(torch.bfloat16).cuda()
+    want = backend.mxfp4_linear(xt, w, s)
+    y = backend.mxfp4_linear(xt.repeat(M // 256 + 1, 1)[:M], w, s)
+    assert y.numel() > 2 ** 31
+    for r0 in (0, 39936, M // 256 * 256 - 256):
+        assert torch.equal(y[r0:r0 + 256], want)
+    del y
+    big = torch.zeros(70000, 32768, dtype=torch.bfloat16, device="cuda")
+    big[-1] = torch.randn(32768, generator=torch.Generator().manual_seed(1)).to(torch.bfloat16).cuda()
+    codes, scales = backend.quantize_mxfp4(big)
+    small = backend.quantize_mxfp4(big[-1:])
+    assert torch.equal(codes[-1:], small[0]) and torch.equal(scales[-1:], small[1])
+    assert int(codes[:-1].count_nonzero()) == 0
+    back = backend.dequantize_mxfp4(codes, scales, output_dtype=torch.bfloat16)
+    assert torch.equal(back[-1:], backend.dequantize_mxfp4(*small, output_dtype=torch.bfloat16))
