@@ -216,12 +216,11 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         __builtin_amdgcn_fence(__ATOMIC_ACQUIRE, "wavefront");
     };
     constexpr int ES = DT == DT_F32 ? 4 : 2;
-    // The store goes through the ring, a quarter a wave: pieces of 32 rows by RB bytes, PR of them at a time.
-    constexpr int RB = 32 * FN * ES < 256 ? 32 * FN * ES : 256, CP = RB / ES, GROUPS = 32 * FN / CP;
-    constexpr int SCR = S::RING / 4, PIECES = FM * GROUPS, FIT = SCR / (32 * RB);
-    constexpr int PR = FIT >= PIECES ? PIECES : FIT >= PIECES / 2 ? PIECES / 2 : 1;
-    constexpr int U = RB / 16, ROWS = 64 / U;              // 16-byte units of a row, rows of a wave's store
-    static_assert(PR >= 1 && PIECES % PR == 0, "whole pieces");
+    // The store goes through the ring, a quarter a wave, in pieces of 32 rows by RB bytes, one after the other: while a
+    // piece's stores drain the next one is converted (all pieces at once: 8192 x 5120 -> 13824 315 us, so 309).
+    constexpr int RB = 32 * FN * ES < 256 ? 32 * FN * ES : 256, CP = RB / ES, GROUPS = 32 * FN / CP, PIECES = FM * GROUPS;
+    constexpr int SCR = 32 * RB, U = RB / 16, ROWS = 64 / U;       // 16-byte units of a row, rows of a wave's store
+    static_assert(4 * SCR <= S::RING, "a piece a wave fits the ring");
 
 #pragma unroll
     for (int ss = 0; ss < SLOTS / 2; ++ss)
@@ -284,61 +283,53 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
             const bool vec = (p.N * ES) % 16 == 0;
             float4 bv[CP / 8];
 #pragma unroll
-            for (int x0 = 0; x0 < PIECES; x0 += PR) {
+            for (int x = 0; x < PIECES; ++x) {
+                const int c = x / FM, i = x % FM;
+                if (i == 0) {
 #pragma unroll
-                for (int x = x0; x < x0 + PR; ++x) {
-                    const int c = x / FM, i = x % FM;
-                    if (i == 0) {
+                    for (int y = 0; y < CP / 8; ++y)
+                        bv[y] = *reinterpret_cast<const float4*>(biases + wn * 32 * FN + c * CP + y * 8 + 4 * eh);
+                }
 #pragma unroll
-                        for (int y = 0; y < CP / 8; ++y)
-                            bv[y] = *reinterpret_cast<const float4*>(biases + wn * 32 * FN + c * CP + y * 8 + 4 * eh);
-                    }
-#pragma unroll
-                    for (int y = 0; y < CP / 8; ++y) {
-                        const int jt = (c * CP + y * 8) / 32, g = y % 4;
-                        const int at = (y * 8 + 4 * eh) * ES;
-                        const float v0 = acc[i][jt][4 * g] + bv[y].x, v1 = acc[i][jt][4 * g + 1] + bv[y].y;
-                        const float v2 = acc[i][jt][4 * g + 2] + bv[y].z, v3 = acc[i][jt][4 * g + 3] + bv[y].w;
-                        uint8_t* d = scr + (x - x0) * 32 * RB + el * RB + (((at >> 4) ^ (el & (U - 1))) << 4) + (at & 15);
-                        if constexpr (DT == DT_F32) *reinterpret_cast<float4*>(d) = make_float4(v0, v1, v2, v3);
-                        else if constexpr (DT == DT_BF16)
-                            *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
-                        else *reinterpret_cast<uint2*>(d) = make_uint2(pack_f16x2(v0, v1), pack_f16x2(v2, v3));
-                    }
+                for (int y = 0; y < CP / 8; ++y) {
+                    const int jt = (c * CP + y * 8) / 32, g = y % 4;
+                    const int at = (y * 8 + 4 * eh) * ES;
+                    const float v0 = acc[i][jt][4 * g] + bv[y].x, v1 = acc[i][jt][4 * g + 1] + bv[y].y;
+                    const float v2 = acc[i][jt][4 * g + 2] + bv[y].z, v3 = acc[i][jt][4 * g + 3] + bv[y].w;
+                    uint8_t* d = scr + el * RB + (((at >> 4) ^ (el & (U - 1))) << 4) + (at & 15);
+                    if constexpr (DT == DT_F32) *reinterpret_cast<float4*>(d) = make_float4(v0, v1, v2, v3);
+                    else if constexpr (DT == DT_BF16)
+                        *reinterpret_cast<uint2*>(d) = make_uint2(pack_bf16x2(v0, v1), pack_bf16x2(v2, v3));
+                    else *reinterpret_cast<uint2*>(d) = make_uint2(pack_f16x2(v0, v1), pack_f16x2(v2, v3));
                 }
                 wave_sync();
-                // eight pieces read together: one by one, each store waited for its own read (11100 cycles a 256 x 256 tile)
-                constexpr int EIGHT = PR * (32 / ROWS) < 8 ? PR * (32 / ROWS) : 8;
+                // a piece's units read together: one by one, each store waited for its own read
+                v4u_mx w[32 / ROWS];
 #pragma unroll
-                for (int y0 = 0; y0 < PR * (32 / ROWS); y0 += EIGHT) {
-                    v4u_mx w[EIGHT];
+                for (int y = 0; y < 32 / ROWS; ++y) {
+                    const int row = y * ROWS + prow;
+                    w[y] = *reinterpret_cast<const v4u_mx*>(scr + row * RB + ((unit ^ (row & (U - 1))) << 4));
+                }
+                __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
-                    for (int y = 0; y < EIGHT; ++y) {
-                        const int x = (y0 + y) / (32 / ROWS), row = (y0 + y) % (32 / ROWS) * ROWS + prow;
-                        w[y] = *reinterpret_cast<const v4u_mx*>(scr + x * 32 * RB + row * RB + ((unit ^ (row & (U - 1))) << 4));
-                    }
-                    __builtin_amdgcn_sched_barrier(0);
+                for (int y = 0; y < 32 / ROWS; ++y) {
+                    const int m = m0 + i * 32 + y * ROWS + prow, col = c0 + c * CP + unit * (16 / ES);
+                    uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + col) * ES;
+                    // not kept in L2, where the next tiles' operands are
+                    if constexpr (!EDGE) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
+                    else if (m < m1 && col < p.N) {
+                        if (vec) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
+                        else {
 #pragma unroll
-                    for (int y = 0; y < EIGHT; ++y) {
-                        const int x = x0 + (y0 + y) / (32 / ROWS), row = (y0 + y) % (32 / ROWS) * ROWS + prow;
-                        const int m = m0 + x % FM * 32 + row, col = c0 + x / FM * CP + unit * (16 / ES);
-                        uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + col) * ES;
-                        // not kept in L2, where the next tiles' operands are
-                        if constexpr (!EDGE) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
-                        else if (m < m1 && col < p.N) {
-                            if (vec) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));
-                            else {
-#pragma unroll
-                                for (int e = 0; e < 16 / ES; ++e)
-                                    if (col + e < p.N) {
-                                        if constexpr (DT == DT_F32) reinterpret_cast<uint32_t*>(o)[e] = w[y][e];
-                                        else reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(w[y][e / 2] >> (16 * (e & 1)));
-                                    }
-                            }
+                            for (int e = 0; e < 16 / ES; ++e)
+                                if (col + e < p.N) {
+                                    if constexpr (DT == DT_F32) reinterpret_cast<uint32_t*>(o)[e] = w[y][e];
+                                    else reinterpret_cast<uint16_t*>(o)[e] = (uint16_t)(w[y][e / 2] >> (16 * (e & 1)));
+                                }
                         }
                     }
-                    __builtin_amdgcn_sched_barrier(0);
                 }
+                __builtin_amdgcn_sched_barrier(0);
                 wave_sync();
             }
         };
