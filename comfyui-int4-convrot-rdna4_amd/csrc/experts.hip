@@ -95,9 +95,13 @@ __global__ __launch_bounds__(64 * WAVES) void expert_place_kernel(const ID* __re
     for (int e0 = 0; e0 < E; e0 += THREADS) {
         const int x = e0 + tid;
         int all = 0, before = 0;                           // of all runs, and of those before this one
+        int own[WAVES];                                    // of this run's waves; read together
         if (x < E) {
+#pragma unroll
+            for (int v = 0; v < WAVES; ++v) own[v] = lds_sort[v * E + x];
             if constexpr (ONE) {
-                for (int v = 0; v < WAVES; ++v) all += lds_sort[v * E + x];
+#pragma unroll
+                for (int v = 0; v < WAVES; ++v) all += own[v];
             } else {
 #pragma unroll 8
                 for (int b = 0; b < runs; ++b) {
@@ -116,17 +120,19 @@ __global__ __launch_bounds__(64 * WAVES) void expert_place_kernel(const ID* __re
         if (lane == 63) wave_sum[wave] = sum;
         __syncthreads();
         int first = used + sum - all;
+#pragma unroll
         for (int v = 0; v < WAVES; ++v) {
-            if (v < wave) first += wave_sum[v];
-            used += wave_sum[v];
+            const int n = wave_sum[v];
+            if (v < wave) first += n;
+            used += n;
         }
         if (x < E) {
             if (blockIdx.x == 0) offsets[x] = first;
             int at = first + before;                       // each wave's first row of the expert
+#pragma unroll
             for (int v = 0; v < WAVES; ++v) {
-                const int c = lds_sort[v * E + x];
                 lds_sort[v * E + x] = at;
-                at += c;
+                at += own[v];
             }
         }
         __syncthreads();
