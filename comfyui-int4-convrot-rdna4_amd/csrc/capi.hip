@@ -49,6 +49,7 @@ hipError_t gemm_splitk_launch(const int8_t* Xp, const int8_t* Wp, const float* x
                               int M, int N, int K, int nsplit, hipStream_t st);
 hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int G, hipStream_t st);
 hipError_t mxfp4_operands_launch(const void* x, int G, const MxProblem& p, bool tiles, hipStream_t st);
+int mxfp4_gemm_tile(const MxProblem& p);
 bool mxfp4_gemm_staged(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
@@ -599,6 +600,15 @@ static int mx_linear_run(const void* x, int rows, int G, convrot::MxProblem p, v
 
 API size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E) {
     return M <= 0 || N <= 0 || E < 1 || K <= 0 || K % convrot::MX_BLOCK != 0 ? 0 : mx_plan(M, (long long)N * E, K).total;
+}
+
+API int cr_mxfp4_tile(int R, int N, int K, int experts) {
+    if (R < 0 || N < 0 || K <= 0 || K % convrot::MX_BLOCK != 0 || experts < 0) return -1;
+    static const int some = 0;
+    convrot::MxProblem p{};
+    p.R = p.as_rows = R; p.N = N; p.K = K; p.E = experts > 0 ? experts : 1;
+    p.offsets = experts > 0 ? &some : nullptr;                        // only asked whether it is there
+    return convrot::mxfp4_gemm_tile(p);
 }
 
 API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,

@@ -341,28 +341,30 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
 // The kernel of a product: 0 the one for few rows (mxfp4_gemm.hip), else the tile, 256 or 128 a side.
 //
 // Few rows run there up to 32, and up to one round of its workgroups of 64 x 32 outputs where there is one weight
-// (512 K, us: 4096 columns 64 rows 15.9, staged 20.2; 192 rows 25.7 and 20.6; 2048 columns of K 8192 256 rows 24 and 31);
-// experts' few rows leave most of such a workgroup idle (64 rows of 32 experts 35.9 and 35.1).
-// Tiles: rounds of the CUs times what a tile takes, measured at K 1600 to 8192: 256 a side, one a CU, 8 + 1.65 us a
-// stage of 256 k; 128 a side, two a CU, 7 + 0.83 us (13824 columns of K 5120: 512 rows 44.5 and 34.3 us, 1024 rows 52.2
-// and 58, 8192 rows 308 and 346; 2048 columns of K 8192: 4096 rows 70.4 and 64.8).
-static int staged_shape(const MxProblem& p) {
+// (us: 4096 columns of K 4096 64 rows 15.9, staged 20.2; 192 rows 25.7 and 20.6; 2048 columns of K 8192 256 rows 24 and
+// 31); experts' few rows leave most of such a workgroup idle (64 rows of 32 experts 35.9 and 35.1).
+// Tiles: rounds of the CUs times what a tile takes, fitted to K 1024 to 13824: 256 a side, one a CU, 12.5 + 1.4 us a
+// stage of 256 k; 128 a side, two a CU, 3.5 + 1.15 us, three quarters of that where a CU gets one.  us, 256 and 128:
+// 13824 columns of K 5120: 512 rows 38.7 and 31.6, 1024 rows 47.4 and 56.6, 1536 rows 82.2 and 78, 8192 rows 307 and 353;
+// 8192 columns of K 1024: 2048 rows 23.5 and 23.9, 8192 rows 86 and 74; 8 experts, 4096 columns of K 4096: 1024 rows 40
+// and 31, 2048 rows 43.5 and 47.4, 16384 rows 202 and 214.
+int mxfp4_gemm_tile(const MxProblem& p) {
     const bool ragged = p.offsets != nullptr;
     if (p.R <= 32) return 0;
     if (!ragged && (p.R + 63LL) / 64 * ((p.N + 31) / 32) <= 256) return 0;
     // the tokens' rows are addressed by 32-bit offsets from the first
     if (p.order != nullptr && (size_t)p.as_rows * (p.Kp / 2) >= (size_t(1) << 32)) return 0;
-    auto cost = [&](int side, int at_once, double fixed, double stage) {
-        // half a tile more for each expert that has rows
-        const double rows = ragged ? (double)p.R / side + 0.5 * (p.E < p.R ? p.E : p.R) : (double)((p.R + side - 1) / side);
-        const double tiles = rows * ((p.N + side - 1) / side);
-        const long long rounds = (long long)(tiles / at_once) + (tiles > (double)at_once * (long long)(tiles / at_once));
-        return rounds * (fixed + stage * ((p.K + 255) / 256));
+    auto tiles = [&](int side) {                           // half a tile more for each expert that has rows
+        const double rows = ragged ? (double)p.R / side + 0.5 * (p.E < p.R ? p.E : p.R) : (double)((p.R + (side - 1LL)) / side);
+        return (long long)(rows * ((p.N + side - 1) / side) + 0.5);
     };
-    return cost(256, 256, 8.0, 1.65) < cost(128, 512, 7.0, 0.83) ? 256 : 128;
+    const double stages = (p.K + 255) / 256;
+    const long long t128 = tiles(128), rest = t128 % 512;
+    const double rounds128 = (double)(t128 / 512) + (rest == 0 ? 0.0 : rest <= 256 ? 0.75 : 1.0);
+    return (tiles(256) + 255) / 256 * (12.5 + 1.4 * stages) < rounds128 * (3.5 + 1.15 * stages) ? 256 : 128;
 }
 
-bool mxfp4_gemm_staged(const MxProblem& p) { return staged_shape(p) != 0; }
+bool mxfp4_gemm_staged(const MxProblem& p) { return mxfp4_gemm_tile(p) != 0; }
 
 template <int DT, int FM, int FN, int SLOTS>
 static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
@@ -383,7 +385,7 @@ static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
 
 template <int DT>
 static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
-    if (staged_shape(p) == 256) return staged_go<DT, 4, 4, 2>(p, st);
+    if (mxfp4_gemm_tile(p) == 256) return staged_go<DT, 4, 4, 2>(p, st);
     // one tile a CU or fewer: nothing but its own copies hides a stage's latency
     const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 128) * ((p.N + 127) / 128);
     return tiles <= 256 ? staged_go<DT, 2, 2, 4>(p, st) : staged_go<DT, 2, 2, 2>(p, st);

@@ -191,9 +191,9 @@ def test_expert_linear_exact(backend, gpu, T, k, E, N, K, rows):
 
 
 @pytest.mark.parametrize("rows", [False, True], ids=["tokens", "sorted"])
-@pytest.mark.parametrize("T,k,E,N,K", [(2048, 2, 8, 4096, 288), (1500, 3, 70, 1000, 544)])
-def test_expert_linear_exact_large(backend, gpu, T, k, E, N, K, rows):
-    """Several rounds of tiles: 256 a side with eight experts, 128 with seventy."""
+@pytest.mark.parametrize("T,k,E,N,K,tile", [(7, 4, 9, 512, 320, 0), (1500, 3, 70, 1000, 544, 128), (1024, 2, 8, 4096, 2848, 256)])
+def test_expert_linear_exact_by_tile(backend, native, gpu, T, k, E, N, K, tile, rows):
+    assert native.load_library().cr_mxfp4_tile(T * k, N, K, E) == tile
     say("experts", T, k, E, N, K, rows)
     ids = choice(T, k, E, seed=T + N, skew=0.5)
     order, _, offsets = mx.plan(ids, E)

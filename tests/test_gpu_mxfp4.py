@@ -191,13 +191,15 @@ def test_linear_exact(backend, gpu, M, N, K):
         assert torch.equal(y.cpu(), torch.from_numpy(want + bias).float().to(dtype))
 
 
-# grids of more than one round of 128 x 128 tiles, and of 256 x 256 tiles; whole tiles, edges, and N that is no multiple
-# of a 16-byte piece
-LARGE_SHAPES = [(2100, 2304, 608), (2048, 2304, 1600), (3900, 4001, 352), (4096, 4096, 512), (4096, 4096, 1312)]
+# the kernel for few rows, one round of 128 x 128 tiles, more of them, and 256 x 256 tiles; whole tiles, edges, and N
+# that is no multiple of a 16-byte piece
+TILES = [(20, 512, 512, 0), (200, 700, 1600, 0), (300, 2400, 1600, 128), (2100, 2304, 608, 128), (4096, 4096, 512, 128),
+         (3900, 4001, 2336, 256), (4096, 4096, 2080, 256), (3000, 4096, 3840, 256)]
 
 
-@pytest.mark.parametrize("M,N,K", LARGE_SHAPES)
-def test_linear_exact_large(backend, gpu, M, N, K):
+@pytest.mark.parametrize("M,N,K,tile", TILES)
+def test_linear_exact_by_tile(backend, native, gpu, M, N, K, tile):
+    assert native.load_library().cr_mxfp4_tile(M, N, K, 0) == tile
     say("linear", M, N, K)
     x, wc, ws = exact_operands(M, N, K, seed=M + N + K)
     bias = torch.from_numpy(np.random.RandomState(1).randint(-64, 64, N) / 8.0).cuda()
