@@ -293,12 +293,10 @@ hipError_t mxfp4_gemm_fused_launch(const MxProblem& p, const void* x, int G, hip
     }
 }
 
-// x quantized with scales in rows.  Row tiles as high as an expert's rows are many on average.
+// x quantized with scales in rows.  32 rows a tile, 16 where one tile or an expert's rows on average are no more.
 hipError_t mxfp4_gemm_few_launch(const MxProblem& p, hipStream_t st) {
-    const int rows = p.offsets != nullptr ? (p.R + p.E - 1) / p.E : p.R;
-    if (rows <= (p.offsets != nullptr ? 8 : 16)) return few_go<0, 0, 1, 2, false>(p, nullptr, st);
-    if (rows <= (p.offsets != nullptr ? 24 : 32)) return few_go<0, 0, 2, 2, false>(p, nullptr, st);
-    return few_go<0, 0, 4, 2, false>(p, nullptr, st);
+    const int rows = p.offsets != nullptr ? 2 * ((p.R + p.E - 1) / p.E) : p.R;
+    return rows <= 16 ? few_go<0, 0, 1, 2, false>(p, nullptr, st) : few_go<0, 0, 2, 2, false>(p, nullptr, st);
 }
 
 }  // namespace convrot

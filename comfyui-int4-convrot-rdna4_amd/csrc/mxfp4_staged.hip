@@ -178,11 +178,13 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
             for (int x = 0; x < X; ++x) {
                 mfma_one(F[s & 1], C[q & 1], step, zero, x);
                 __builtin_amdgcn_sched_barrier(0);
-                if (x < Y) {
-                    if (s < 3) read_frag(F[(s + 1) & 1], here, (s + 1) & 3, x);
+                // one fragment after each MFMA while there are any, or all of them spread over fewer MFMAs
+#pragma unroll
+                for (int r = X < Y ? x * Y / X : x; r < (X < Y ? (x + 1) * Y / X : x < Y ? x + 1 : x); ++r) {
+                    if (s < 3) read_frag(F[(s + 1) & 1], here, (s + 1) & 3, r);
                     else {
-                        read_frag(F[0], next, 0, x);
-                        read_scale(C[(q + 1) & 1], sc_next, x);
+                        read_frag(F[0], next, 0, r);
+                        read_scale(C[(q + 1) & 1], sc_next, r);
                     }
                 }
                 if (s == 3 ? late : early) {
@@ -340,9 +342,8 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
 
 // The kernel of a product: 0 the one for few rows (mxfp4_gemm.hip), else the tile, 256 or 128 a side.
 //
-// Few rows run there up to 32, and up to one round of its workgroups of 64 x 32 outputs where there is one weight
-// (us: 4096 columns of K 4096 64 rows 15.9, staged 20.2; 192 rows 25.7 and 20.6; 2048 columns of K 8192 256 rows 24 and
-// 31); experts' few rows leave most of such a workgroup idle (64 rows of 32 experts 35.9 and 35.1).
+// Up to 32 rows run there (us, there and staged: 4096 columns of K 4096 12.6 and 13.8, 2048 of K 8192 16.2 and 17.9; with
+// 64 rows 16 and 14.1, 22.3 and 18).
 // Tiles: rounds of the CUs times what a tile takes, fitted to K 1024 to 13824: 256 a side, one a CU, 12.5 + 1.4 us a
 // stage of 256 k; 128 a side, two a CU, 3.5 + 1.15 us, three quarters of that where a CU gets one.  us, 256 and 128:
 // 13824 columns of K 5120: 512 rows 38.7 and 31.6, 1024 rows 47.4 and 56.6, 1536 rows 82.2 and 78, 8192 rows 307 and 353;
@@ -351,7 +352,6 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
 int mxfp4_gemm_tile(const MxProblem& p) {
     const bool ragged = p.offsets != nullptr;
     if (p.R <= 32) return 0;
-    if (!ragged && (p.R + 63LL) / 64 * ((p.N + 31) / 32) <= 256) return 0;
     // the tokens' rows are addressed by 32-bit offsets from the first
     if (p.order != nullptr && (size_t)p.as_rows * (p.Kp / 2) >= (size_t(1) << 32)) return 0;
     auto tiles = [&](int side) {                           // half a tile more for each expert that has rows
@@ -386,8 +386,10 @@ static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
 template <int DT>
 static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
     if (mxfp4_gemm_tile(p) == 256) return staged_go<DT, 4, 4, 2>(p, st);
-    // one tile a CU or fewer: nothing but its own copies hides a stage's latency
+    // One tile a CU or fewer: nothing but its own copies hides a stage's latency, so four slots; and where that leaves half
+    // of the CUs idle, tiles of half the rows (256 rows of K 4096 -> 4096: two slots 18, four 17, half the rows 15.1 us).
     const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 128) * ((p.N + 127) / 128);
+    if (tiles <= 128) return staged_go<DT, 1, 2, 4>(p, st);
     return tiles <= 256 ? staged_go<DT, 2, 2, 4>(p, st) : staged_go<DT, 2, 2, 2>(p, st);
 }
 

@@ -274,6 +274,21 @@ def test_rows_past_32_bits(backend, gpu):
     assert torch.equal(d_rows[T:T + 3], x[-3:]) and int(d_rows[T + 3:].count_nonzero()) == 0
 
 
+def test_tokens_past_32_bit_offsets(backend, native, gpu):
+    """Tokens whose codes take more than 2^32 bytes: the last ones' products as a small call gives them."""
+    T, K, N = 2 ** 21 + 37, 4096, 40
+    g = torch.Generator().manual_seed(1)
+    last = torch.randn(50, K, generator=g).to(torch.bfloat16).cuda()
+    wc, ws = backend.quantize_mxfp4(torch.randn(2, N, K, generator=g).cuda())
+    x = torch.zeros(T, K, dtype=torch.bfloat16, device="cuda")
+    x[-50:] = last
+    ids = torch.zeros(T, 1, dtype=torch.int64, device="cuda")
+    ids[-20:] = 1
+    y = backend.mxfp4_expert_linear(x, wc, ws, backend.sort_tokens_by_expert(ids, 2))
+    want = backend.mxfp4_expert_linear(last, wc, ws, backend.sort_tokens_by_expert(ids[-50:].contiguous(), 2))
+    assert torch.equal(y[-50:], want) and int(y[:-50].count_nonzero()) == 0
+
+
 def test_differentiating_twice_raises(backend, gpu):
     ids, plan, x, rows, w = routed(backend, 6, 2, 3, 16, torch.float32, seed=1)
     x, rows, w = (t.cuda().requires_grad_() for t in (x, rows, w))

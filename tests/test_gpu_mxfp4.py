@@ -191,9 +191,9 @@ def test_linear_exact(backend, gpu, M, N, K):
         assert torch.equal(y.cpu(), torch.from_numpy(want + bias).float().to(dtype))
 
 
-# the kernel for few rows, one round of 128 x 128 tiles, more of them, and 256 x 256 tiles; whole tiles, edges, and N
+# the kernel for few rows, 64 x 128 tiles, one round of 128 x 128 tiles, more of them, and 256 x 256 tiles; whole tiles, edges, and N
 # that is no multiple of a 16-byte piece
-TILES = [(20, 512, 512, 0), (200, 700, 1600, 0), (300, 2400, 1600, 128), (2100, 2304, 608, 128), (4096, 4096, 512, 128),
+TILES = [(20, 512, 512, 0), (200, 700, 1600, 128), (300, 2400, 1600, 128), (500, 5000, 416, 128), (2100, 2304, 608, 128), (4096, 4096, 512, 128),
          (3900, 4001, 2336, 256), (4096, 4096, 2080, 256), (3000, 4096, 3840, 256)]
 
 
