@@ -13,6 +13,13 @@
 // and stage cost twice the requests to L2, 16-byte pieces of the scales' rows a
 // quarter more: 8192^3 316 us with both), and why the scales are laid out by
 // columns of 512 k first.
+//
+// Measured on MI355X: 8192 x 5120 -> 13824 279 us in the kernel, 4.2 PFLOP/s; a
+// stage takes 2570 cycles, a tile 15000 more to set up (1800), fill (2600) and store
+// (11000), at 1.7 GHz, the clock that the card holds under this load.  A
+// workgroup that went from tile to tile, copying the next one's first stage while
+// it stored, measured slower: loads and stores share one counter, so the next
+// tile's first wait is for the stores too.
 
 #include <type_traits>
 
