@@ -12,8 +12,7 @@
 //
 // Measured on MI355X, kernel trace: 16384 x 5120 bf16 42.8 us (5.0 TB/s of values
 // in and codes out, the rate of a device copy; 28.7 with the values in the last
-// cache, 34.9 rotated in groups of 256 on top, so from memory the rotation hides
-// behind the loads); back to bf16 32 us (6.6 TB/s, the codes from cache); one row
+// cache, 34.9 rotated in groups of 256 on top); back to bf16 32 us (6.6 TB/s, the codes from cache); one row
 // 1.5 us each way, a launch's latency.
 
 #include "mxfp4_gemm.h"
