@@ -26,8 +26,7 @@ constexpr int DPP_XOR1 = 0xB1, DPP_XOR2 = 0x4E, DPP_XOR3 = 0x1B, DPP_ROR4 = 0x12
 
 // One base-4 digit of the rotation: y_a = (x_0 + x_1 + x_2 + x_3) / 2 - x_{3-a}
 // is row a of [[1,1,1,-1],[1,1,-1,1],[1,-1,1,1],[-1,1,1,1]] / 2, which is
-// orthogonal and its own inverse.  The sums are fp32; the halves are exact, so
-// nothing overflows that the result does not.
+// orthogonal and its own inverse.  The sums are fp32.
 __device__ __forceinline__ void digit4(float& a, float& b, float& c, float& d) {
     const float h = 0.5f * ((a + b) + (c + d));
     const float a1 = h - d, b1 = h - c, c1 = h - b, d1 = h - a;
@@ -37,9 +36,11 @@ __device__ __forceinline__ void digit4(float& a, float& b, float& c, float& d) {
 // The rotation in groups of G (0: none, 16, 64, 256) of values held 16
 // consecutive ones a lane, groups starting at a lane that is a multiple of
 // G/16: the low two digits are in the lane, the third is the lane's place in
-// its quad, the fourth the quad's place in its row of 16 lanes.
+// its quad, the fourth the quad's place in its row of 16 lanes.  Every digit
+// at most doubles a value, so no partial sum is more than 2 sqrt(G) <= 32 times
+// the group's largest value: below 2^122 none overflows.
 template <int G>
-__device__ __forceinline__ void rotate16(float (&v)[16]) {
+__device__ __forceinline__ void rotate_digits(float (&v)[16]) {
     if constexpr (G >= 16) {
 #pragma unroll
         for (int i = 0; i < 16; i += 4) digit4(v[i], v[i + 1], v[i + 2], v[i + 3]);
@@ -58,6 +59,39 @@ __device__ __forceinline__ void rotate16(float (&v)[16]) {
         for (int i = 0; i < 16; ++i) {
             const float s = v[i] + dpp<DPP_ROR8>(v[i]);
             v[i] = 0.5f * (s + dpp<DPP_ROR4>(s)) - dpp<DPP_XOR3>(dpp<DPP_MIRROR>(v[i]));   // mirror, xor 3: lane ^ 12
+        }
+    }
+}
+
+// Whether `p` holds in a lane of this lane's rotation group; `some`: of the wave.
+template <int G>
+__device__ __forceinline__ bool group_any(bool p, bool& some) {
+    const unsigned long long b = __ballot(p);
+    some = b != 0;
+    if constexpr (G <= 16) return p;
+    constexpr int L = G / 16;
+    return (b >> (threadIdx.x & 63 & ~(L - 1)) & ((1ull << L) - 1)) != 0;
+}
+
+// The rotation of any values: finite wherever the exact result is.  A group with
+// a value of 2^122 or more is rotated 2^-6 times as large, which is exact but for
+// bits below 2^-143.
+template <int G>
+__device__ __forceinline__ void rotate16(float (&v)[16]) {
+    if constexpr (G > 0) {
+        float m = __builtin_fabsf(v[0]);
+#pragma unroll
+        for (int i = 1; i < 16; ++i) m = fmaxf(m, __builtin_fabsf(v[i]));
+        bool some;
+        const bool large = group_any<G>(m >= 0x1p122f, some);
+        if (some) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] *= large ? 0x1p-6f : 1.0f;
+        }
+        rotate_digits<G>(v);
+        if (some) {
+#pragma unroll
+            for (int i = 0; i < 16; ++i) v[i] *= large ? 0x1p6f : 1.0f;
         }
     }
 }

@@ -112,7 +112,11 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
     // code -> value / 2: sign, exponent and mantissa bits moved to their places in a float whose
     // exponent 0 is a half unit (0 and 1 are 0 and .5: the mantissa bit counts 2^-2 there), times
     // 2^126, which makes subnormal numbers of the moved bits normal ones.
-    const float scale = sb == 255u ? __builtin_nanf("") : sb == 0u ? 0x1p-127f : __uint_as_float(sb << 23);
+    float scale = sb == 255u ? __builtin_nanf("") : sb == 0u ? 0x1p-127f : __uint_as_float(sb << 23);
+    // as rotate16; by the scale, since 2^126 times a code's value can be past fp32 where the rotated values are not
+    bool some = false;
+    const bool large = G > 0 && group_any<G>(sb >= 240u, some);
+    if (some) scale *= large ? 0x1p-8f : 1.0f;
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) {
@@ -120,7 +124,11 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
         const float m = __uint_as_float(((n & 8u) << 28) | ((n & 7u) << 22));
         v[i] = (m * 0x1p126f) * scale;
     }
-    rotate16<G>(v);
+    rotate_digits<G>(v);
+    if (some) {
+#pragma unroll
+        for (int i = 0; i < 16; ++i) v[i] *= large ? 0x1p8f : 1.0f;
+    }
     if (u >= units) return;
     uint8_t* o = out + (size_t)u * 16 * ES;
     if constexpr (DT == DT_F32) {
