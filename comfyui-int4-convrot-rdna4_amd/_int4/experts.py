@@ -106,58 +106,72 @@ def _gather(x, plan):
     return rows
 
 
-def _combine(rows, weights, plan):
+def _combine(rows, weights, position):
     lib = native.load_library()
-    (T, k), D = plan.position.shape, rows.shape[1]
+    (T, k), D = position.shape, rows.shape[1]
     rows = native._aligned(rows)
     out = torch.empty((T, D), dtype=rows.dtype, device=rows.device)
     if D == 0:
         return out
     with native.on_device(rows.device):
         rc = lib.cr_expert_combine(rows.data_ptr(), native._IN_DTYPE_CODE[rows.dtype], native._ptr(weights),
-                                   plan.position.data_ptr(), out.data_ptr(), T, k, D, native._stream(rows.device))
+                                   position.data_ptr(), out.data_ptr(), T, k, D, native._stream(rows.device))
     if rc != 0:
         raise RuntimeError(f"cr_expert_combine failed, hipError={rc}")
     return out
 
 
+def _restored(t, what, dtype, shape, device):
+    """A saved tensor as the kernels take it: hooks on saved tensors may hand back
+    another one than was saved."""
+    if type(t) not in (torch.Tensor, torch.nn.Parameter) or t.layout != torch.strided or t.dtype != dtype \
+            or tuple(t.shape) != tuple(shape) or t.device != device:
+        raise RuntimeError(f"the saved {what} came back in another form: {dtype} {tuple(shape)} on {device} expected, got "
+                           f"{t.dtype} {tuple(t.shape)} on {t.device}")
+    return native._aligned(t)
+
+
 class _Gather(torch.autograd.Function):
     @staticmethod
     def forward(ctx, x, plan):
-        ctx.plan = plan
+        ctx.save_for_backward(plan.position)
+        ctx.slots = plan.position.shape
         return _gather(x, plan)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_rows):
-        return _combine(d_rows, None, ctx.plan), None
+        position = _restored(ctx.saved_tensors[0], "positions", torch.int32, ctx.slots, d_rows.device)
+        return _combine(d_rows, None, position), None
 
 
 class _Combine(torch.autograd.Function):
     @staticmethod
     def forward(ctx, rows, weights, plan):
         w = native._aligned(weights.to(torch.float32))
-        ctx.save_for_backward(rows, w)
-        ctx.plan, ctx.weights_dtype = plan, weights.dtype
-        return _combine(rows, w, plan)
+        ctx.save_for_backward(rows, w, plan.position, plan.offsets)
+        ctx.slots, ctx.offsets, ctx.weights_dtype = plan.position.shape, plan.offsets.shape, weights.dtype
+        return _combine(rows, w, plan.position)
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, d_out):
-        rows, w = ctx.saved_tensors
-        plan = ctx.plan
-        (T, k), D, E = plan.position.shape, rows.shape[1], plan.num_experts
+        rows, w, position, offsets = ctx.saved_tensors
+        (T, k), D, E, dev = ctx.slots, d_out.shape[1], ctx.offsets[0] - 1, d_out.device
+        rows = _restored(rows, "rows", d_out.dtype, (T * k, D), dev)
+        w = _restored(w, "weights", torch.float32, ctx.slots, dev)
+        position = _restored(position, "positions", torch.int32, ctx.slots, dev)
+        offsets = _restored(offsets, "offsets", torch.int32, ctx.offsets, dev)
         need_rows, need_weights = ctx.needs_input_grad[:2]
-        rows, d_out = native._aligned(rows), native._aligned(d_out)
+        d_out = native._aligned(d_out)
         d_rows = torch.empty_like(rows) if need_rows else None
-        d_w = torch.empty((T, k), dtype=torch.float32, device=rows.device) if need_weights else None
+        d_w = torch.empty((T, k), dtype=torch.float32, device=dev) if need_weights else None
         if D == 0:
             return d_rows, None if d_w is None else d_w.zero_().to(ctx.weights_dtype), None
-        with native.on_device(rows.device):
+        with native.on_device(dev):
             rc = native.load_library().cr_expert_combine_grad(
-                rows.data_ptr(), native._IN_DTYPE_CODE[rows.dtype], w.data_ptr(), plan.position.data_ptr(),
-                plan.offsets.data_ptr(), d_out.data_ptr(), native._ptr(d_rows), native._ptr(d_w), T, k, E, D,
-                native._stream(rows.device))
+                rows.data_ptr(), native._IN_DTYPE_CODE[rows.dtype], w.data_ptr(), position.data_ptr(), offsets.data_ptr(),
+                d_out.data_ptr(), native._ptr(d_rows), native._ptr(d_w), T, k, E, D, native._stream(dev))
         if rc != 0:
             raise RuntimeError(f"cr_expert_combine_grad failed, hipError={rc}")
         return d_rows, None if d_w is None else d_w.to(ctx.weights_dtype), None
@@ -205,4 +219,4 @@ def combine_expert_rows(rows: torch.Tensor, weights: torch.Tensor, plan: ExpertP
     _no_tangent("combine_expert_rows", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):
         return _Combine.apply(rows, weights, plan)
-    return _combine(rows, native._aligned(weights.to(torch.float32)), plan)
+    return _combine(rows, native._aligned(weights.to(torch.float32)), plan.position)

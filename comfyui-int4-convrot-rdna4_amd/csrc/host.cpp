@@ -422,6 +422,21 @@ at::Tensor settled(const at::Tensor& t) {
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 != 0 ? c.clone() : c;
 }
 
+// A saved tensor as the kernels take it: hooks on saved tensors may hand back another one than was saved.
+at::Tensor restored(const at::Tensor& t, const char* what, at::ScalarType type, at::IntArrayRef sizes, c10::Device dev) {
+    TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.device() == dev && t.scalar_type() == type && t.sizes() == sizes,
+                "the saved ", what, " came back in another form: ", type, " ", sizes, " on ", dev, " expected, got ",
+                t.toString(), " ", t.sizes(), " on ", t.device());
+    return settled(t.detach());
+}
+
+// The saved positions [T, k] of T tokens' slots, or of any number of tokens (T < 0)
+at::Tensor restored_position(const at::Tensor& t, int64_t T, c10::Device dev) {
+    TORCH_CHECK(t.dim() == 2 && t.size(1) >= 1 && t.numel() <= INT32_MAX && (T < 0 || t.size(0) == T),
+                "the saved positions came back in another form: ", t.sizes());
+    return restored(t, "positions", at::kInt, t.sizes(), dev);
+}
+
 // Gradients that cannot be differentiated again: where a graph of them is built, using it raises.
 torch::autograd::variable_list once(torch::autograd::variable_list grads) {
     if (!at::GradMode::is_enabled()) return grads;
@@ -449,7 +464,9 @@ struct GatherRows : torch::autograd::Function<GatherRows> {
         at::Tensor d_x;
         {
             at::NoGradGuard no_grad;
-            d_x = combine_rows(settled(g[0]), at::Tensor(), ctx->get_saved_variables()[0]);
+            const at::Tensor position = restored_position(ctx->get_saved_variables()[0], -1, g[0].device());
+            TORCH_CHECK(position.numel() == g[0].size(0), "the saved positions came back in another form: ", position.sizes());
+            d_x = combine_rows(settled(g[0]), at::Tensor(), position);
         }
         return once({d_x, at::Tensor(), at::Tensor()});
     }
@@ -459,6 +476,7 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
     static at::Tensor forward(torch::autograd::AutogradContext* ctx, const at::Tensor& rows, const at::Tensor& weights,
                               const at::Tensor& position, const at::Tensor& offsets) {
         ctx->save_for_backward({rows, weights, position, offsets});
+        ctx->saved_data["offsets"] = offsets.numel();
         return combine_rows(rows, weights, position);
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
@@ -466,8 +484,12 @@ struct CombineRows : torch::autograd::Function<CombineRows> {
         {
             at::NoGradGuard no_grad;
             const auto saved = ctx->get_saved_variables();
-            const at::Tensor rows = saved[0].detach(), w = saved[1].detach(), &position = saved[2], &offsets = saved[3];
-            const at::Tensor d_out = settled(g[0]);
+            const at::Tensor d_out = settled(g[0]);                      // [T, D], which autograd has checked
+            const c10::Device dev = d_out.device();
+            const at::Tensor position = restored_position(saved[2], d_out.size(0), dev);
+            const at::Tensor rows = restored(saved[0], "rows", d_out.scalar_type(), {position.numel(), d_out.size(1)}, dev);
+            const at::Tensor w = restored(saved[1], "weights", at::kFloat, position.sizes(), dev);
+            const at::Tensor offsets = restored(saved[3], "offsets", at::kInt, {ctx->saved_data["offsets"].toInt()}, dev);
             if (ctx->needs_input_grad(0)) d_rows = like(rows, rows.sizes(), rows.scalar_type());
             if (ctx->needs_input_grad(1)) d_w = like(w, w.sizes(), at::kFloat);
             const int rc = cr_expert_combine_grad(
