@@ -58,6 +58,7 @@ def sort_tokens_by_expert(expert_ids: torch.Tensor, num_experts: int) -> ExpertP
         p = None if host is None else host.expert_sort(expert_ids, num_experts)
         if p is not None:
             return ExpertPlan(*p)
+    native.check_runs("sort_tokens_by_expert", expert_ids)
     if expert_ids.dim() != 2 or expert_ids.shape[1] < 1:
         raise ValueError(f"expert_ids must be [T, k], got shape {tuple(expert_ids.shape)}")
     if expert_ids.dtype not in (torch.int32, torch.int64):
@@ -186,6 +187,7 @@ def gather_expert_rows(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
         rows = None if host is None else host.expert_gather(x, plan.order, plan.position, plan.offsets)
         if rows is not None:
             return rows
+    native.check_runs("gather_expert_rows", x, *plan)
     _check_dtype(x, "x")
     plan.check()
     if x.dim() != 2 or x.shape[0] != plan.position.shape[0]:
@@ -207,6 +209,7 @@ def combine_expert_rows(rows: torch.Tensor, weights: torch.Tensor, plan: ExpertP
         out = None if host is None else host.expert_combine(rows, weights, plan.order, plan.position, plan.offsets)
         if out is not None:
             return out
+    native.check_runs("combine_expert_rows", rows, weights, *plan)
     _check_dtype(rows, "rows")
     _check_dtype(weights, "weights")
     plan.check()

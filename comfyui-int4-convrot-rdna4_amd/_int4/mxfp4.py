@@ -65,6 +65,7 @@ def quantize_mxfp4(x: torch.Tensor, convrot_groupsize: int | None = None) -> tup
         q = None if host is None else host.mx_quantize(x, convrot_groupsize)
         if q is not None:
             return q
+    native.check_runs("quantize_mxfp4", x)
     dt = _check_dtype(x, "x")
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -96,6 +97,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, convrot_groupsiz
                                                          native._IN_DTYPE_CODE[output_dtype])
         if x is not None:
             return x
+    native.check_runs("dequantize_mxfp4", codes, scales)
     if output_dtype not in native._IN_DTYPE_CODE:
         raise ValueError(f"output_dtype must be float32, bfloat16 or float16, got {output_dtype}")
     _check_operand(codes, scales, codes.shape[:-1], codes.shape[-1] * 2 if codes.dim() else 0, "codes")
@@ -126,6 +128,7 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
         y = None if host is None else host.mx_linear(x, qweight, wscales, bias, convrot_groupsize)
         if y is not None:
             return y
+    native.check_runs("mxfp4_linear", x, qweight, wscales, bias)
     dt = _check_dtype(x, "x")
     if x.dim() == 0:
         raise ValueError("x must have at least one dimension")
@@ -175,6 +178,7 @@ def mxfp4_expert_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.T
                                                             bias, convrot_groupsize, sorted_rows)
         if y is not None:
             return y
+    native.check_runs("mxfp4_expert_linear", x, qweight, wscales, bias, *plan)
     dt = _check_dtype(x, "x")
     if x.dim() != 2:
         raise ValueError(f"x must be 2-D, got shape {tuple(x.shape)}")

@@ -243,6 +243,27 @@ def has_tangent(*ts) -> bool:
         t is not None and torch.autograd.forward_ad.unpack_dual(t).tangent is not None for t in ts)
 
 
+_TRACING_MODES = tuple(getattr(torch._C._TorchDispatchModeKey, k) for k in ("PROXY", "FAKE", "FUNCTIONAL"))
+
+
+def check_runs(what: str, *ts) -> None:
+    """Raises where the call would not run on real tensors: a trace would record
+    the empty outputs and not the kernels that fill them, and a tensor without
+    memory (of a fake or functional mode, a wrapper) has a null pointer."""
+    if torch.jit.is_tracing() or any(torch._C._get_dispatch_mode(k) is not None for k in _TRACING_MODES):
+        raise RuntimeError(f"{what} cannot be traced: its kernels are no torch operations")
+    for t in ts:
+        if t is not None:
+            _check_memory(t)
+
+
+def _check_memory(t: torch.Tensor) -> torch.Tensor:
+    if t.data_ptr() == 0 and t.numel() != 0:
+        raise RuntimeError(f"the tensor of shape {tuple(t.shape)} on {t.device} has no memory of its own "
+                           f"({type(t).__name__})")
+    return t
+
+
 # One reusable workspace per (device, stream): calls on a stream run in stream
 # order, so a call may reuse the workspace of the previous call on the same
 # stream; calls on other streams get their own.  It only grows.  A dropped
@@ -303,7 +324,7 @@ def _check_cuda(*ts):
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
     """Contiguous and 16-byte aligned (the kernels use 128-bit loads/stores)."""
-    t = t.contiguous()
+    t = _check_memory(t.contiguous())
     if t.data_ptr() % 16:
         t = t.clone()
     return t

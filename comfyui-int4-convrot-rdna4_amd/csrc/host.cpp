@@ -18,6 +18,7 @@
 #include <torch/csrc/autograd/custom_function.h>
 #include <torch/csrc/autograd/functions/basic_ops.h>
 #include <torch/csrc/autograd/python_variable.h>
+#include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ATen.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
@@ -39,10 +40,11 @@ int dtype_code(const at::Tensor& t) {
 
 constexpr int kEpiF16 = 5;
 
-// A plain strided GPU tensor on `dev`, contiguous, its data 16-byte aligned.
+// A plain strided GPU tensor on `dev`, contiguous, its data 16-byte aligned and there (a functional tensor's is not).
 bool plain(const at::Tensor& t, c10::Device dev) {
     return t.defined() && t.layout() == at::kStrided && t.device() == dev && !t.is_neg() && t.has_storage() &&
-           t.is_contiguous() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
+           t.is_contiguous() && (t.const_data_ptr() != nullptr || t.numel() == 0) &&
+           reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0;
 }
 
 // None, or a tensor of exactly torch.Tensor / Parameter type; false for other objects
@@ -220,7 +222,7 @@ bool operand(PyObject* o, at::Tensor* t, c10::Device* dev, bool first = false) {
     *t = THPVariable_Unpack(o);
     if (!t->is_cuda() || t->_fw_grad(0).defined()) return false;
     if (first) {
-        if (c10::impl::TorchDispatchModeTLS::any_modes_set()) return false;
+        if (c10::impl::TorchDispatchModeTLS::any_modes_set() || torch::jit::tracer::isTracing()) return false;
         *dev = t->device();
         if (dev->index() != c10::hip::current_device()) return false;
     }
