@@ -36,7 +36,7 @@ class ExpertPlan(NamedTuple):
     def check(self, E: int | None = None) -> None:
         """Raises ValueError where the tensors are no plan (of E experts)."""
         o, p, f = self.order, self.position, self.offsets
-        if any(t.dtype != torch.int32 or not t.is_contiguous() for t in (o, p, f)) or p.dim() != 2 or o.dim() != 1 \
+        if any(t.dtype != torch.int32 or not t.is_contiguous() or t.is_neg() for t in (o, p, f)) or p.dim() != 2 or o.dim() != 1 \
                 or f.dim() != 1 or o.shape[0] != p.numel() or f.shape[0] < 2 or p.shape[1] < 1 \
                 or not (o.device == p.device == f.device):
             raise ValueError("a plan is contiguous int32 tensors order [T k], position [T, k] and offsets [E + 1] of one "
@@ -67,7 +67,7 @@ def sort_tokens_by_expert(expert_ids: torch.Tensor, num_experts: int) -> ExpertP
     lib = native.load_library()
     if not 1 <= num_experts <= max_experts():
         raise ValueError(f"num_experts must be 1 to {max_experts()}, got {num_experts}")
-    ids = expert_ids.contiguous()
+    ids = native._aligned(expert_ids)
     T, k = ids.shape
     R = T * k
     if R >= 1 << 31:

@@ -323,8 +323,9 @@ def _check_cuda(*ts):
 
 
 def _aligned(t: torch.Tensor) -> torch.Tensor:
-    """Contiguous and 16-byte aligned (the kernels use 128-bit loads/stores)."""
-    t = _check_memory(t.contiguous())
+    """Contiguous and 16-byte aligned (the kernels use 128-bit loads/stores), a
+    lazily negated view written out."""
+    t = _check_memory((t.resolve_neg() if t.is_neg() else t).contiguous())
     if t.data_ptr() % 16:
         t = t.clone()
     return t

@@ -418,9 +418,9 @@ at::Tensor combine_rows(const at::Tensor& rows, const at::Tensor& weights, const
     return out;
 }
 
-// A gradient's own form: contiguous, aligned, on the device whose current stream the backward runs on
+// A gradient's own form: its values as they are read, contiguous, aligned
 at::Tensor settled(const at::Tensor& t) {
-    at::Tensor c = t.contiguous();
+    at::Tensor c = t.resolve_neg().contiguous();
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 != 0 ? c.clone() : c;
 }
 
