@@ -17,7 +17,7 @@ from typing import NamedTuple
 import torch
 
 from . import native
-from .mxfp4 import _check_dtype, _same_device
+from .mxfp4 import _check_dtype, _count, _same_device
 
 
 class ExpertPlan(NamedTuple):
@@ -41,6 +41,8 @@ class ExpertPlan(NamedTuple):
                 or not (o.device == p.device == f.device):
             raise ValueError("a plan is contiguous int32 tensors order [T k], position [T, k] and offsets [E + 1] of one "
                              f"device, got {tuple(o.shape)}, {tuple(p.shape)}, {tuple(f.shape)}")
+        if o.shape[0] >= 1 << 31:
+            raise ValueError(f"{o.shape[0]} slots are more than one plan holds (2^31 - 1)")
         if E is not None and f.shape[0] != E + 1:
             raise ValueError(f"the plan is of {f.shape[0] - 1} experts, the weights are of {E}")
 
@@ -192,6 +194,7 @@ def gather_expert_rows(x: torch.Tensor, plan: ExpertPlan) -> torch.Tensor:
     plan.check()
     if x.dim() != 2 or x.shape[0] != plan.position.shape[0]:
         raise ValueError(f"x of shape {tuple(x.shape)} does not fit a plan of {plan.position.shape[0]} tokens")
+    _count(x.shape[1], "columns")
     _same_device(x, plan.order)
     _no_tangent("gather_expert_rows", x)
     if torch.is_grad_enabled() and x.requires_grad:
@@ -218,6 +221,7 @@ def combine_expert_rows(rows: torch.Tensor, weights: torch.Tensor, plan: ExpertP
         raise ValueError(f"rows of shape {tuple(rows.shape)} do not fit a plan of {T * k} rows")
     if tuple(weights.shape) != (T, k):
         raise ValueError(f"weights of shape {tuple(weights.shape)} do not fit: {(T, k)} expected")
+    _count(rows.shape[1], "columns")
     _same_device(rows, weights, plan.order)
     _no_tangent("combine_expert_rows", rows, weights)
     if torch.is_grad_enabled() and (rows.requires_grad or weights.requires_grad):

@@ -20,11 +20,14 @@ import torch
 from . import native
 
 _BLOCK = 32
+_MAX_K = 1 << 24             # widest row that the library takes
 
 
 def _check_group(K: int, convrot_groupsize: int | None, what: str = "in_features") -> int:
     if K == 0 or K % _BLOCK:
         raise ValueError(f"{what} {K} is not a multiple of {_BLOCK}, the values that share a scale")
+    if K > _MAX_K:
+        raise ValueError(f"{what} {K} is too wide: at most {_MAX_K}")
     if convrot_groupsize is None:
         return 0
     if convrot_groupsize not in (16, 64, 256):
@@ -71,15 +74,15 @@ def quantize_mxfp4(x: torch.Tensor, convrot_groupsize: int | None = None) -> tup
         raise ValueError("x must have at least one dimension")
     K = x.shape[-1]
     G = _check_group(K, convrot_groupsize)
+    M = _count(x.numel() // K, "rows")
     _no_grad("quantize_mxfp4", x)
     dev = x.device
     lib = native.load_library()
     xg = native._aligned(_on_gpu(x))
-    M = xg.numel() // K
     codes = torch.empty((*x.shape[:-1], K // 2), dtype=torch.uint8, device=xg.device)
     scales = torch.empty((*x.shape[:-1], K // _BLOCK), dtype=torch.uint8, device=xg.device)
     with native.on_device(xg.device):
-        rc = lib.cr_mxfp4_quant(xg.data_ptr(), dt, codes.data_ptr(), scales.data_ptr(), _rows(M), K, G,
+        rc = lib.cr_mxfp4_quant(xg.data_ptr(), dt, codes.data_ptr(), scales.data_ptr(), M, K, G,
                                 native._stream(xg.device))
     if rc != 0:
         raise RuntimeError(f"cr_mxfp4_quant failed, hipError={rc}")
@@ -103,6 +106,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, convrot_groupsiz
     _check_operand(codes, scales, codes.shape[:-1], codes.shape[-1] * 2 if codes.dim() else 0, "codes")
     K = codes.shape[-1] * 2
     G = _check_group(K, convrot_groupsize)
+    M = _count(codes.numel() * 2 // K, "rows")
     dev = codes.device
     lib = native.load_library()
     c, s = native._aligned(_on_gpu(codes)), native._aligned(_on_gpu(scales))
@@ -110,7 +114,7 @@ def dequantize_mxfp4(codes: torch.Tensor, scales: torch.Tensor, convrot_groupsiz
     out = torch.empty((*codes.shape[:-1], K), dtype=output_dtype, device=c.device)
     with native.on_device(c.device):
         rc = lib.cr_mxfp4_dequant(c.data_ptr(), s.data_ptr(), out.data_ptr(), native._IN_DTYPE_CODE[output_dtype],
-                                  _rows(out.numel() // K), K, G, native._stream(c.device))
+                                  M, K, G, native._stream(c.device))
     if rc != 0:
         raise RuntimeError(f"cr_mxfp4_dequant failed, hipError={rc}")
     return out if out.device == dev else out.to(dev)
@@ -138,7 +142,7 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     if qweight.shape[-1] * 2 != K:
         raise ValueError(f"Input K={K} does not match qweight K={qweight.shape[-1] * 2}")
     G = _check_group(K, convrot_groupsize)
-    N = qweight.shape[0]
+    M, N = _count(x.numel() // K, "rows"), _count(qweight.shape[0], "columns")
     _check_operand(qweight, wscales, (N,), K, "qweight")
     bdt = _check_bias(bias, (N,))
     _no_grad("mxfp4_linear", x, bias)
@@ -147,7 +151,6 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     x2 = native._aligned(x)
     w, ws = native._aligned(qweight), native._aligned(wscales)
     b = None if bias is None else native._aligned(bias)
-    M = _rows(x2.numel() // K)
     out = torch.empty((*x.shape[:-1], N), dtype=x.dtype, device=x.device)
     nbytes = lib.cr_mxfp4_linear_workspace(M, N, K, 1)
     st = native._stream(x.device)
@@ -188,9 +191,11 @@ def mxfp4_expert_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.T
     if qweight.shape[-1] * 2 != K:
         raise ValueError(f"Input K={K} does not match qweight K={qweight.shape[-1] * 2}")
     G = _check_group(K, convrot_groupsize)
-    E, N = qweight.shape[:2]
+    E, N = qweight.shape[0], _count(qweight.shape[1], "columns")
     _check_operand(qweight, wscales, (E, N), K, "qweight")
     plan.check(E)
+    if E > native._limit("cr_max_experts"):
+        raise ValueError(f"{E} experts are too many: at most {native._limit('cr_max_experts')} experts")
     T, k = plan.position.shape
     R = T * k
     if x.shape[0] != (R if sorted_rows else T):
@@ -224,10 +229,10 @@ def _on_gpu(t: torch.Tensor) -> torch.Tensor:
     return t.to("cuda")
 
 
-def _rows(M: int) -> int:
-    if M >= 1 << 31:
-        raise ValueError(f"{M} rows are more than one call takes (2^31 - 1)")
-    return M
+def _count(n: int, what: str) -> int:
+    if n >= 1 << 31:
+        raise ValueError(f"{n} {what} are more than one call takes (2^31 - 1)")
+    return n
 
 
 def _check_operand(codes, scales, rows, K: int, what: str) -> None:

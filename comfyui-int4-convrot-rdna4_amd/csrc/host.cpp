@@ -231,9 +231,9 @@ bool operand(PyObject* o, at::Tensor* t, c10::Device* dev, bool first = false) {
 
 bool wants_grad(const at::Tensor& t) { return t.defined() && t.requires_grad() && at::GradMode::is_enabled(); }
 
-// None -> 0, 16, 64 or 256; -1: not one of them, or K is not whole groups and blocks
+// None -> 0, 16, 64 or 256; -1: not one of them, or K is not whole groups and blocks or past what the library takes
 int mx_group(PyObject* o, int64_t K) {
-    if (K <= 0 || K % 32 != 0) return -1;
+    if (K <= 0 || K % 32 != 0 || K > (1 << 24)) return -1;
     if (o == Py_None) return 0;
     const int G = group_of(o);
     return G > 0 && K % G == 0 ? G : -1;
