@@ -620,7 +620,7 @@ API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wsc
     p.ws = reinterpret_cast<const uint8_t*>(wscales);
     p.bias = bias;
     p.out = out;
-    p.R = M; p.N = N; p.K = K; p.E = 1; p.dt = dtype; p.bias_dt = bias_dtype;
+    p.R = M; p.N = N; p.K = K; p.E = 1; p.dt = (short)dtype; p.bias_dt = (short)bias_dtype;
     convrot::mx_set_top_k(p, 1);
     return mx_linear_run(x, M, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }
@@ -639,7 +639,7 @@ API int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int t
     p.out = out;
     p.offsets = offsets;
     p.order = order;
-    p.R = R; p.N = N; p.K = K; p.E = E; p.dt = dtype; p.bias_dt = bias_dtype;
+    p.R = R; p.N = N; p.K = K; p.E = E; p.dt = (short)dtype; p.bias_dt = (short)bias_dtype;
     convrot::mx_set_top_k(p, order != nullptr ? top_k : 1);
     return mx_linear_run(x, R / p.top_k, G, p, workspace, workspace_bytes, reinterpret_cast<hipStream_t>(stream));
 }

@@ -37,6 +37,24 @@ inline hipError_t lds_limit_once(std::atomic<bool> (&done)[kMaxDev], int dev, co
     return e;
 }
 
+// Workgroups of `threads` that one launch takes: its threads are counted in 32
+// bits (a longer grid is cut short without an error).  A multiple of 8, so that
+// the workgroups of a later launch meet the same XCDs.
+constexpr long long launch_most(int threads) { return ((1LL << 32) / threads - 1) / 8 * 8; }
+static_assert(launch_most(256) == (1 << 24) - 8 && launch_most(512) * 512 < (1LL << 32), "threads of a launch in 32 bits");
+
+// launch(first, count) for the workgroups first .. first + count - 1 of `blocks`, as many launches as that takes.
+template <typename F>
+inline hipError_t launch_parts(long long blocks, int threads, F launch) {
+    const long long most = launch_most(threads);
+    for (long long first = 0; first < blocks; first += most) {
+        launch(first, dim3((unsigned)(blocks - first < most ? blocks - first : most)));
+        const hipError_t e = hipGetLastError();
+        if (e != hipSuccess) return e;
+    }
+    return hipSuccess;
+}
+
 // Bytes 0 .. 2047 of every workspace the library takes hold the split
 // counters of the bf6 GEMM's small-tile kernel (one per tile, at most 512):
 // zero when a workspace is first used and zero again after every call; no

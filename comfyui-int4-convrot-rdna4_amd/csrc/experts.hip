@@ -207,7 +207,7 @@ struct Piece {
     }
 };
 
-// Zeros in the rows past the last used one; the grid's workgroups share them.
+// Zeros in the rows past the last used one; the workgroups of a call's first launch share them.
 template <int DT, bool VEC>
 __device__ __forceinline__ void zero_tail(uint8_t* rows, const int* offsets, int R, int E, int D) {
     using P = Piece<DT, VEC>;
@@ -236,10 +236,11 @@ __device__ __forceinline__ void slots_of(const int* position, const float* w, lo
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_gather_kernel(const uint8_t* __restrict__ x, const int* __restrict__ position,
                                                             const int* __restrict__ offsets, uint8_t* __restrict__ rows, int R,
-                                                            int k, int E, int D, int parts) {
+                                                            int k, int E, int D, int parts, unsigned first) {
     using P = Piece<DT, VEC>;
-    const long long t = blockIdx.x / parts;
-    const int i = (blockIdx.x % parts) * 256 + threadIdx.x;
+    const unsigned b = first + blockIdx.x;
+    const long long t = b / parts;
+    const int i = (b % parts) * 256 + threadIdx.x;
     if (i < D / P::N) {
         float v[P::N];
         P::load(x + (size_t)t * D * P::ES, i, v);
@@ -248,7 +249,7 @@ __global__ __launch_bounds__(256) void expert_gather_kernel(const uint8_t* __res
             if ((unsigned)r < (unsigned)R) P::store(rows + (size_t)r * D * P::ES, i, v);
         }
     }
-    zero_tail<DT, VEC>(rows, offsets, R, E, D);
+    if (first == 0) zero_tail<DT, VEC>(rows, offsets, R, E, D);
 }
 
 // out[t] = sum_j w[t, j] rows[position[t, j]] (w NULL: 1).  Bound by reading the rows, which lie apart: 8192 x 4 rows of
@@ -256,10 +257,11 @@ __global__ __launch_bounds__(256) void expert_gather_kernel(const uint8_t* __res
 template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_combine_kernel(const uint8_t* __restrict__ rows, const float* __restrict__ w,
                                                              const int* __restrict__ position, uint8_t* __restrict__ out, int R,
-                                                             int k, int D, int parts) {
+                                                             int k, int D, int parts, unsigned first) {
     using P = Piece<DT, VEC>;
-    const long long t = blockIdx.x / parts;
-    const int i = (blockIdx.x % parts) * 256 + threadIdx.x;
+    const unsigned b = first + blockIdx.x;
+    const long long t = b / parts;
+    const int i = (b % parts) * 256 + threadIdx.x;
     if (i >= D / P::N) return;
     float s[P::N] = {};
     for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
@@ -288,10 +290,10 @@ template <int DT, bool VEC>
 __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
         const uint8_t* __restrict__ rows, const float* __restrict__ w, const int* __restrict__ position,
         const int* __restrict__ offsets, const uint8_t* __restrict__ d_out, uint8_t* __restrict__ d_rows,
-        float* __restrict__ d_w, int R, int k, int E, int D) {
+        float* __restrict__ d_w, int R, int k, int E, int D, unsigned first) {
     using P = Piece<DT, VEC>;
     __shared__ float part[4][ROW_SLOTS];
-    const long long t = blockIdx.x;
+    const long long t = first + blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
         int r[ROW_SLOTS];
@@ -330,7 +332,7 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
                                             (part[2][threadIdx.x] + part[3][threadIdx.x]);
         __syncthreads();
     }
-    if (d_rows != nullptr) zero_tail<DT, VEC>(d_rows, offsets, R, E, D);
+    if (first == 0 && d_rows != nullptr) zero_tail<DT, VEC>(d_rows, offsets, R, E, D);
 }
 
 int expert_max() { return SORT_MAX_E; }
@@ -375,14 +377,14 @@ hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* po
 
 // f(type code, vector pieces) for the row type; vector pieces where rows are whole 16-byte pieces
 template <typename F>
-static void by_type(int dt, int D, F f) {
+static hipError_t by_type(int dt, int D, F f) {
     const bool vec = D % (dt == DT_F32 ? 4 : 8) == 0;
     using std::integral_constant;
     using T = std::true_type;
     using N = std::false_type;
-    if (dt == DT_F32) vec ? f(integral_constant<int, DT_F32>{}, T{}) : f(integral_constant<int, DT_F32>{}, N{});
-    else if (dt == DT_BF16) vec ? f(integral_constant<int, DT_BF16>{}, T{}) : f(integral_constant<int, DT_BF16>{}, N{});
-    else vec ? f(integral_constant<int, DT_F16>{}, T{}) : f(integral_constant<int, DT_F16>{}, N{});
+    if (dt == DT_F32) return vec ? f(integral_constant<int, DT_F32>{}, T{}) : f(integral_constant<int, DT_F32>{}, N{});
+    if (dt == DT_BF16) return vec ? f(integral_constant<int, DT_BF16>{}, T{}) : f(integral_constant<int, DT_BF16>{}, N{});
+    return vec ? f(integral_constant<int, DT_F16>{}, T{}) : f(integral_constant<int, DT_F16>{}, N{});
 }
 
 // workgroups of 256 pieces that a row takes
@@ -391,40 +393,42 @@ static long long row_parts(int D) { return (D / Piece<DT, VEC>::N + 255) / 256; 
 
 hipError_t expert_gather_launch(const void* x, int dt, const int* position, const int* offsets, void* rows, int T, int k, int E,
                                 int D, hipStream_t st) {
-    bool fits = true;
-    by_type(dt, D, [&](auto d, auto v) {
-        const long long parts = row_parts<decltype(d)::value, decltype(v)::value>(D);
-        fits = T * parts <= 0x7fffffffLL;
-        if (fits)
-            hipLaunchKernelGGL((expert_gather_kernel<decltype(d)::value, decltype(v)::value>), dim3((unsigned)(T * parts)),
-                               dim3(256), 0, st, reinterpret_cast<const uint8_t*>(x), position, offsets,
-                               reinterpret_cast<uint8_t*>(rows), T * k, k, E, D, (int)parts);
+    return by_type(dt, D, [&](auto d, auto v) {
+        constexpr int DT = decltype(d)::value;
+        constexpr bool VEC = decltype(v)::value;
+        const long long parts = row_parts<DT, VEC>(D);
+        if (T * parts > 0xffffffffLL) return hipErrorInvalidValue;
+        return launch_parts(T * parts, 256, [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((expert_gather_kernel<DT, VEC>), grid, dim3(256), 0, st, reinterpret_cast<const uint8_t*>(x),
+                               position, offsets, reinterpret_cast<uint8_t*>(rows), T * k, k, E, D, (int)parts, (unsigned)first);
+        });
     });
-    return fits ? hipGetLastError() : hipErrorInvalidValue;
 }
 
 hipError_t expert_combine_launch(const void* rows, int dt, const float* w, const int* position, void* out, int T, int k, int D,
                                  hipStream_t st) {
-    bool fits = true;
-    by_type(dt, D, [&](auto d, auto v) {
-        const long long parts = row_parts<decltype(d)::value, decltype(v)::value>(D);
-        fits = T * parts <= 0x7fffffffLL;
-        if (fits)
-            hipLaunchKernelGGL((expert_combine_kernel<decltype(d)::value, decltype(v)::value>), dim3((unsigned)(T * parts)),
-                               dim3(256), 0, st, reinterpret_cast<const uint8_t*>(rows), w, position,
-                               reinterpret_cast<uint8_t*>(out), T * k, k, D, (int)parts);
+    return by_type(dt, D, [&](auto d, auto v) {
+        constexpr int DT = decltype(d)::value;
+        constexpr bool VEC = decltype(v)::value;
+        const long long parts = row_parts<DT, VEC>(D);
+        if (T * parts > 0xffffffffLL) return hipErrorInvalidValue;
+        return launch_parts(T * parts, 256, [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((expert_combine_kernel<DT, VEC>), grid, dim3(256), 0, st, reinterpret_cast<const uint8_t*>(rows), w,
+                               position, reinterpret_cast<uint8_t*>(out), T * k, k, D, (int)parts, (unsigned)first);
+        });
     });
-    return fits ? hipGetLastError() : hipErrorInvalidValue;
 }
 
 hipError_t expert_combine_grad_launch(const void* rows, int dt, const float* w, const int* position, const int* offsets,
                                       const void* d_out, void* d_rows, float* d_w, int T, int k, int E, int D, hipStream_t st) {
-    by_type(dt, D, [&](auto d, auto v) {
-        hipLaunchKernelGGL((expert_combine_grad_kernel<decltype(d)::value, decltype(v)::value>), dim3(T), dim3(256), 0, st,
-                           reinterpret_cast<const uint8_t*>(rows), w, position, offsets, reinterpret_cast<const uint8_t*>(d_out),
-                           reinterpret_cast<uint8_t*>(d_rows), d_w, T * k, k, E, D);
+    return by_type(dt, D, [&](auto d, auto v) {
+        return launch_parts(T, 256, [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((expert_combine_grad_kernel<decltype(d)::value, decltype(v)::value>), grid, dim3(256), 0, st,
+                               reinterpret_cast<const uint8_t*>(rows), w, position, offsets,
+                               reinterpret_cast<const uint8_t*>(d_out), reinterpret_cast<uint8_t*>(d_rows), d_w, T * k, k, E, D,
+                               (unsigned)first);
+        });
     });
-    return hipGetLastError();
 }
 
 }  // namespace convrot

@@ -19,7 +19,9 @@ struct MxProblem {
     const void* bias;
     void* out;
     const int *offsets, *order;
-    int R, N, K, Kp, Ks, as_rows, E, top_k, dt, bias_dt;
+    int R, N, K, Kp, Ks, as_rows, E, top_k;
+    int block0;                                            // workgroups of earlier launches of the call
+    short dt, bias_dt;                                     // 120 bytes in all: the arguments of a launch in two cache lines
     unsigned k_mul;                                        // n / top_k = n k_mul >> k_shift for 0 <= n < 2^31
     int k_shift;
 };

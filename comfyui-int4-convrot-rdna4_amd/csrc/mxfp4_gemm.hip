@@ -66,9 +66,10 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void mxfp4_gemm_few_kernel(MxProble
     extern __shared__ __attribute__((aligned(16))) uint8_t lds_few[];
     const int tid = threadIdx.x, lane = tid & 63, wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int tiles_m = mx_tile_count<BM>(p), tiles_n = (p.N + BN - 1) / BN;
-    if ((int)blockIdx.x >= tiles_m * tiles_n) return;
+    const int block = p.block0 + (int)blockIdx.x;
+    if (block >= tiles_m * tiles_n) return;
     int tm, tn;
-    tile_of_block(blockIdx.x, tiles_m, tiles_n, tiles_m, tm, tn);   // an XCD's row tiles of the same columns together
+    tile_of_block(block, tiles_m, tiles_n, tiles_m, tm, tn);   // an XCD's row tiles of the same columns together
     const MxTile t = mx_tile<BM>(p, tm);
     const int n0 = tn * BN;
     if (t.e == p.E && p.offsets != nullptr) return mx_zero(p, t.m0, t.m1, n0, min(n0 + BN, p.N));
@@ -246,7 +247,7 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void mxfp4_gemm_few_kernel(MxProble
 }
 
 template <int DT, int G, int MF, int NF, bool FUSE>
-static hipError_t few_go(const MxProblem& p, const void* x, hipStream_t st) {
+static hipError_t few_go(MxProblem p, const void* x, hipStream_t st) {
     static std::atomic<bool> attr[kMaxDev];
     const long long grid = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 16 * MF) * ((p.N + 16 * NF - 1) / (16 * NF));
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
@@ -260,9 +261,11 @@ static hipError_t few_go(const MxProblem& p, const void* x, hipStream_t st) {
     if (e != hipSuccess) return e;
     e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&mxfp4_gemm_few_kernel<DT, G, MF, NF, FUSE>), 160 << 10);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((mxfp4_gemm_few_kernel<DT, G, MF, NF, FUSE>), dim3((unsigned)grid), dim3(64 * FEW_WAVES), lds, st, p,
-                       reinterpret_cast<const uint8_t*>(x));
-    return hipGetLastError();
+    return launch_parts(grid, 64 * FEW_WAVES, [&](long long first, dim3 part) {
+        p.block0 = (int)first;
+        hipLaunchKernelGGL((mxfp4_gemm_few_kernel<DT, G, MF, NF, FUSE>), part, dim3(64 * FEW_WAVES), lds, st, p,
+                           reinterpret_cast<const uint8_t*>(x));
+    });
 }
 
 // Rows that each workgroup quantizes itself: few of them in a tile, so that the work is less than a launch costs (5120 ->

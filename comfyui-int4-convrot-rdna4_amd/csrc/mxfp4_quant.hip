@@ -23,9 +23,9 @@ namespace convrot {
 
 template <int DT, int G>
 __global__ __launch_bounds__(256) void mxfp4_quant_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
-                                                          uint8_t* __restrict__ scales, long long units) {
+                                                          uint8_t* __restrict__ scales, long long units, long long first) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
-    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;       // 16 values of the matrix
+    const long long u = (first + blockIdx.x) * 256 + threadIdx.x;        // 16 values of the matrix
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.0f;
@@ -70,14 +70,15 @@ __device__ __forceinline__ void tile_scales(const MxTileScales& w, long long i, 
 template <int DT, int G, bool TILES>
 __global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __restrict__ x, uint8_t* __restrict__ codes,
                                                                uint8_t* __restrict__ scales, int M, int K, int Kp, int Ks,
-                                                               unsigned blocks, MxTileScales w) {
+                                                               unsigned blocks, MxTileScales w, unsigned first) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
     __shared__ __attribute__((aligned(16))) uint8_t sc[8][16];
+    const unsigned b = first + blockIdx.x;
     if constexpr (TILES) {
-        if (blockIdx.x >= blocks) return tile_scales(w, (long long)(blockIdx.x - blocks) * 256 + threadIdx.x, Ks);
+        if (b >= blocks) return tile_scales(w, (long long)(b - blocks) * 256 + threadIdx.x, Ks);
     }
     const int per = Ks / 16;
-    const int ss = blockIdx.x % per, row0 = (int)(blockIdx.x / per) * 8;
+    const int ss = b % per, row0 = (int)(b / per) * 8;
     const int r = threadIdx.x >> 5, l = threadIdx.x & 31;
     const int row = row0 + r, k = ss * 512 + l * 16;
     float v[16];
@@ -100,9 +101,9 @@ __global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __
 template <int DT, int G>
 __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __restrict__ codes,
                                                             const uint8_t* __restrict__ scales, uint8_t* __restrict__ out,
-                                                            long long units) {
+                                                            long long units, long long first) {
     constexpr int ES = DT == DT_F32 ? 4 : 2;
-    const long long u = (long long)blockIdx.x * 256 + threadIdx.x;
+    const long long u = (first + blockIdx.x) * 256 + threadIdx.x;
     v2u_mx c = {0u, 0u};
     uint32_t sb = 127u;
     if (u < units) {
@@ -150,16 +151,17 @@ __global__ __launch_bounds__(256) void mxfp4_dequant_kernel(const uint8_t* __res
 }
 
 template <int DT, int G>
-static void quant_go(const void* x, void* codes, void* scales, int M, int K, hipStream_t st) {
+static hipError_t quant_go(const void* x, void* codes, void* scales, int M, int K, hipStream_t st) {
     const long long units = (long long)M * (K / 16);
-    hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G>), dim3((unsigned)((units + 255) / 256)), dim3(256), 0, st,
-                       reinterpret_cast<const uint8_t*>(x), reinterpret_cast<uint8_t*>(codes), reinterpret_cast<uint8_t*>(scales),
-                       units);
+    return launch_parts((units + 255) / 256, 256, [&](long long first, dim3 grid) {
+        hipLaunchKernelGGL((mxfp4_quant_kernel<DT, G>), grid, dim3(256), 0, st, reinterpret_cast<const uint8_t*>(x),
+                           reinterpret_cast<uint8_t*>(codes), reinterpret_cast<uint8_t*>(scales), units, first);
+    });
 }
 
 // f(type code, group) as compile-time constants
 template <typename F>
-static void by_type_and_group(int dt, int G, F f) {
+static auto by_type_and_group(int dt, int G, F f) {
     using std::integral_constant;
     auto group = [&](auto d) {
         switch (G) {
@@ -178,55 +180,43 @@ static void by_type_and_group(int dt, int G, F f) {
 
 // x [M, K] -> codes [M, K/2], scales [M, K/32]
 hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, int M, int K, int G, hipStream_t st) {
-    if (M == 0) return hipSuccess;
-    by_type_and_group(dt, G, [&](auto d, auto g) { quant_go<decltype(d)::value, decltype(g)::value>(x, codes, scales, M, K, st); });
-    return hipGetLastError();
+    return by_type_and_group(dt, G, [&](auto d, auto g) {
+        return quant_go<decltype(d)::value, decltype(g)::value>(x, codes, scales, M, K, st);
+    });
 }
 
 // x [rows, K] as the operand p.a, p.as of a product; with `tiles` in the order of staged tiles, and p.ws as p.wp
 hipError_t mxfp4_operands_launch(const void* x, int G, const MxProblem& p, bool tiles, hipStream_t st) {
-    const unsigned blocks = (unsigned)((p.as_rows + 7LL) / 8 * (p.Ks / 16));
+    const long long blocks = (p.as_rows + 7LL) / 8 * (p.Ks / 16);
     MxTileScales w{p.ws, const_cast<uint8_t*>(p.wp), (long long)p.E * p.N * (p.Ks / 16), p.N, p.K / 32};
-    const long long grid = tiles ? blocks + (w.pieces + 255) / 256 : blocks;
-    if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    by_type_and_group(p.dt, G, [&](auto d, auto g) {
+    const long long all = tiles ? blocks + (w.pieces + 255) / 256 : blocks;
+    if (all > 0xffffffffLL) return hipErrorInvalidValue;
+    return by_type_and_group(p.dt, G, [&](auto d, auto g) {
         constexpr int DT = decltype(d)::value, GG = decltype(g)::value;
         const auto xb = reinterpret_cast<const uint8_t*>(x);
         const auto cb = const_cast<uint8_t*>(p.a), sb = const_cast<uint8_t*>(p.as);
-        if (tiles)
-            hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, true>), dim3((unsigned)grid), dim3(256), 0, st, xb, cb, sb,
-                               p.as_rows, p.K, p.Kp, p.Ks, blocks, w);
-        else
-            hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, false>), dim3((unsigned)grid), dim3(256), 0, st, xb, cb, sb,
-                               p.as_rows, p.K, p.Kp, p.Ks, blocks, w);
+        return launch_parts(all, 256, [&](long long first, dim3 grid) {
+            if (tiles)
+                hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, true>), grid, dim3(256), 0, st, xb, cb, sb, p.as_rows, p.K,
+                                   p.Kp, p.Ks, (unsigned)blocks, w, (unsigned)first);
+            else
+                hipLaunchKernelGGL((mxfp4_quant_rows_kernel<DT, GG, false>), grid, dim3(256), 0, st, xb, cb, sb, p.as_rows, p.K,
+                                   p.Kp, p.Ks, (unsigned)blocks, w, (unsigned)first);
+        });
     });
-    return hipGetLastError();
 }
 
-template <int DT>
-static void dequant_group(const void* codes, const void* scales, void* out, long long units, int G, hipStream_t st) {
-    const dim3 grid((unsigned)((units + 255) / 256));
-    const auto cb = reinterpret_cast<const uint8_t*>(codes);
-    const auto sb = reinterpret_cast<const uint8_t*>(scales);
-    const auto ob = reinterpret_cast<uint8_t*>(out);
-    switch (G) {
-        case 0: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 0>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
-        case 16: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 16>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
-        case 64: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 64>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
-        default: hipLaunchKernelGGL((mxfp4_dequant_kernel<DT, 256>), grid, dim3(256), 0, st, cb, sb, ob, units); break;
-    }
-}
-
+// codes [M, K/2], scales [M, K/32] -> out [M, K]
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st) {
-    if (M == 0) return hipSuccess;
     const long long units = (long long)M * (K / 16);
-    switch (dt) {
-        case DT_F32: dequant_group<DT_F32>(codes, scales, out, units, G, st); break;
-        case DT_BF16: dequant_group<DT_BF16>(codes, scales, out, units, G, st); break;
-        default: dequant_group<DT_F16>(codes, scales, out, units, G, st); break;
-    }
-    return hipGetLastError();
+    return by_type_and_group(dt, G, [&](auto d, auto g) {
+        return launch_parts((units + 255) / 256, 256, [&](long long first, dim3 grid) {
+            hipLaunchKernelGGL((mxfp4_dequant_kernel<decltype(d)::value, decltype(g)::value>), grid, dim3(256), 0, st,
+                               reinterpret_cast<const uint8_t*>(codes), reinterpret_cast<const uint8_t*>(scales),
+                               reinterpret_cast<uint8_t*>(out), units, first);
+        });
+    });
 }
 
 }  // namespace convrot

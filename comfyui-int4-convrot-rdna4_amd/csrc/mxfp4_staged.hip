@@ -58,7 +58,8 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     const int wave = __builtin_amdgcn_readfirstlane(tid >> 6);
     const int wm = wave >> 1, wn = wave & 1;
     const int tiles_m = mx_tile_count<S::BM>(p), tiles_n = (p.N + S::BN - 1) / S::BN;
-    if ((int)blockIdx.x >= tiles_m * tiles_n) return;
+    const int block = p.block0 + (int)blockIdx.x;
+    if (block >= tiles_m * tiles_n) return;
 
     // Copy j of this wave and stage: rows 8 i .. 8 i + 7 of the tile (i = wave L + j; the A rows, then the W rows),
     // lane l row l / 8 and the chunk that belongs at place l % 8.
@@ -73,7 +74,7 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         return (wave * S::L + ((S::BM / 8) % S::L == 0 ? 0 : j)) * 8 < S::BM;
     };
     int tm, tn;
-    tile_of_block(blockIdx.x, tiles_m, tiles_n, min(gm_max, tiles_m), tm, tn);
+    tile_of_block(block, tiles_m, tiles_n, min(gm_max, tiles_m), tm, tn);
     const MxTile t = mx_tile<S::BM>(p, tm);
     const int n0 = tn * S::BN;
     if (t.e == p.E && p.offsets != nullptr) return mx_zero(p, t.m0, t.m1, n0, min(n0 + S::BN, p.N));
@@ -374,7 +375,7 @@ int mxfp4_gemm_tile(const MxProblem& p) {
 bool mxfp4_gemm_staged(const MxProblem& p) { return mxfp4_gemm_tile(p) != 0; }
 
 template <int DT, int FM, int FN, int SLOTS>
-static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
+static hipError_t staged_go(MxProblem p, hipStream_t st) {
     using S = Staged<FM, FN, SLOTS>;
     static std::atomic<bool> attr[kMaxDev];
     int dev = 0;
@@ -383,11 +384,13 @@ static hipError_t staged_go(const MxProblem& p, hipStream_t st) {
     e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&mxfp4_gemm_staged_kernel<DT, FM, FN, SLOTS>), S::LDS);
     if (e != hipSuccess) return e;
     const long long rows = mx_row_tiles(p.R, p.E, p.offsets != nullptr, S::BM);
-    long long grid = rows * ((p.N + S::BN - 1) / S::BN);
+    const long long grid = rows * ((p.N + S::BN - 1) / S::BN);
     if (grid > 0x7fffffffLL) return hipErrorInvalidValue;
-    hipLaunchKernelGGL((mxfp4_gemm_staged_kernel<DT, FM, FN, SLOTS>), dim3((unsigned)grid), dim3(S::THREADS), S::LDS, st, p,
-                       tile_group_rows((int)rows));
-    return hipGetLastError();
+    return launch_parts(grid, S::THREADS, [&](long long first, dim3 part) {
+        p.block0 = (int)first;
+        hipLaunchKernelGGL((mxfp4_gemm_staged_kernel<DT, FM, FN, SLOTS>), part, dim3(S::THREADS), S::LDS, st, p,
+                           tile_group_rows((int)rows));
+    });
 }
 
 template <int DT>
