@@ -49,14 +49,45 @@ __global__ __launch_bounds__(64 * SORT_MANY) void expert_count_kernel(const ID* 
     for (int i = threadIdx.x; i < E; i += 64 * SORT_MANY) counts[(size_t)blockIdx.x * E + i] = n[i];
 }
 
+// Counts of a run -> counts of the runs before it, and behind the last run's the totals.  A workgroup takes 64
+// experts, each of its waves a sixteenth of the runs, eight of them read at a time.
+__global__ __launch_bounds__(1024) void expert_scan_kernel(int* __restrict__ counts, int E, int runs) {
+    __shared__ int part[16][64];
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6, x = blockIdx.x * 64 + lane;
+    const int b0 = (int)((long long)runs * wave / 16), b1 = (int)((long long)runs * (wave + 1) / 16);
+    int sum = 0;
+    if (x < E) {
+#pragma unroll 8
+        for (int b = b0; b < b1; ++b) sum += counts[(size_t)b * E + x];
+    }
+    part[wave][lane] = sum;
+    __syncthreads();
+    int before = 0;
+    for (int v = 0; v < wave; ++v) before += part[v][lane];
+    if (x >= E) return;
+    for (int b = b0; b < b1; b += 8) {
+        int c[8];
+#pragma unroll
+        for (int i = 0; i < 8; ++i) c[i] = b + i < b1 ? counts[(size_t)(b + i) * E + x] : 0;
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            if (b + i < b1) counts[(size_t)(b + i) * E + x] = before;
+            before += c[i];
+        }
+    }
+    if (wave == 15) counts[(size_t)runs * E + x] = before;
+}
+
 // Workgroup b places its run: expert e's first row there is offsets[e] plus the
 // counts of the runs before.  Each wave takes a part of the run, in order, 64
 // slots at a time; the lanes that go to one expert find each other by the bits of
 // its number, so that one of them counts for all, and their order is the slots'.
-// A single run needs no counts from elsewhere (ONE): one launch.  Bound by the
+// A single run needs no counts from elsewhere (ONE): one launch.  Of a few runs each
+// workgroup adds up the counts itself; of more than SCAN_RUNS (SCANNED) that would be the
+// square of their number, and a launch between has done it.  Bound by the
 // chain of loads, ballots and LDS, so a wave has few slots: 2000 slots of 32
 // experts 5.3 us (7.4 with four waves of 512), 64 slots 2.7 (3.4 with sixteen waves).
-template <typename ID, bool ONE, int WAVES>
+template <typename ID, bool ONE, int WAVES, bool SCANNED>
 __global__ __launch_bounds__(64 * WAVES) void expert_place_kernel(const ID* __restrict__ ids,
                                                                     const int* __restrict__ counts, int* __restrict__ order,
                                                                     int* __restrict__ position, int* __restrict__ offsets,
@@ -102,6 +133,9 @@ __global__ __launch_bounds__(64 * WAVES) void expert_place_kernel(const ID* __re
             if constexpr (ONE) {
 #pragma unroll
                 for (int v = 0; v < WAVES; ++v) all += own[v];
+            } else if constexpr (SCANNED) {
+                before = counts[(size_t)blockIdx.x * E + x];
+                all = counts[(size_t)runs * E + x];
             } else {
 #pragma unroll 8
                 for (int b = 0; b < runs; ++b) {
@@ -341,9 +375,14 @@ static int sort_runs(int R) {
     return R <= sort_slots(SORT_FEW) ? 1 : (int)((R + (long long)sort_slots(SORT_MANY) - 1) / sort_slots(SORT_MANY));
 }
 
-size_t expert_sort_bytes(int R, int E) { return (size_t)sort_runs(R) * E * sizeof(int); }
+// counts of every run, and the totals
+size_t expert_sort_bytes(int R, int E) { return ((size_t)sort_runs(R) + 1) * E * sizeof(int); }
 
-template <typename ID, bool ONE, int WAVES>
+// Runs whose counts each placing workgroup adds up itself.  us, itself and after the launch between, 32 experts: 16 runs
+// 9.9 and 11.8, 64 runs 11.7 and 12.8, 128 runs 14.4 and 13.0, 512 runs 46.5 and 25.3; 1000 experts: 64 runs 16.1 and 16.6.
+constexpr int SCAN_RUNS = 64;
+
+template <typename ID, bool ONE, int WAVES, bool SCANNED>
 static hipError_t place_go(const ID* ids, const int* counts, int* order, int* position, int* offsets, int R, int E, int runs,
                            hipStream_t st) {
     static std::atomic<bool> attr[kMaxDev];
@@ -351,9 +390,9 @@ static hipError_t place_go(const ID* ids, const int* counts, int* order, int* po
     int dev = 0;
     hipError_t e = current_device(&dev);
     if (e != hipSuccess) return e;
-    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&expert_place_kernel<ID, ONE, WAVES>), MOST);
+    e = lds_limit_once(attr, dev, reinterpret_cast<const void*>(&expert_place_kernel<ID, ONE, WAVES, SCANNED>), MOST);
     if (e != hipSuccess) return e;
-    hipLaunchKernelGGL((expert_place_kernel<ID, ONE, WAVES>), dim3(runs), dim3(64 * WAVES), WAVES * (E + 1) * sizeof(int), st,
+    hipLaunchKernelGGL((expert_place_kernel<ID, ONE, WAVES, SCANNED>), dim3(runs), dim3(64 * WAVES), WAVES * (E + 1) * sizeof(int), st,
                        ids, counts, order, position, offsets, R, E, runs);
     return hipGetLastError();
 }
@@ -362,11 +401,15 @@ template <typename ID>
 static hipError_t sort_go(const void* ids, int* order, int* position, int* offsets, int* counts, int R, int E, hipStream_t st) {
     const int runs = sort_runs(R);
     const ID* p = reinterpret_cast<const ID*>(ids);
-    if (R <= sort_slots(SORT_FEW)) return place_go<ID, true, SORT_FEW>(p, counts, order, position, offsets, R, E, runs, st);
-    if (runs == 1) return place_go<ID, true, SORT_MANY>(p, counts, order, position, offsets, R, E, runs, st);
+    if (R <= sort_slots(SORT_FEW)) return place_go<ID, true, SORT_FEW, false>(p, counts, order, position, offsets, R, E, runs, st);
+    if (runs == 1) return place_go<ID, true, SORT_MANY, false>(p, counts, order, position, offsets, R, E, runs, st);
     hipLaunchKernelGGL((expert_count_kernel<ID>), dim3(runs), dim3(64 * SORT_MANY), 0, st, p, counts, R, E);
-    const hipError_t e = hipGetLastError();
-    return e != hipSuccess ? e : place_go<ID, false, SORT_MANY>(p, counts, order, position, offsets, R, E, runs, st);
+    hipError_t e = hipGetLastError();
+    if (e != hipSuccess) return e;
+    if (runs <= SCAN_RUNS) return place_go<ID, false, SORT_MANY, false>(p, counts, order, position, offsets, R, E, runs, st);
+    hipLaunchKernelGGL(expert_scan_kernel, dim3((E + 63) / 64), dim3(1024), 0, st, counts, E, runs);
+    e = hipGetLastError();
+    return e != hipSuccess ? e : place_go<ID, false, SORT_MANY, true>(p, counts, order, position, offsets, R, E, runs, st);
 }
 
 hipError_t expert_sort_launch(const void* ids, int id_bytes, int* order, int* position, int* offsets, int* counts, int R, int E,
