@@ -21,6 +21,7 @@ from . import native
 
 _BLOCK = 32
 _MAX_K = 1 << 24             # widest row that the library takes
+_MAX_N = (1 << 31) - 256     # columns of a product
 
 
 def _check_group(K: int, convrot_groupsize: int | None, what: str = "in_features") -> int:
@@ -142,7 +143,7 @@ def mxfp4_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.Tensor, 
     if qweight.shape[-1] * 2 != K:
         raise ValueError(f"Input K={K} does not match qweight K={qweight.shape[-1] * 2}")
     G = _check_group(K, convrot_groupsize)
-    M, N = _count(x.numel() // K, "rows"), _count(qweight.shape[0], "columns")
+    M, N = _count(x.numel() // K, "rows"), _count(qweight.shape[0], "columns", _MAX_N)
     _check_operand(qweight, wscales, (N,), K, "qweight")
     bdt = _check_bias(bias, (N,))
     _no_grad("mxfp4_linear", x, bias)
@@ -191,7 +192,7 @@ def mxfp4_expert_linear(x: torch.Tensor, qweight: torch.Tensor, wscales: torch.T
     if qweight.shape[-1] * 2 != K:
         raise ValueError(f"Input K={K} does not match qweight K={qweight.shape[-1] * 2}")
     G = _check_group(K, convrot_groupsize)
-    E, N = qweight.shape[0], _count(qweight.shape[1], "columns")
+    E, N = qweight.shape[0], _count(qweight.shape[1], "columns", _MAX_N)
     _check_operand(qweight, wscales, (E, N), K, "qweight")
     plan.check(E)
     if E > native._limit("cr_max_experts"):
@@ -229,9 +230,9 @@ def _on_gpu(t: torch.Tensor) -> torch.Tensor:
     return t.to("cuda")
 
 
-def _count(n: int, what: str) -> int:
-    if n >= 1 << 31:
-        raise ValueError(f"{n} {what} are more than one call takes (2^31 - 1)")
+def _count(n: int, what: str, most: int = (1 << 31) - 1) -> int:
+    if n > most:
+        raise ValueError(f"{n} {what} are more than one call takes ({most})")
     return n
 
 

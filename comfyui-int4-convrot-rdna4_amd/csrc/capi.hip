@@ -613,7 +613,7 @@ API int cr_mxfp4_tile(int R, int N, int K, int experts) {
 
 API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,
                         void* out, int M, int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!mx_args_ok(dtype, M, K, G) || N < 0 || bias_dtype < 0 || bias_dtype > 2) return -1;
+    if (!mx_args_ok(dtype, M, K, G) || N < 0 || N > convrot::MX_MAX_N || bias_dtype < 0 || bias_dtype > 2) return -1;
     if (M == 0 || N == 0) return 0;
     convrot::MxProblem p{};
     p.w = reinterpret_cast<const uint8_t*>(W);
@@ -628,7 +628,7 @@ API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wsc
 API int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k, const int* offsets, int E,
                                const void* W, const void* wscales, const void* bias, int bias_dtype, void* out, int R,
                                int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream) {
-    if (!mx_args_ok(dtype, R, K, G) || N < 0 || bias_dtype < 0 || bias_dtype > 2) return -1;
+    if (!mx_args_ok(dtype, R, K, G) || N < 0 || N > convrot::MX_MAX_N || bias_dtype < 0 || bias_dtype > 2) return -1;
     if (E < 1 || E > convrot::expert_max() || offsets == nullptr) return -1;
     if (order != nullptr && (top_k < 1 || R % top_k != 0)) return -1;
     if (R == 0 || N == 0) return 0;

@@ -246,19 +246,19 @@ template <int DT, bool VEC>
 __device__ __forceinline__ void zero_tail(uint8_t* rows, const int* offsets, int R, int E, int D) {
     using P = Piece<DT, VEC>;
     const float z[P::N] = {};
-    for (int r = max(offsets[E], 0) + blockIdx.x; r < R; r += gridDim.x)
-        for (int i = threadIdx.x; i < D / P::N; i += blockDim.x) P::store(rows + (size_t)r * D * P::ES, i, z);
+    for (long long r = max(offsets[E], 0) + (long long)blockIdx.x; r < R; r += gridDim.x)
+        for (unsigned i = threadIdx.x; i < (unsigned)(D / P::N); i += 256) P::store(rows + (size_t)r * D * P::ES, i, z);
 }
 
 // A workgroup takes 256 pieces of one token's row; a token's slots are read four at a time, their rows together.
 constexpr int ROW_SLOTS = 4;
 
 // Rows position[t, j0 .. j0 + 3] (-1: none) and with W their weights
-__device__ __forceinline__ void slots_of(const int* position, const float* w, long long t, int j0, int k, int R, int (&r)[ROW_SLOTS],
-                                         float (&f)[ROW_SLOTS]) {
+__device__ __forceinline__ void slots_of(const int* position, const float* w, long long t, unsigned j0, int k, int R,
+                                         int (&r)[ROW_SLOTS], float (&f)[ROW_SLOTS]) {
 #pragma unroll
     for (int j = 0; j < ROW_SLOTS; ++j) {
-        const bool there = j0 + j < k;
+        const bool there = j0 + j < (unsigned)k;
         const int p = there ? position[t * k + j0 + j] : -1;
         r[j] = (unsigned)p < (unsigned)R ? p : -1;
         f[j] = there && w != nullptr ? w[t * k + j0 + j] : 1.0f;
@@ -298,7 +298,7 @@ __global__ __launch_bounds__(256) void expert_combine_kernel(const uint8_t* __re
     const int i = (b % parts) * 256 + threadIdx.x;
     if (i >= D / P::N) return;
     float s[P::N] = {};
-    for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
+    for (unsigned j0 = 0; j0 < (unsigned)k; j0 += ROW_SLOTS) {
         int r[ROW_SLOTS];
         float f[ROW_SLOTS], v[ROW_SLOTS][P::N];
         slots_of(position, w, t, j0, k, R, r, f);
@@ -329,11 +329,11 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
     __shared__ float part[4][ROW_SLOTS];
     const long long t = first + blockIdx.x;
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    for (int j0 = 0; j0 < k; j0 += ROW_SLOTS) {
+    for (unsigned j0 = 0; j0 < (unsigned)k; j0 += ROW_SLOTS) {
         int r[ROW_SLOTS];
         float f[ROW_SLOTS], dot[ROW_SLOTS] = {};
         slots_of(position, w, t, j0, k, R, r, f);
-        for (int i = threadIdx.x; i < D / P::N; i += 256) {
+        for (unsigned i = threadIdx.x; i < (unsigned)(D / P::N); i += 256) {
             float g[P::N], v[ROW_SLOTS][P::N];
             P::load(d_out + (size_t)t * D * P::ES, i, g);
             if (d_w != nullptr) {
@@ -361,7 +361,7 @@ __global__ __launch_bounds__(256) void expert_combine_grad_kernel(
             if (lane == 0) part[wave][j] = dot[j];
         }
         __syncthreads();
-        if (threadIdx.x < ROW_SLOTS && j0 + (int)threadIdx.x < k)
+        if (threadIdx.x < ROW_SLOTS && j0 + threadIdx.x < (unsigned)k)
             d_w[t * k + j0 + threadIdx.x] = (part[0][threadIdx.x] + part[1][threadIdx.x]) +
                                             (part[2][threadIdx.x] + part[3][threadIdx.x]);
         __syncthreads();
@@ -432,7 +432,7 @@ static hipError_t by_type(int dt, int D, F f) {
 
 // workgroups of 256 pieces that a row takes
 template <int DT, bool VEC>
-static long long row_parts(int D) { return (D / Piece<DT, VEC>::N + 255) / 256; }
+static long long row_parts(int D) { return (D / Piece<DT, VEC>::N + 255LL) / 256; }
 
 hipError_t expert_gather_launch(const void* x, int dt, const int* position, const int* offsets, void* rows, int T, int k, int E,
                                 int D, hipStream_t st) {

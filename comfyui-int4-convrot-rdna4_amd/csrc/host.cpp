@@ -296,7 +296,7 @@ bool mx_weight(PyObject* ow, PyObject* os, PyObject* ob, c10::Device dev, int64_
     c10::Device d = dev;
     if (!operand(ow, w, &d) || !operand(os, s, &d) || w->dim() != dim || w->size(-1) * 2 != K || w->numel() == 0 ||
         w->scalar_type() != at::kByte || s->scalar_type() != at::kByte || s->dim() != dim || s->size(-1) != K / 32 ||
-        s->sizes().slice(0, dim - 1) != w->sizes().slice(0, dim - 1) || w->size(-2) > INT32_MAX)
+        s->sizes().slice(0, dim - 1) != w->sizes().slice(0, dim - 1) || w->size(-2) > 0x7fffff00)
         return false;
     *bdt = 0;
     if (ob == Py_None) return true;

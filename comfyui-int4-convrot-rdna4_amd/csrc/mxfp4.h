@@ -12,6 +12,7 @@
 namespace convrot {
 
 constexpr int MX_BLOCK = 32;         // values that share a scale
+constexpr int MX_MAX_N = 0x7fffff00; // columns of a product: a tile's past them stay below 2^31
 
 typedef unsigned v4u_mx __attribute__((ext_vector_type(4)));
 typedef unsigned v2u_mx __attribute__((ext_vector_type(2)));

@@ -49,6 +49,16 @@ inline long long mx_row_tiles(int R, int E, bool ragged, int BM) {
     return R / BM + (E + 1LL < R ? E + 1LL : R);
 }
 
+// Row numbers go up to 2^31 - 2: sums of one and a tile's rows are taken unsigned, or as distances.
+
+// Tiles of n rows
+template <int BM>
+__device__ __forceinline__ int mx_tiles_of(int n) { return (int)(((unsigned)n + (BM - 1)) / BM); }
+
+// End of the tile that begins at row m0 of those before r1
+template <int BM>
+__device__ __forceinline__ int mx_tile_end(int m0, int r1) { return m0 + min(BM, r1 - m0); }
+
 // Expert e's rows as the wave's lanes hold them, 64 experts a run; expert E is the rows past the last used one.
 template <int BM>
 struct MxRun {
@@ -56,7 +66,7 @@ struct MxRun {
     __device__ __forceinline__ MxRun(const MxProblem& p, int e) {
         r0 = e <= p.E ? min(max(p.offsets[e], 0), p.R) : p.R;
         r1 = e < p.E ? min(max(p.offsets[e + 1], r0), p.R) : p.R;
-        sum = n = (r1 - r0 + BM - 1) / BM;
+        sum = n = mx_tiles_of<BM>(r1 - r0);
         const int lane = threadIdx.x & 63;
 #pragma unroll
         for (int d = 1; d < 64; d <<= 1) {
@@ -69,7 +79,7 @@ struct MxRun {
 // Row tiles that there are.
 template <int BM>
 __device__ __forceinline__ int mx_tile_count(const MxProblem& p) {
-    if (p.offsets == nullptr) return (p.R + BM - 1) / BM;
+    if (p.offsets == nullptr) return mx_tiles_of<BM>(p.R);
     int count = 0;
     for (int e0 = 0; e0 <= p.E; e0 += 64) count += __shfl(MxRun<BM>(p, e0 + (threadIdx.x & 63)).sum, 63);
     return __builtin_amdgcn_readfirstlane(count);
@@ -78,7 +88,7 @@ __device__ __forceinline__ int mx_tile_count(const MxProblem& p) {
 // Row tile t, which there is.
 template <int BM>
 __device__ __forceinline__ MxTile mx_tile(const MxProblem& p, int t) {
-    if (p.offsets == nullptr) return {0, t * BM, min(t * BM + BM, p.R)};
+    if (p.offsets == nullptr) return {0, t * BM, mx_tile_end<BM>(t * BM, p.R)};
     int base = 0;
     for (int e0 = 0; e0 <= p.E; e0 += 64) {
         const MxRun<BM> run(p, e0 + (threadIdx.x & 63));
@@ -87,7 +97,7 @@ __device__ __forceinline__ MxTile mx_tile(const MxProblem& p, int t) {
         if (here) {
             const int l = __builtin_ctzll(here);
             const int m0 = __builtin_amdgcn_readfirstlane(__shfl(run.r0 + (t - first) * BM, l));
-            return {e0 + l, m0, __builtin_amdgcn_readfirstlane(min(m0 + BM, __shfl(run.r1, l)))};
+            return {e0 + l, m0, __builtin_amdgcn_readfirstlane(mx_tile_end<BM>(m0, __shfl(run.r1, l)))};
         }
         base += __shfl(run.sum, 63);
     }
@@ -125,7 +135,7 @@ __device__ __forceinline__ int mx_source_row(const MxProblem& p, int r) {
 // time, 16 bytes a lane where rows are whole pieces of that.
 __device__ __forceinline__ void mx_zero(const MxProblem& p, int m0, int m1, int n0, int n1) {
     const int es = p.dt == DT_F32 ? 4 : 2, lane = threadIdx.x & 63;
-    for (int m = m0 + (threadIdx.x >> 6); m < m1; m += blockDim.x >> 6) {
+    for (unsigned m = m0 + (threadIdx.x >> 6); m < (unsigned)m1; m += blockDim.x >> 6) {
         uint8_t* row = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + n0) * es;
         const int bytes = (n1 - n0) * es;
         if ((size_t)p.N * es % 16 == 0) {

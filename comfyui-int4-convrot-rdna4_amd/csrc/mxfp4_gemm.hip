@@ -234,8 +234,9 @@ __global__ __launch_bounds__(64 * FEW_WAVES) void mxfp4_gemm_few_kernel(MxProble
             o.x += b.x; o.y += b.y; o.z += b.z; o.w += b.w;
         }
         const int f = q >> 6, l = q & 63;
-        const int m = t.m0 + f % MF * 16 + (l & 15), n = n0 + f / MF * 16 + (l >> 4) * 4;
-        if (m >= t.m1 || n >= p.N) continue;
+        const unsigned m = (unsigned)t.m0 + f % MF * 16 + (l & 15);
+        const int n = n0 + f / MF * 16 + (l >> 4) * 4;
+        if (m >= (unsigned)t.m1 || n >= p.N) continue;
         float r[4] = {o.x, o.y, o.z, o.w};
         if (p.bias != nullptr) {
 #pragma unroll
@@ -302,7 +303,7 @@ hipError_t mxfp4_gemm_fused_launch(const MxProblem& p, const void* x, int G, hip
 
 // x quantized with scales in rows.  32 rows a tile, 16 where one tile or an expert's rows on average are no more.
 hipError_t mxfp4_gemm_few_launch(const MxProblem& p, hipStream_t st) {
-    const int rows = p.offsets != nullptr ? 2 * ((p.R + p.E - 1) / p.E) : p.R;
+    const long long rows = p.offsets != nullptr ? 2 * ((p.R + p.E - 1LL) / p.E) : p.R;
     return rows <= 16 ? few_go<0, 0, 1, 2, false>(p, nullptr, st) : few_go<0, 0, 2, 2, false>(p, nullptr, st);
 }
 

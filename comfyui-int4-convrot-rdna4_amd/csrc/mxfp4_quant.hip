@@ -80,19 +80,20 @@ __global__ __launch_bounds__(256) void mxfp4_quant_rows_kernel(const uint8_t* __
     const int per = Ks / 16;
     const int ss = b % per, row0 = (int)(b / per) * 8;
     const int r = threadIdx.x >> 5, l = threadIdx.x & 31;
-    const int row = row0 + r, k = ss * 512 + l * 16;
+    const unsigned row = (unsigned)row0 + r;
+    const int k = ss * 512 + l * 16;
     float v[16];
 #pragma unroll
     for (int i = 0; i < 16; ++i) v[i] = 0.0f;
-    if (row < M && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
+    if (row < (unsigned)M && k < K) load16<DT>(x + ((size_t)row * K + k) * ES, v);
     rotate16<G>(v);
     uint32_t sb;
     const v2u_mx c = mx_encode16(v, sb);
-    if (row < M && k < Kp) *reinterpret_cast<v2u_mx*>(codes + (size_t)row * (Kp / 2) + k / 2) = c;
+    if (row < (unsigned)M && k < Kp) *reinterpret_cast<v2u_mx*>(codes + (size_t)row * (Kp / 2) + k / 2) = c;
     if ((l & 1) == 0) sc[r][TILES ? mx_scale_place(l >> 1) : l >> 1] = (uint8_t)sb;
     __syncthreads();
-    const int m = row0 + threadIdx.x;
-    if (threadIdx.x < 8 && m < M)
+    const unsigned m = row0 + threadIdx.x;
+    if (threadIdx.x < 8 && m < (unsigned)M)
         *reinterpret_cast<v4u_mx*>(scales + (TILES ? ((size_t)ss * M + m) * 16 : (size_t)m * Ks + ss * 16)) =
                 *reinterpret_cast<const v4u_mx*>(sc[threadIdx.x]);
 }

@@ -285,7 +285,8 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
         int ln = lane;                                     // not the lane's value: no address of the store waits in
         asm volatile("" : "+v"(ln));                       // registers during the main loop
         const int el = ln & 31, eh = ln >> 5, unit = ln % U, prow = ln / U;
-        const int m0 = t.m0 + wm * 32 * FM, m1 = t.m1, c0 = n0 + wn * 32 * FN;
+        const unsigned m0 = (unsigned)t.m0 + wm * 32 * FM, m1 = t.m1;
+        const int c0 = n0 + wn * 32 * FN;
         uint8_t* scr = lds_mx + wave * SCR;
         // piece x: columns c = x / FM, rows i = x % FM; 16-byte unit u of a row at u ^ (row % U) against bank conflicts
         auto store = [&](auto edge) __attribute__((always_inline)) {
@@ -323,7 +324,8 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
                 __builtin_amdgcn_sched_barrier(0);
 #pragma unroll
                 for (int y = 0; y < 32 / ROWS; ++y) {
-                    const int m = m0 + i * 32 + y * ROWS + prow, col = c0 + c * CP + unit * (16 / ES);
+                    const unsigned m = m0 + i * 32 + y * ROWS + prow;
+                    const int col = c0 + c * CP + unit * (16 / ES);
                     uint8_t* o = reinterpret_cast<uint8_t*>(p.out) + ((size_t)m * p.N + col) * ES;
                     // not kept in L2, where the next tiles' operands are
                     if constexpr (!EDGE) __builtin_nontemporal_store(w[y], reinterpret_cast<v4u_mx*>(o));

@@ -423,7 +423,7 @@ int cr_convrot_dequant(const void* q, int bits, const void* scale, void* out, in
  *   bias_dtype.  workspace: >= cr_mxfp4_linear_workspace(M, N, K, 1) bytes.
  * cr_mxfp4_tile: the kernel of such a product, or (experts > 0) of R routed rows:
  *   0 the one for few rows, 128 or 256 the staged tile's side.
- * Pointers 16-byte aligned; K <= 2^24.
+ * Pointers 16-byte aligned; K <= 2^24, N <= 2^31 - 256.
  */
 int cr_mxfp4_tile(int R, int N, int K, int experts);
 int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream);

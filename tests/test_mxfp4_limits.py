@@ -1,5 +1,7 @@
 """CPU checks: sizes past what a call takes are refused by name, before they are cut to 32 bits on the way to the library.
 Expanded tensors of one element stand for the large ones."""
+import ctypes
+
 import pytest
 import torch
 
@@ -46,6 +48,18 @@ def test_more_than_32_bits_of_columns_or_rows(backend, n):
         backend.quantize_mxfp4(big(n, 32))
     with pytest.raises(ValueError, match="more than one call takes"):
         backend.dequantize_mxfp4(big(n, 16, dtype=u), big(n, 1, dtype=u))
+
+
+def test_columns_that_a_tile_cannot_count(backend, native):
+    """A tile's columns past the last one are counted in 31 bits."""
+    n, u = 2 ** 31 - 255, torch.uint8
+    with pytest.raises(ValueError, match="more than one call takes"):
+        backend.mxfp4_linear(big(1, 32), big(n, 16, dtype=u), big(n, 1, dtype=u))
+    with pytest.raises(ValueError, match="more than one call takes"):
+        backend.mxfp4_expert_linear(big(1, 32), big(2, n, 16, dtype=u), big(2, n, 1, dtype=u), plan_of(backend, 1))
+    lib, z = native.load_library(), ctypes.c_void_p(0)
+    assert lib.cr_mxfp4_linear(z, 1, z, z, z, 0, z, 1, n, 32, 0, z, 1 << 40, z) == -1
+    assert lib.cr_mxfp4_expert_linear(z, 1, z, 1, ctypes.c_void_p(16), 2, z, z, z, 0, z, 1, n, 32, 0, z, 1 << 40, z) == -1
 
 
 def test_plans_past_their_limits(backend):
