@@ -83,6 +83,7 @@ _SIGNATURES = {
     "cr_convrot_w4a4_linear_packed_workspace": ([_i, _i, _i, _i], ctypes.c_size_t),
     "cr_convrot_dequant": ([_vp, _i, _vp, _vp, _i, _i, _i, _i, _vp], _i),
     "cr_mxfp4_tile": ([_i] * 4, _i),
+    "cr_mxfp4_kernel": ([_i] * 5 + [_vp], _i),
     "cr_mxfp4_quant": ([_vp, _i, _vp, _vp, _i, _i, _i, _vp], _i),
     "cr_mxfp4_dequant": ([_vp, _vp, _vp, _i, _i, _i, _i, _vp], _i),
     "cr_mxfp4_linear_workspace": ([_i] * 4, ctypes.c_size_t),

@@ -51,6 +51,8 @@ hipError_t mxfp4_quant_launch(const void* x, int dt, void* codes, void* scales, 
 hipError_t mxfp4_operands_launch(const void* x, int G, const MxProblem& p, bool tiles, hipStream_t st);
 int mxfp4_gemm_tile(const MxProblem& p);
 bool mxfp4_gemm_staged(const MxProblem& p);
+MxKernel mxfp4_staged_kernel(const MxProblem& p);
+MxKernel mxfp4_few_kernel(const MxProblem& p);
 hipError_t mxfp4_dequant_launch(const void* codes, const void* scales, void* out, int dt, int M, int K, int G,
                                 hipStream_t st);
 hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st);
@@ -602,13 +604,37 @@ API size_t cr_mxfp4_linear_workspace(int M, int N, int K, int E) {
     return M <= 0 || N <= 0 || E < 1 || K <= 0 || K % convrot::MX_BLOCK != 0 ? 0 : mx_plan(M, (long long)N * E, K).total;
 }
 
-API int cr_mxfp4_tile(int R, int N, int K, int experts) {
-    if (R < 0 || N < 0 || K <= 0 || K % convrot::MX_BLOCK != 0 || experts < 0) return -1;
+// A product that is only asked about: its pointers only say whether there is something
+static convrot::MxProblem mx_asked(int R, int N, int K, int experts, int tokens) {
     static const int some = 0;
     convrot::MxProblem p{};
-    p.R = p.as_rows = R; p.N = N; p.K = K; p.E = experts > 0 ? experts : 1;
-    p.offsets = experts > 0 ? &some : nullptr;                        // only asked whether it is there
-    return convrot::mxfp4_gemm_tile(p);
+    p.R = R; p.N = N; p.K = K; p.E = experts > 0 ? experts : 1;
+    p.as_rows = tokens > 0 ? tokens : R;
+    p.Kp = mx_plan(p.as_rows, 1, K).Kp;
+    p.offsets = experts > 0 ? &some : nullptr;
+    p.order = tokens > 0 ? &some : nullptr;
+    return p;
+}
+
+static bool mx_asked_ok(int R, int N, int K, int experts, int tokens) {
+    return R >= 0 && N >= 0 && N <= convrot::MX_MAX_N && K > 0 && K <= (1 << 24) && K % convrot::MX_BLOCK == 0 && experts >= 0 &&
+           tokens >= 0 && (tokens == 0 || experts > 0);
+}
+
+API int cr_mxfp4_tile(int R, int N, int K, int experts) {
+    return mx_asked_ok(R, N, K, experts, 0) ? convrot::mxfp4_gemm_tile(mx_asked(R, N, K, experts, 0)) : -1;
+}
+
+API int cr_mxfp4_kernel(int R, int N, int K, int experts, int tokens, int* kernel) {
+    if (!mx_asked_ok(R, N, K, experts, tokens) || kernel == nullptr) return -1;
+    const convrot::MxProblem p = mx_asked(R, N, K, experts, tokens);
+    const convrot::MxKernel k = !convrot::mxfp4_gemm_fused(p) && convrot::mxfp4_gemm_staged(p) ? convrot::mxfp4_staged_kernel(p)
+                                                                                              : convrot::mxfp4_few_kernel(p);
+    kernel[0] = k.rows;
+    kernel[1] = k.cols;
+    kernel[2] = k.slots;
+    kernel[3] = k.fused;
+    return 0;
 }
 
 API int cr_mxfp4_linear(const void* x, int dtype, const void* W, const void* wscales, const void* bias, int bias_dtype,

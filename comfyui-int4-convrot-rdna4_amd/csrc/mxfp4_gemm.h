@@ -26,6 +26,13 @@ struct MxProblem {
     int k_shift;
 };
 
+// The kernel of a product: rows and columns of its tile, stages in LDS (0: the kernel for few rows), and whether that
+// quantizes x itself.
+struct MxKernel {
+    int rows, cols, slots;
+    bool fused;
+};
+
 // l = ceil(log2 d), m = ceil(2^(31 + l) / d): n m >> (31 + l) is n / d for every n < 2^31, and m < 2^32.
 inline void mx_set_top_k(MxProblem& p, int d) {
     int l = 0;

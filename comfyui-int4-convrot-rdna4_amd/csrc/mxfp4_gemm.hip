@@ -276,10 +276,20 @@ bool mxfp4_gemm_fused(const MxProblem& p) {
     return p.R <= (p.offsets != nullptr ? 8 : 4) && p.K <= FEW_MAX_K && (long long)p.R * p.Kp <= (64 << 10);
 }
 
+// Its tile.  Fused: 16 rows, 32 columns where that leaves a workgroup for each CU.  Else 32 rows, 16 where one tile or an
+// expert's rows on average are no more.
+MxKernel mxfp4_few_kernel(const MxProblem& p) {
+    if (mxfp4_gemm_fused(p)) {
+        const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 16) * ((p.N + 31) / 32);
+        return {16, tiles >= 256 ? 32 : 16, 0, true};
+    }
+    const long long rows = p.offsets != nullptr ? 2 * ((p.R + p.E - 1LL) / p.E) : p.R;
+    return {rows <= 16 ? 16 : 32, 32, 0, false};
+}
+
 template <int DT, int G>
 static hipError_t fused_go(const MxProblem& p, const void* x, hipStream_t st) {
-    const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 16) * ((p.N + 31) / 32);
-    return tiles >= 256 ? few_go<DT, G, 1, 2, true>(p, x, st) : few_go<DT, G, 1, 1, true>(p, x, st);
+    return mxfp4_few_kernel(p).cols == 32 ? few_go<DT, G, 1, 2, true>(p, x, st) : few_go<DT, G, 1, 1, true>(p, x, st);
 }
 
 template <int DT>
@@ -301,10 +311,9 @@ hipError_t mxfp4_gemm_fused_launch(const MxProblem& p, const void* x, int G, hip
     }
 }
 
-// x quantized with scales in rows.  32 rows a tile, 16 where one tile or an expert's rows on average are no more.
+// x quantized with scales in rows
 hipError_t mxfp4_gemm_few_launch(const MxProblem& p, hipStream_t st) {
-    const long long rows = p.offsets != nullptr ? 2 * ((p.R + p.E - 1LL) / p.E) : p.R;
-    return rows <= 16 ? few_go<0, 0, 1, 2, false>(p, nullptr, st) : few_go<0, 0, 2, 2, false>(p, nullptr, st);
+    return mxfp4_few_kernel(p).rows == 16 ? few_go<0, 0, 1, 2, false>(p, nullptr, st) : few_go<0, 0, 2, 2, false>(p, nullptr, st);
 }
 
 }  // namespace convrot

@@ -350,7 +350,7 @@ __global__ __launch_bounds__(256, 1) void mxfp4_gemm_staged_kernel(MxProblem p, 
     }
 }
 
-// The kernel of a product: 0 the one for few rows (mxfp4_gemm.hip), else the tile, 256 or 128 a side.
+// The kernel of a product: 0 the one for few rows (mxfp4_gemm.hip), else the tile's columns, 256 or 128.
 //
 // Up to 32 rows run there (us, there and staged: 4096 columns of K 4096 12.6 and 13.8, 2048 of K 8192 16.2 and 17.9; with
 // 64 rows 16 and 14.1, 22.3 and 18).
@@ -395,14 +395,22 @@ static hipError_t staged_go(MxProblem p, hipStream_t st) {
     });
 }
 
-template <int DT>
-static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
-    if (mxfp4_gemm_tile(p) == 256) return staged_go<DT, 4, 4, 2>(p, st);
+// The instance that a staged product runs.
+MxKernel mxfp4_staged_kernel(const MxProblem& p) {
+    if (mxfp4_gemm_tile(p) == 256) return {256, 256, 2, false};
     // One tile a CU or fewer: nothing but its own copies hides a stage's latency, so four slots; and where that leaves half
     // of the CUs idle, tiles of half the rows (256 rows of K 4096 -> 4096: two slots 18, four 17, half the rows 15.1 us).
     const long long tiles = mx_row_tiles(p.R, p.E, p.offsets != nullptr, 128) * ((p.N + 127) / 128);
-    if (tiles <= 128) return staged_go<DT, 1, 2, 4>(p, st);
-    return tiles <= 256 ? staged_go<DT, 2, 2, 4>(p, st) : staged_go<DT, 2, 2, 2>(p, st);
+    if (tiles <= 128) return {64, 128, 4, false};
+    return {128, 128, tiles <= 256 ? 4 : 2, false};
+}
+
+template <int DT>
+static hipError_t staged_type(const MxProblem& p, hipStream_t st) {
+    const MxKernel k = mxfp4_staged_kernel(p);
+    if (k.rows == 256) return staged_go<DT, 4, 4, 2>(p, st);
+    if (k.rows == 64) return staged_go<DT, 1, 2, 4>(p, st);
+    return k.slots == 4 ? staged_go<DT, 2, 2, 4>(p, st) : staged_go<DT, 2, 2, 2>(p, st);
 }
 
 hipError_t mxfp4_gemm_staged_launch(const MxProblem& p, hipStream_t st) {

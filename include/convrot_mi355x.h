@@ -421,10 +421,13 @@ int cr_convrot_dequant(const void* q, int bits, const void* scale, void* out, in
  *   [M, ..] of `dtype`, W codes [N, K/2] with scales [N, K/32] as cr_mxfp4_quant
  *   writes them; products and sums in fp32, rounded once; bias NULL or of
  *   bias_dtype.  workspace: >= cr_mxfp4_linear_workspace(M, N, K, 1) bytes.
- * cr_mxfp4_tile: the kernel of such a product, or (experts > 0) of R routed rows:
- *   0 the one for few rows, 128 or 256 the staged tile's side.
+ * cr_mxfp4_kernel: the kernel of such a product, or (experts > 0) of R routed rows, which x has in the plan's order
+ *   (tokens 0) or which are taken from its `tokens` rows: kernel[0], [1] the rows and columns of its tile,
+ *   kernel[2] the stages of 256 k in LDS (0: the kernel for few rows), kernel[3] whether it quantizes x itself.
+ * cr_mxfp4_tile: of R rows of x, 0 for few rows, else the staged tile's columns, 128 or 256.
  * Pointers 16-byte aligned; K <= 2^24, N <= 2^31 - 256.
  */
+int cr_mxfp4_kernel(int R, int N, int K, int experts, int tokens, int* kernel);
 int cr_mxfp4_tile(int R, int N, int K, int experts);
 int cr_mxfp4_quant(const void* x, int in_dtype, void* codes, void* scales, int M, int K, int G, void* stream);
 int cr_mxfp4_dequant(const void* codes, const void* scales, void* out, int out_dtype, int M, int K, int G,
