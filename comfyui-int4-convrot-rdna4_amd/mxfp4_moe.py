@@ -4,7 +4,7 @@ operators of ``_int4.mxfp4`` and ``_int4.experts`` are for, run together.
     moe = Mxfp4MoE.from_float(w_gate, w_up, w_down, convrot_groupsize=256)
     y = moe(x, expert_ids, weights)
 
-``expert_ids`` [..., k] is the router's choice (an id outside [0, E) leaves a
+``x`` is [..., D]; ``expert_ids`` [..., k] is the router's choice (an id outside [0, E) leaves a
 slot unused), ``weights`` [..., k] what it gives each.  A token's output is
 ``sum_j weights[j] * down_e(silu(gate_e(x)) * up_e(x))``.  The experts are frozen
 and run without a graph; the router's weights get their gradient, so a router
@@ -43,6 +43,9 @@ class Mxfp4MoE(torch.nn.Module):
     def forward(self, x: torch.Tensor, expert_ids: torch.Tensor, weights: torch.Tensor) -> torch.Tensor:
         if torch.is_grad_enabled() and x.requires_grad:
             raise RuntimeError("the experts are frozen: gradients reach the router's weights only; pass x.detach()")
+        if expert_ids.dim() == 0 or weights.shape != expert_ids.shape or expert_ids.shape[:-1] != x.shape[:-1]:
+            raise ValueError(f"expert_ids of shape {tuple(expert_ids.shape)} and weights of shape {tuple(weights.shape)} do not "
+                             f"fit x of shape {tuple(x.shape)}")
         k = expert_ids.shape[-1]
         G = self.convrot_groupsize
         x2 = x.reshape(-1, x.shape[-1])
