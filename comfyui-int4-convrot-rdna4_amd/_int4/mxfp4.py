@@ -11,7 +11,8 @@ groups of that many values (the products stay the same, outliers are spread over
 their group); None does not.
 
 The forms here are for inference: they have no gradient, and refuse an input
-that asks for one.
+that asks for one.  Their kernels are no torch operations, so a trace is refused
+too.
 """
 from __future__ import annotations
 

@@ -214,7 +214,8 @@ struct RowVec {                              // 16 bytes of a row as floats
     }
 };
 
-// One piece of a row: 16 bytes (VEC) or one element.
+// One piece of a row: 16 bytes (VEC) or one element, where rows are no whole number of 16 bytes.  8192 tokens of 4095
+// bf16 to 4 experts so: gather 156 us, combine 191, its gradient 203; of 4096 in 16 bytes 65, 57 and 121.
 template <int DT, bool VEC>
 struct Piece {
     static constexpr int N = VEC ? RowVec<DT>::N : 1;

@@ -1,7 +1,6 @@
 // Host path of the linears, of the microscaled 4-bit tier and of expert routing:
-// one native call per forward for the calls a model
-// makes (contiguous GPU activations, operands as the layers keep them).  It
-// checks the operands, allocates the output and the intermediates and calls the
+// one native call per forward for the calls a model makes (contiguous GPU
+// activations, operands as the layers keep them, no trace).  It checks the operands, allocates the output and the intermediates and calls the
 // library; anything else returns None and takes the Python path, which handles
 // every form and raises the errors.
 //

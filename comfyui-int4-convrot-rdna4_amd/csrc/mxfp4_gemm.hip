@@ -269,9 +269,10 @@ static hipError_t few_go(MxProblem p, const void* x, hipStream_t st) {
     });
 }
 
-// Rows that each workgroup quantizes itself: few of them in a tile, so that the work is less than a launch costs (5120 ->
-// 13824, us: 1 row 11.9, 4 rows 15.6, 8 rows 22.1, quantized in a launch of their own 16.1), and their codes fit its LDS.
-// Experts' rows are spread over the tiles.
+// Rows that each workgroup quantizes itself: few of them in a tile, so that the work is less than a launch costs, and their
+// codes fit its LDS.  us, in the product and ahead of it: 5120 -> 13824 1 row 9.3 and 12.1, 2 rows 10.6 and 12.2, 4 rows
+// 12.9 and 12.5, 8 rows 19.1 and 12.8; 4096 -> 4096 4 rows 6.7 and 8.1, 8 rows 9.3 and 8.3.  Experts' rows are spread over
+// the tiles: 2048 -> 4096, 1 token's four 7.5 and 9.4, 2 tokens' eight 11.5 and 14.3.
 bool mxfp4_gemm_fused(const MxProblem& p) {
     return p.R <= (p.offsets != nullptr ? 8 : 4) && p.K <= FEW_MAX_K && (long long)p.R * p.Kp <= (64 << 10);
 }

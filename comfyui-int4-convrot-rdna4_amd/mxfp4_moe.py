@@ -4,8 +4,9 @@ operators of ``_int4.mxfp4`` and ``_int4.experts`` are for, run together.
     moe = Mxfp4MoE.from_float(w_gate, w_up, w_down, convrot_groupsize=256)
     y = moe(x, expert_ids, weights)
 
-``x`` is [..., D]; ``expert_ids`` [..., k] is the router's choice (an id outside [0, E) leaves a
-slot unused), ``weights`` [..., k] what it gives each.  A token's output is
+``x`` is [..., D], ``expert_ids`` [..., k] the router's choice (an id outside
+[0, E) leaves a slot unused), ``weights`` [..., k] what it gives each, with the
+same leading sizes.  A token's output is
 ``sum_j weights[j] * down_e(silu(gate_e(x)) * up_e(x))``.  The experts are frozen
 and run without a graph; the router's weights get their gradient, so a router
 can be trained over them.
