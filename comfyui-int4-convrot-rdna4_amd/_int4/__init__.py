@@ -15,7 +15,9 @@ Public API:
 Beside the reference's API, the microscaled 4-bit tier (``mxfp4``:
 quantize_mxfp4, dequantize_mxfp4, mxfp4_linear, mxfp4_expert_linear) and expert
 routing (``experts``: sort_tokens_by_expert, gather_expert_rows,
-combine_expert_rows).
+combine_expert_rows), with the router's choice in front of it (``router``:
+choose_experts) and the norm in front of both (``norm``: rms_norm, rms_norm_int8
+and the int8 linear of its rows, convrot_w8a8_linear_rows).
 
 Numerics are those of the reference eager path (``_int4/eager.py``): packed
 codes and scales equal the eager ones, the integer accumulators are exact, and
@@ -33,6 +35,8 @@ from ._codec import _INT4_GROUP_SIZE, _INT4_MAX, _pack_int4_row_major, _unpack_i
 from .native import is_available as _native_available
 from .experts import ExpertPlan, combine_expert_rows, gather_expert_rows, max_experts, sort_tokens_by_expert
 from .mxfp4 import dequantize_mxfp4, mxfp4_expert_linear, mxfp4_linear, quantize_mxfp4
+from .norm import Int8Rows, convrot_w8a8_linear_rows, max_norm_width, rms_norm, rms_norm_int8
+from .router import choose_experts
 
 __all__ = [
     "quantize_convrot_w4a4_weight",
@@ -57,6 +61,12 @@ __all__ = [
     "sort_tokens_by_expert",
     "gather_expert_rows",
     "combine_expert_rows",
+    "choose_experts",
+    "rms_norm",
+    "rms_norm_int8",
+    "Int8Rows",
+    "max_norm_width",
+    "convrot_w8a8_linear_rows",
 ]
 
 # largest concatenated rank of the fused LoRA side path (padded to a multiple of 32)

@@ -20,8 +20,9 @@ _HERE = os.path.dirname(os.path.abspath(__file__))
 _PKG = os.path.dirname(_HERE)
 _CSRC = os.path.join(_PKG, "csrc")
 SOURCES = ("rotquant.hip", "gemm.hip", "gemm_bf6.hip", "gemm_bf6_direct.hip", "gemm_int.hip", "lora.hip", "dequant.hip",
-           "mxfp4_quant.hip", "mxfp4_gemm.hip", "mxfp4_staged.hip", "experts.hip", "capi.hip")
-HEADERS = ("common.h", "gemm_common.h", "gemm_direct.h", "gemm_int.h", "b6t_layout.h", "mxfp4.h", "mxfp4_gemm.h")
+           "mxfp4_quant.hip", "mxfp4_gemm.hip", "mxfp4_staged.hip", "experts.hip", "router.hip", "rmsnorm.hip", "capi.hip")
+HEADERS = ("common.h", "gemm_common.h", "gemm_direct.h", "gemm_int.h", "b6t_layout.h", "mxfp4.h", "mxfp4_gemm.h", "lanes.h",
+           "rotate64.h", "router.h", "rmsnorm.h")
 ARCH = "gfx950"
 
 

@@ -96,6 +96,15 @@ _SIGNATURES = {
     "cr_expert_gather": ([_vp, _i, _vp, _vp, _vp] + [_i] * 4 + [_vp], _i),
     "cr_expert_combine": ([_vp, _i, _vp, _vp, _vp] + [_i] * 3 + [_vp], _i),
     "cr_expert_combine_grad": ([_vp, _i] + [_vp] * 6 + [_i] * 4 + [_vp], _i),
+    "cr_choose_experts": ([_vp, _i, _vp, _vp, _vp] + [_i] * 8 + [ctypes.c_float, _vp], _i),
+    "cr_choose_experts_grad": ([_vp, _i, _vp, _vp, _vp] + [_i] * 5 + [ctypes.c_float, _vp], _i),
+    "cr_max_norm_width": ([], _i),
+    "cr_rms_norm": ([_vp, _i, _vp, _vp, _i, _vp, _vp, _i, _i, ctypes.c_double, _vp], _i),
+    "cr_rms_norm_grad_workspace": ([_i, _i], ctypes.c_size_t),
+    "cr_rms_norm_grad": ([_vp, _vp, _vp, _i, _vp, _i, _vp, _vp, _i, _i, ctypes.c_double, _vp, ctypes.c_size_t, _vp], _i),
+    "cr_rms_norm_int8": ([_vp, _i, _vp, _vp, _i, _vp, _vp, _vp] + [_i] * 4 + [ctypes.c_double, _vp], _i),
+    "cr_w8a8_rows_linear_workspace": ([_i] * 3, ctypes.c_size_t),
+    "cr_w8a8_rows_linear": ([_vp] * 5 + [_i, _vp] + [_i] * 4 + [_vp, ctypes.c_size_t, _vp], _i),
     "cr_max_quant_k": ([], _i),
     "cr_abi_version": ([], _i),
 }
@@ -137,7 +146,7 @@ def load_library():
 
 _host = None
 _HOST_FUNCTIONS = ("w4a4", "w8a8", "mx_quantize", "mx_dequantize", "mx_linear", "mx_expert_linear", "expert_sort",
-                   "expert_gather", "expert_combine")
+                   "expert_gather", "expert_combine", "choose_experts", "rms_norm", "rms_norm_int8", "w8a8_rows")
 
 
 def host_module():

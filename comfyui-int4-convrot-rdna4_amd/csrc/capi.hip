@@ -4,6 +4,8 @@
 #include "../../include/convrot_mi355x.h"
 #include "gemm_common.h"
 #include "mxfp4_gemm.h"
+#include "rmsnorm.h"
+#include "router.h"
 
 namespace convrot {
 hipError_t rotquant_launch(const void* x, int in_dtype, const void* noise, int8_t* q, float* s,
@@ -711,6 +713,103 @@ API int cr_expert_combine_grad(const void* rows, int dtype, const float* weights
     if (T == 0) return 0;
     return (int)convrot::expert_combine_grad_launch(rows, dtype, weights, position, offsets, d_out, d_rows, d_weights, T, k, E,
                                                     D, reinterpret_cast<hipStream_t>(stream));
+}
+
+// ---------------------------------------------------------------------------
+// The router's choice, the norm in front of a block's linears, and 8-bit rows
+// ---------------------------------------------------------------------------
+
+static int choice_ok(int dtype, int T, int E, int k, float scale) {
+    return dtype >= 0 && dtype <= 2 && T >= 0 && E >= 1 && E <= convrot::router_max_experts() && k >= 1 && k <= E &&
+           (long long)T * k < (1ll << 31) && scale - scale == 0.0f;
+}
+
+API int cr_choose_experts(const void* logits, int dtype, const float* bias, int* ids, float* weights, int T, int E, int k,
+                          int sigmoid, int groups, int top_groups, int group_sum2, int renormalize, float scale, void* stream) {
+    if (!choice_ok(dtype, T, E, k, scale) || groups < 1 || E % groups != 0 || top_groups < 1 || top_groups > groups ||
+        k > E / groups * top_groups)
+        return -1;
+    if (T == 0) return 0;
+    convrot::RouterArgs a{};
+    a.logits = logits; a.bias = bias; a.ids = ids; a.weights = weights;
+    a.T = T; a.E = E; a.k = k;
+    a.groups = top_groups == groups ? 1 : groups;                      // all groups stay: none to rank
+    a.top_groups = top_groups;
+    a.scale = scale; a.sigmoid = sigmoid != 0; a.sum2 = group_sum2 != 0; a.renormalize = renormalize != 0;
+    return (int)convrot::choose_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_choose_experts_grad(const void* logits, int dtype, const int* ids, const float* d_weights, void* d_logits, int T, int E,
+                               int k, int sigmoid, int renormalize, float scale, void* stream) {
+    if (!choice_ok(dtype, T, E, k, scale)) return -1;
+    if (T == 0) return 0;
+    convrot::RouterGradArgs a{};
+    a.logits = logits; a.ids = ids; a.d_weights = d_weights; a.d_logits = d_logits;
+    a.T = T; a.E = E; a.k = k; a.scale = scale; a.sigmoid = sigmoid != 0; a.renormalize = renormalize != 0;
+    return (int)convrot::choose_grad_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+static int norm_ok(int dtype, int weight_dtype, int M, int D, double eps) {
+    return dtype >= 0 && dtype <= 2 && weight_dtype >= 0 && weight_dtype <= 2 && M >= 0 && D >= 1 && D <= convrot::NORM_MAX_D &&
+           eps >= 0.0;
+}
+
+API int cr_max_norm_width(void) { return convrot::NORM_MAX_D; }
+
+API int cr_rms_norm(const void* x, int dtype, const void* residual, const void* weight, int weight_dtype, void* h, void* y, int M,
+                    int D, double eps, void* stream) {
+    if (!norm_ok(dtype, weight_dtype, M, D, eps) || (residual != nullptr && h == nullptr)) return -1;
+    if (M == 0) return 0;
+    convrot::NormArgs a{};
+    a.x = x; a.residual = residual; a.weight = weight; a.h = h; a.y = y;
+    a.eps = eps; a.M = M; a.D = D; a.weight_dt = weight_dtype;
+    return (int)convrot::norm_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+API size_t cr_rms_norm_grad_workspace(int M, int D) {
+    return M <= 0 || D < 1 || D > convrot::NORM_MAX_D ? 0 : kSplitCounterBytes + convrot::norm_grad_bytes(M, D);
+}
+
+API int cr_rms_norm_grad(const void* d_y, const void* d_h, const void* h, int dtype, const void* weight, int weight_dtype, void* d_x,
+                         void* d_weight, int M, int D, double eps, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!norm_ok(dtype, weight_dtype, M, D, eps) || (d_weight != nullptr && weight == nullptr)) return -1;
+    if (M == 0) return 0;
+    convrot::NormGradArgs a{};
+    a.d_y = d_y; a.d_h = d_h; a.h = h; a.weight = weight; a.d_x = d_x; a.d_weight = d_weight;
+    a.eps = eps; a.M = M; a.D = D; a.weight_dt = weight_dtype;
+    if (d_weight != nullptr) {
+        if (workspace == nullptr || workspace_bytes < cr_rms_norm_grad_workspace(M, D)) return -1;
+        a.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + kSplitCounterBytes);
+    }
+    return (int)convrot::norm_grad_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+}
+
+API int cr_rms_norm_int8(const void* x, int dtype, const void* residual, const void* weight, int weight_dtype, void* h, void* codes,
+                         float* scales, int M, int D, int G, int tiled, double eps, void* stream) {
+    if (!norm_ok(dtype, weight_dtype, M, D, eps) || (residual != nullptr && h == nullptr) || !quant_args_ok(dtype, M, D, G) ||
+        (tiled && D % 64 != 0))
+        return -1;
+    if (M == 0) return 0;
+    convrot::NormArgs a{};
+    a.x = x; a.residual = residual; a.weight = weight; a.h = h; a.y = codes; a.scales = scales;
+    a.eps = eps; a.M = M; a.D = D; a.weight_dt = weight_dtype;
+    return (int)convrot::norm_int8_launch(a, dtype, G, tiled != 0, reinterpret_cast<hipStream_t>(stream));
+}
+
+API size_t cr_w8a8_rows_linear_workspace(int M, int N, int K) {
+    return M <= 0 || N <= 0 || !i8t_k_ok(K) ? 0 : int_plan(8, M, N, K, 0).a6;
+}
+
+API int cr_w8a8_rows_linear(const void* X8, const float* xscale, const void* W8, const void* wscale, const void* bias, int bias_dtype,
+                            void* out, int epilogue, int M, int N, int K, void* workspace, size_t workspace_bytes, void* stream) {
+    if (!i8t_k_ok(K) || M < 0 || N < 0 || bias_dtype < 0 || bias_dtype > 2) return -1;
+    if (epilogue != convrot::EPI_F32 && epilogue != convrot::EPI_BF16 && epilogue != convrot::EPI_F16) return -1;
+    if (M == 0 || N == 0) return 0;
+    const LinPlan p = int_plan(8, M, N, K, 0);
+    if (workspace == nullptr || workspace_bytes < p.a6) return -1;
+    return (int)convrot::gemm_i8t_launch(reinterpret_cast<const int8_t*>(X8), reinterpret_cast<const int8_t*>(W8), xscale,
+                                         reinterpret_cast<const float*>(wscale), bias, bias_dtype, out, M, N, K, epilogue,
+                                         p.nsplit > 1 ? workspace : nullptr, reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_max_quant_k(void) { return convrot::rotquant_max_k(); }

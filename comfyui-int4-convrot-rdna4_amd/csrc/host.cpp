@@ -532,7 +532,282 @@ PyObject* expert_combine(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// ---------------------------------------------------------------------------
+// The router's choice (_int4/router.py) and the norm (_int4/norm.py)
+// ---------------------------------------------------------------------------
+
+struct Choice {
+    at::Tensor bias;           // undefined: none
+    int k, sigmoid, groups, top_groups, sum2, renormalize;
+    float scale;
+};
+
+bool whole(PyObject* o, long* v) {
+    if (!PyLong_CheckExact(o)) return false;
+    *v = PyLong_AsLong(o);
+    if (*v == -1 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+
+// A float or an int as a double; false for other objects
+bool real(PyObject* o, double* v) {
+    if (!PyFloat_CheckExact(o) && !PyLong_CheckExact(o)) return false;
+    *v = PyFloat_AsDouble(o);
+    if (*v == -1.0 && PyErr_Occurred()) { PyErr_Clear(); return false; }
+    return true;
+}
+
+int64_t rows_of(const at::Tensor& t) { return t.numel() / t.size(-1); }
+
+std::vector<int64_t> with_last(const at::Tensor& t, int64_t n) {
+    std::vector<int64_t> sizes(t.sizes().begin(), t.sizes().end());
+    sizes.back() = n;
+    return sizes;
+}
+
+std::pair<at::Tensor, at::Tensor> choose(const at::Tensor& logits, const Choice& c) {
+    const auto sizes = with_last(logits, c.k);
+    at::Tensor ids = like(logits, sizes, at::kInt), weights = like(logits, sizes, at::kFloat);
+    const int rc = cr_choose_experts(logits.const_data_ptr(), dtype_code(logits), (const float*)ptr(c.bias), (int*)ids.mutable_data_ptr(),
+                                     (float*)weights.mutable_data_ptr(), (int)rows_of(logits), (int)logits.size(-1), c.k, c.sigmoid,
+                                     c.groups, c.top_groups, c.sum2, c.renormalize, c.scale, stream_of(logits.device()));
+    TORCH_CHECK(rc == 0, "cr_choose_experts failed, hipError=", rc);
+    return {ids, weights};
+}
+
+struct Choose : torch::autograd::Function<Choose> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& logits, const Choice& c) {
+        auto [ids, weights] = choose(logits, c);
+        ctx->save_for_backward({logits, ids});
+        ctx->mark_non_differentiable({ids});
+        ctx->saved_data["how"] = std::vector<int64_t>{c.sigmoid, c.renormalize, logits.size(-1), (int64_t)logits.scalar_type()};
+        ctx->saved_data["scale"] = (double)c.scale;
+        return {ids, weights};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        at::Tensor d_logits;
+        {
+            at::NoGradGuard no_grad;
+            const auto saved = ctx->get_saved_variables();
+            const auto how = ctx->saved_data["how"].toIntVector();
+            const at::Tensor d_w = settled(g[1]);
+            const c10::Device dev = d_w.device();
+            const at::Tensor ids = restored(saved[1], "ids", at::kInt, d_w.sizes(), dev);
+            const at::Tensor logits = restored(saved[0], "logits", (at::ScalarType)how[3], with_last(d_w, how[2]), dev);
+            d_logits = like(logits, logits.sizes(), logits.scalar_type());
+            const int rc = cr_choose_experts_grad(logits.const_data_ptr(), dtype_code(logits), (const int*)ids.const_data_ptr(),
+                                                  (const float*)d_w.const_data_ptr(), d_logits.mutable_data_ptr(), (int)rows_of(logits),
+                                                  (int)how[2], (int)ids.size(-1), (int)how[0], (int)how[1],
+                                                  (float)ctx->saved_data["scale"].toDouble(), stream_of(dev));
+            TORCH_CHECK(rc == 0, "cr_choose_experts_grad failed, hipError=", rc);
+        }
+        return once({d_logits, at::Tensor()});
+    }
+};
+
+PyObject* tuple_of(std::initializer_list<at::Tensor> ts) {
+    PyObject* t = PyTuple_New((Py_ssize_t)ts.size());
+    if (t == nullptr) return nullptr;
+    Py_ssize_t i = 0;
+    for (const at::Tensor& v : ts) {
+        PyObject* o = THPVariable_Wrap(v);
+        if (o == nullptr) { Py_DECREF(t); return nullptr; }
+        PyTuple_SET_ITEM(t, i++, o);
+    }
+    return t;
+}
+
+// choose_experts(logits, k, bias, sigmoid, groups, top_groups, sum2, renormalize, scale) -> (ids, weights)
+PyObject* choose_experts(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor logits, bias;
+    c10::Device dev(c10::kCPU);
+    long k, groups, top;
+    double scale;
+    if (n != 9 || !operand(a[0], &logits, &dev, true) || logits.dim() < 1 || logits.numel() == 0 || dtype_code(logits) < 0 ||
+        !whole(a[1], &k) || !whole(a[4], &groups) || !real(a[8], &scale))
+        Py_RETURN_NONE;
+    if (a[5] == Py_None) top = groups;
+    else if (!whole(a[5], &top)) Py_RETURN_NONE;
+    if (a[2] != Py_None && (!operand(a[2], &bias, &dev) || bias.scalar_type() != at::kFloat || bias.dim() != 1 ||
+                            bias.size(0) != logits.size(-1)))
+        Py_RETURN_NONE;
+    const int64_t E = logits.size(-1), T = rows_of(logits);
+    if (E > cr_max_experts() || groups < 1 || groups > E || E % groups != 0 || top < 1 || top > groups || k < 1 ||
+        k > E / groups * top || T > INT32_MAX || T * k > INT32_MAX || !(scale >= -3.4028234663852886e38 && scale <= 3.4028234663852886e38) ||
+        (a[3] != Py_True && a[3] != Py_False) || (a[6] != Py_True && a[6] != Py_False) || (a[7] != Py_True && a[7] != Py_False))
+        Py_RETURN_NONE;
+    const Choice c{bias, (int)k, a[3] == Py_True, (int)groups, (int)top, a[6] == Py_True, a[7] == Py_True, (float)scale};
+    if (wants_grad(logits)) {
+        const auto out = Choose::apply(logits, c);
+        return tuple_of({out[0], out[1]});
+    }
+    auto [ids, weights] = choose(logits, c);
+    return tuple_of({ids, weights});
+    END_HANDLE_TH_ERRORS
+}
+
+// The operands of a norm; weight and residual undefined: none
+struct Norm {
+    at::Tensor x, weight, residual;
+    c10::Device dev = c10::Device(c10::kCPU);
+    double eps;
+    int M, D, wdt;
+    bool take(PyObject* ox, PyObject* ow, PyObject* orr, PyObject* oe) {
+        if (!operand(ox, &x, &dev, true) || x.dim() < 1 || x.numel() == 0 || dtype_code(x) < 0 || x.size(-1) > cr_max_norm_width() ||
+            rows_of(x) > INT32_MAX || !real(oe, &eps) || !(eps >= 0.0 && eps < HUGE_VAL))
+            return false;
+        D = (int)x.size(-1);
+        M = (int)rows_of(x);
+        wdt = 0;
+        if (ow != Py_None) {
+            if (!operand(ow, &weight, &dev) || weight.dim() != 1 || weight.size(0) != D) return false;
+            wdt = dtype_code(weight);
+            if (wdt < 0) return false;
+        }
+        return orr == Py_None || (operand(orr, &residual, &dev) && residual.scalar_type() == x.scalar_type() && residual.sizes() == x.sizes());
+    }
+};
+
+// (y, h), h undefined without a residual
+std::pair<at::Tensor, at::Tensor> norm(const at::Tensor& x, const at::Tensor& weight, const at::Tensor& residual, double eps) {
+    at::Tensor y = like(x, x.sizes(), x.scalar_type()), h;
+    if (residual.defined()) h = like(x, x.sizes(), x.scalar_type());
+    const int rc = cr_rms_norm(x.const_data_ptr(), dtype_code(x), ptr(residual), ptr(weight), weight.defined() ? dtype_code(weight) : 0,
+                               h.defined() ? h.mutable_data_ptr() : nullptr, y.mutable_data_ptr(), (int)rows_of(x), (int)x.size(-1), eps,
+                               stream_of(x.device()));
+    TORCH_CHECK(rc == 0, "cr_rms_norm failed, hipError=", rc);
+    return {y, h};
+}
+
+struct RmsNorm : torch::autograd::Function<RmsNorm> {
+    static torch::autograd::variable_list forward(torch::autograd::AutogradContext* ctx, const at::Tensor& x,
+                                                  const std::optional<at::Tensor>& some_weight, const std::optional<at::Tensor>& residual,
+                                                  double eps) {
+        const at::Tensor weight = some_weight.value_or(at::Tensor());
+        auto [y, h] = norm(x, weight, residual.value_or(at::Tensor()), eps);
+        ctx->save_for_backward({h.defined() ? h : x, weight});
+        ctx->saved_data["eps"] = eps;
+        ctx->saved_data["sizes"] = x.sizes().vec();
+        ctx->saved_data["types"] = std::vector<int64_t>{(int64_t)x.scalar_type(), weight.defined() ? (int64_t)weight.scalar_type() : -1};
+        ctx->saved_data["residual"] = h.defined();
+        ctx->set_materialize_grads(false);
+        return h.defined() ? torch::autograd::variable_list{y, h} : torch::autograd::variable_list{y};
+    }
+    static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
+        const auto types = ctx->saved_data["types"].toIntVector();
+        // the tensors that are there count
+        const bool has_w = types[1] >= 0, has_r = ctx->saved_data["residual"].toBool();
+        const bool need_x = ctx->needs_input_grad(0), need_w = has_w && ctx->needs_input_grad(1),
+                   need_r = has_r && ctx->needs_input_grad(has_w ? 2 : 1);
+        at::Tensor d_x, d_w;
+        if (!g[0].defined()) {
+            if (g.size() > 1) d_x = g[1];
+        } else {
+            at::NoGradGuard no_grad;
+            const auto saved = ctx->get_saved_variables();
+            const auto sizes = ctx->saved_data["sizes"].toIntVector();
+            const double eps = ctx->saved_data["eps"].toDouble();
+            const at::Tensor d_y = settled(g[0]), d_h = g.size() > 1 && g[1].defined() ? settled(g[1]) : at::Tensor();
+            const c10::Device dev = d_y.device();
+            const at::Tensor h = restored(saved[0], "rows", (at::ScalarType)types[0], sizes, dev);
+            const at::Tensor w = !has_w ? at::Tensor() : restored(saved[1], "weight", (at::ScalarType)types[1], {sizes.back()}, dev);
+            if (need_x || need_r) d_x = like(h, h.sizes(), h.scalar_type());
+            if (need_w) d_w = like(w, w.sizes(), w.scalar_type());
+            const int M = (int)rows_of(h), D = (int)h.size(-1);
+            const size_t bytes = need_w ? cr_rms_norm_grad_workspace(M, D) : 0;
+            const at::Tensor ws = like(h, {(int64_t)bytes}, at::kByte);
+            const int rc = cr_rms_norm_grad(d_y.const_data_ptr(), ptr(d_h), h.const_data_ptr(), dtype_code(h), ptr(w),
+                                            w.defined() ? dtype_code(w) : 0, d_x.defined() ? d_x.mutable_data_ptr() : nullptr,
+                                            d_w.defined() ? d_w.mutable_data_ptr() : nullptr, M, D, eps,
+                                            bytes > 0 ? ws.mutable_data_ptr() : nullptr, bytes, stream_of(dev));
+            TORCH_CHECK(rc == 0, "cr_rms_norm_grad failed, hipError=", rc);
+        }
+        auto grads = once({d_x, d_w});
+        return {need_x ? grads[0] : at::Tensor(), grads[1], need_r ? grads[0] : at::Tensor(), at::Tensor()};
+    }
+};
+
+std::optional<at::Tensor> some(const at::Tensor& t) { return t.defined() ? std::optional<at::Tensor>(t) : std::nullopt; }
+
+// rms_norm(x, weight, residual, eps) -> y, or (y, h)
+PyObject* rms_norm(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Norm o;
+    if (n != 4 || !o.take(a[0], a[1], a[2], a[3])) Py_RETURN_NONE;
+    if (wants_grad(o.x) || wants_grad(o.weight) || wants_grad(o.residual)) {
+        const auto out = RmsNorm::apply(o.x, some(o.weight), some(o.residual), o.eps);
+        return out.size() == 1 ? THPVariable_Wrap(out[0]) : tuple_of({out[0], out[1]});
+    }
+    auto [y, h] = norm(o.x, o.weight, o.residual, o.eps);
+    return h.defined() ? tuple_of({y, h}) : THPVariable_Wrap(y);
+    END_HANDLE_TH_ERRORS
+}
+
+// rms_norm_int8(x, weight, residual, eps, groupsize, i8t) -> (codes, scales) or (codes, scales, h)
+PyObject* rms_norm_int8(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    Norm o;
+    if (n != 6 || !o.take(a[0], a[1], a[2], a[3]) || wants_grad(o.x) || wants_grad(o.weight) || wants_grad(o.residual)) Py_RETURN_NONE;
+    const int G = group_of(a[4]);
+    const bool tiled = a[5] == Py_True;
+    if (G < 0 || o.D % G != 0 || (!tiled && a[5] != Py_False) || (tiled && o.D % 64 != 0) || o.D > cr_max_quant_k()) Py_RETURN_NONE;
+    at::Tensor codes = like(o.x, {tiled ? ((int64_t)o.M + 255) / 256 * 256 : o.M, o.D}, at::kChar);
+    at::Tensor scales = like(o.x, {o.M}, at::kFloat), h;
+    if (o.residual.defined()) h = like(o.x, o.x.sizes(), o.x.scalar_type());
+    const int rc = cr_rms_norm_int8(o.x.const_data_ptr(), dtype_code(o.x), ptr(o.residual), ptr(o.weight), o.wdt,
+                                    h.defined() ? h.mutable_data_ptr() : nullptr, codes.mutable_data_ptr(),
+                                    (float*)scales.mutable_data_ptr(), o.M, o.D, G, tiled, o.eps, stream_of(o.dev));
+    TORCH_CHECK(rc == 0, "cr_rms_norm_int8 failed, hipError=", rc);
+    return h.defined() ? tuple_of({codes, scales, h}) : tuple_of({codes, scales});
+    END_HANDLE_TH_ERRORS
+}
+
+// w8a8_rows(codes, scales, sizes, f32 / bf16 / f16 code, qweight, wscales, bias, qweight_i8t): rows and weight in the I8T layout
+PyObject* w8a8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor x, xs, qw, ws, b, w;
+    c10::Device dev(c10::kCPU);
+    long dt;
+    if (n != 8 || !operand(a[0], &x, &dev, true) || !operand(a[1], &xs, &dev) || !PyTuple_CheckExact(a[2]) ||
+        PyTuple_GET_SIZE(a[2]) < 1 || !whole(a[3], &dt) || !operand(a[4], &qw, &dev) || !operand(a[5], &ws, &dev) ||
+        (a[6] != Py_None && !operand(a[6], &b, &dev)) || !operand(a[7], &w, &dev))
+        Py_RETURN_NONE;
+    std::vector<int64_t> sizes;
+    int64_t M = 1;
+    for (Py_ssize_t i = 0; i < PyTuple_GET_SIZE(a[2]); ++i) {
+        long v;
+        if (!whole(PyTuple_GET_ITEM(a[2], i), &v) || v < 1 || v > INT32_MAX) Py_RETURN_NONE;
+        sizes.push_back(v);
+        if (i + 1 < PyTuple_GET_SIZE(a[2])) M *= v;
+        if (M > INT32_MAX) Py_RETURN_NONE;
+    }
+    const int64_t K = sizes.back();
+    if (dt < 0 || dt > 2 || K % 64 != 0 || K > cr_max_quant_bf6_k() || x.scalar_type() != at::kChar || x.dim() != 2 || x.size(1) != K ||
+        x.size(0) != (M + 255) / 256 * 256 || xs.scalar_type() != at::kFloat || xs.dim() != 1 || xs.size(0) != M || qw.dim() != 2 ||
+        qw.scalar_type() != at::kChar || qw.size(1) != K || qw.size(0) < 1 || qw.size(0) > INT32_MAX)
+        Py_RETURN_NONE;
+    const int64_t N = qw.size(0);
+    if (ws.scalar_type() != at::kFloat || ws.numel() != N || wants_grad(ws) || w.scalar_type() != at::kChar || w.dim() != 2 ||
+        w.size(0) != (N + 255) / 256 * 256 || w.size(1) != K ||
+        (b.defined() && (dtype_code(b) < 0 || b.numel() != N || wants_grad(b))) || cr_convrot_w8a8_linear_i8t_split((int)M, (int)N, (int)K))
+        Py_RETURN_NONE;
+    sizes.back() = N;
+    at::Tensor out = like(x, sizes, dt == 0 ? at::kFloat : dt == 1 ? at::kBFloat16 : at::kHalf);
+    const size_t bytes = cr_w8a8_rows_linear_workspace((int)M, (int)N, (int)K);
+    const at::Tensor work = like(x, {(int64_t)bytes}, at::kByte);
+    const int rc = cr_w8a8_rows_linear(x.const_data_ptr(), (const float*)xs.const_data_ptr(), w.const_data_ptr(), ws.const_data_ptr(),
+                                       ptr(b), b.defined() ? dtype_code(b) : 0, out.mutable_data_ptr(), dt == 2 ? kEpiF16 : (int)dt, (int)M,
+                                       (int)N, (int)K, work.mutable_data_ptr(), bytes, stream_of(dev));
+    return finish(rc, "cr_w8a8_rows_linear", std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"choose_experts", (PyCFunction)(void (*)(void))choose_experts, METH_FASTCALL, nullptr},
+    {"rms_norm", (PyCFunction)(void (*)(void))rms_norm, METH_FASTCALL, nullptr},
+    {"rms_norm_int8", (PyCFunction)(void (*)(void))rms_norm_int8, METH_FASTCALL, nullptr},
+    {"w8a8_rows", (PyCFunction)(void (*)(void))w8a8_rows, METH_FASTCALL, nullptr},
     {"mx_quantize", (PyCFunction)(void (*)(void))mx_quantize, METH_FASTCALL, nullptr},
     {"mx_dequantize", (PyCFunction)(void (*)(void))mx_dequantize, METH_FASTCALL, nullptr},
     {"mx_linear", (PyCFunction)(void (*)(void))mx_linear, METH_FASTCALL, nullptr},

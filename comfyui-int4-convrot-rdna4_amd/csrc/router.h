@@ -1,0 +1,34 @@
+// What the router's kernels are given (router.hip).
+#pragma once
+
+#include "common.h"
+
+namespace convrot {
+
+struct RouterArgs {
+    const void* logits;        // [T, E]
+    const float* bias;         // [E] or NULL
+    int* ids;                  // [T, k]
+    float* weights;            // [T, k]
+    long long T;
+    int E, k, groups, top_groups;
+    float scale;
+    bool sigmoid, sum2, renormalize;
+};
+
+struct RouterGradArgs {
+    const void* logits;        // [T, E]
+    const int* ids;            // [T, k]
+    const float* d_weights;    // [T, k]
+    void* d_logits;            // [T, E], in the logits' type
+    long long T;
+    int E, k;
+    float scale;
+    bool sigmoid, renormalize;
+};
+
+int router_max_experts();
+hipError_t choose_launch(const RouterArgs& a, int dt, hipStream_t st);
+hipError_t choose_grad_launch(const RouterGradArgs& a, int dt, hipStream_t st);
+
+}  // namespace convrot

@@ -10,6 +10,12 @@ same leading sizes.  A token's output is
 ``sum_j weights[j] * down_e(silu(gate_e(x)) * up_e(x))``.  The experts are frozen
 and run without a graph; the router's weights get their gradient, so a router
 can be trained over them.
+
+    block = RoutedMxfp4MoE(moe, router_weight, norm_weight, top_k=4)
+    y, h = block(x, residual)
+
+is a block's feed-forward whole: the residual's addition, the norm, the router and
+its choice in front of the experts.
 """
 from __future__ import annotations
 
@@ -56,3 +62,39 @@ class Mxfp4MoE(torch.nn.Module):
             h = torch.nn.functional.silu(gate) * up
             rows = _int4.mxfp4_expert_linear(h, self.w2, self.s2, plan, convrot_groupsize=G, sorted_rows=True)
         return _int4.combine_expert_rows(rows, weights.reshape(-1, k), plan).reshape(x.shape)
+
+
+class RoutedMxfp4MoE(torch.nn.Module):
+    """Norm, router and experts: y = moe(n, choice of n's logits), n the norm of x, or of
+    the stream h = x + residual, which is returned beside y.
+
+    ``router_weight`` [E, D] is the one parameter (its logits are taken in float32);
+    the norm's weight and the ``balance_bias`` [E] are buffers.  The other arguments
+    are choose_experts'.  As the experts are frozen, x is too."""
+
+    def __init__(self, moe: Mxfp4MoE, router_weight: torch.Tensor, norm_weight: torch.Tensor | None = None, *, top_k: int,
+                 balance_bias: torch.Tensor | None = None, scoring: str = "softmax", num_groups: int = 1,
+                 top_groups: int | None = None, group_score: str = "max", renormalize: bool = True, scale: float = 1.0,
+                 eps: float = 1e-6):
+        super().__init__()
+        D = 2 * moe.w1.shape[-1]
+        if tuple(router_weight.shape) != (moe.num_experts, D):
+            raise ValueError(f"router_weight of shape {tuple(router_weight.shape)} does not fit {moe.num_experts} experts of {D}")
+        self.moe = moe
+        self.router_weight = torch.nn.Parameter(router_weight.detach())
+        self.register_buffer("norm_weight", norm_weight)
+        self.register_buffer("balance_bias", balance_bias)
+        self.top_k, self.eps = top_k, eps
+        self.how = dict(scoring=scoring, num_groups=num_groups, top_groups=top_groups, group_score=group_score,
+                        renormalize=renormalize, scale=scale)
+
+    def forward(self, x: torch.Tensor, residual: torch.Tensor | None = None):
+        if torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in (x, residual)):
+            raise RuntimeError("the experts are frozen: gradients reach the router's weights only; pass x.detach()")
+        with torch.no_grad():
+            n = _int4.rms_norm(x, self.norm_weight, residual, self.eps)
+        n, h = (n, None) if residual is None else n
+        logits = torch.nn.functional.linear(n.to(torch.float32), self.router_weight.to(torch.float32))
+        ids, weights = _int4.choose_experts(logits, self.top_k, self.balance_bias, **self.how)
+        y = self.moe(n, ids, weights)
+        return y if residual is None else (y, h)

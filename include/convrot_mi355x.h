@@ -473,6 +473,49 @@ int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k
                            const void* W, const void* wscales, const void* bias, int bias_dtype, void* out, int R,
                            int N, int K, int G, void* workspace, size_t workspace_bytes, void* stream);
 
+/*
+ * A router's choice.  No counterpart in the reference.
+ *
+ * Of token t's logits l [E] (dtype) and a bias b [E] (f32; NULL: 0): scores s = softmax(l), or 1 / (1 + exp(-l)) with
+ * `sigmoid`; choices c = s + b.  The `groups` groups of E / groups experts in order are ranked by their greatest c, or
+ * with group_sum2 by the sum of their two greatest; experts outside the top_groups greatest are left out.  ids[t, 0 .. k - 1]
+ * are the k greatest of those left, greatest first, equal ones (in 43 bits) by index; weights[t, j] = s[ids[t, j]], over their
+ * sum with `renormalize`, times `scale`.  Without a bias the order is the logits'.  An expert whose logit or bias is -inf is
+ * not available; a slot that finds none has id -1 and weight 0.  A NaN logit ranks first, and makes the weights NaN that
+ * depend on it.
+ * cr_choose_experts_grad: d_logits [T, E] (dtype) from d_weights [T, k]; ids outside [0, E) add nothing.
+ * E <= cr_max_experts(), groups divides E, k <= E / groups * top_groups, scale finite.
+ */
+int cr_choose_experts(const void* logits, int dtype, const float* bias, int* ids, float* weights, int T, int E, int k, int sigmoid,
+                      int groups, int top_groups, int group_sum2, int renormalize, float scale, void* stream);
+int cr_choose_experts_grad(const void* logits, int dtype, const int* ids, const float* d_weights, void* d_logits, int T, int E, int k,
+                           int sigmoid, int renormalize, float scale, void* stream);
+
+/*
+ * Root-mean-square norm of rows [M, D].  No counterpart in the reference.
+ *
+ * h = dtype(x + residual) (residual NULL: h is x, and not written); y = dtype(h w / sqrt(mean(h^2) + eps)), w [D] of
+ * weight_dtype (NULL: 1).  D <= cr_max_norm_width().
+ * cr_rms_norm_grad: d_x of x, and of the residual, from d_y and the sum's own gradient d_h (NULL: 0); d_weight [D] in
+ *   weight_dtype; either may be NULL.  workspace: >= cr_rms_norm_grad_workspace(M, D) bytes where d_weight is asked for.
+ * cr_rms_norm_int8: z = H_G(h w) / sqrt(mean(h^2) + eps), scales[m] = f32(max(max|z|, 1e-10) / 127), codes the nearest of
+ *   z / scale, ties to even; [M, D] int8, or with `tiled` in the I8T layout (D % 64 == 0; padding rows zero).  A row that is
+ *   not finite gets scale NaN and codes 0.
+ * cr_w8a8_rows_linear: the W8A8 product of such I8T rows: out = epilogue(X W^T) as cr_convrot_w8a8_linear_i8t's;
+ *   workspace: >= cr_w8a8_rows_linear_workspace(M, N, K) bytes, the first 2048 zero before its first use.
+ */
+int cr_max_norm_width(void);
+int cr_rms_norm(const void* x, int dtype, const void* residual, const void* weight, int weight_dtype, void* h, void* y, int M, int D,
+                double eps, void* stream);
+size_t cr_rms_norm_grad_workspace(int M, int D);
+int cr_rms_norm_grad(const void* d_y, const void* d_h, const void* h, int dtype, const void* weight, int weight_dtype, void* d_x,
+                     void* d_weight, int M, int D, double eps, void* workspace, size_t workspace_bytes, void* stream);
+int cr_rms_norm_int8(const void* x, int dtype, const void* residual, const void* weight, int weight_dtype, void* h, void* codes,
+                     float* scales, int M, int D, int G, int tiled, double eps, void* stream);
+size_t cr_w8a8_rows_linear_workspace(int M, int N, int K);
+int cr_w8a8_rows_linear(const void* X8, const float* xscale, const void* W8, const void* wscale, const void* bias, int bias_dtype,
+                        void* out, int epilogue, int M, int N, int K, void* workspace, size_t workspace_bytes, void* stream);
+
 /* CR_ABI_VERSION of the header this library was built with. */
 int cr_abi_version(void);
 
