@@ -79,7 +79,7 @@ def choose_experts(logits: torch.Tensor, top_k: int, balance_bias: torch.Tensor 
 
     An expert whose logit (or bias) is -inf is not available.  A slot for which no
     expert is left has id -1 and weight 0, which the routing takes for an unused
-    slot.  A NaN logit ranks first, and every weight that depends on it is NaN.
+    slot.  A NaN ranks with +inf, and every weight that depends on it is NaN.
 
     Differentiable in the logits, for a given choice; ids and the bias have no gradient."""
     if logits.is_cuda and scoring in _SCORING and group_score in _GROUP_SCORES:

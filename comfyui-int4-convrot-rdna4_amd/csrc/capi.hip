@@ -732,11 +732,11 @@ API int cr_choose_experts(const void* logits, int dtype, const float* bias, int*
     if (T == 0) return 0;
     convrot::RouterArgs a{};
     a.logits = logits; a.bias = bias; a.ids = ids; a.weights = weights;
-    a.T = T; a.E = E; a.k = k;
+    a.dt = dtype; a.T = T; a.E = E; a.k = k;
     a.groups = top_groups == groups ? 1 : groups;                      // all groups stay: none to rank
     a.top_groups = top_groups;
     a.scale = scale; a.sigmoid = sigmoid != 0; a.sum2 = group_sum2 != 0; a.renormalize = renormalize != 0;
-    return (int)convrot::choose_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+    return (int)convrot::choose_launch(a, reinterpret_cast<hipStream_t>(stream));
 }
 
 API int cr_choose_experts_grad(const void* logits, int dtype, const int* ids, const float* d_weights, void* d_logits, int T, int E,
@@ -745,8 +745,8 @@ API int cr_choose_experts_grad(const void* logits, int dtype, const int* ids, co
     if (T == 0) return 0;
     convrot::RouterGradArgs a{};
     a.logits = logits; a.ids = ids; a.d_weights = d_weights; a.d_logits = d_logits;
-    a.T = T; a.E = E; a.k = k; a.scale = scale; a.sigmoid = sigmoid != 0; a.renormalize = renormalize != 0;
-    return (int)convrot::choose_grad_launch(a, dtype, reinterpret_cast<hipStream_t>(stream));
+    a.dt = dtype; a.T = T; a.E = E; a.k = k; a.scale = scale; a.sigmoid = sigmoid != 0; a.renormalize = renormalize != 0;
+    return (int)convrot::choose_grad_launch(a, reinterpret_cast<hipStream_t>(stream));
 }
 
 static int norm_ok(int dtype, int weight_dtype, int M, int D, double eps) {

@@ -17,17 +17,54 @@ __device__ __forceinline__ double dpp(double v) {
     return __longlong_as_double((long long)((uint64_t)hi << 32 | lo));
 }
 
-// op(v, v of the lanes that share this lane's part of L lanes)
-template <int L, typename T, typename Op>
+// v of the lanes 0 .. 15 and 16 .. 31 of each half of a wave (HALF 16), or of a wave's first and second half (HALF 32),
+// the first's in both and the second's in both
+template <int HALF>
+__device__ __forceinline__ void halves(uint32_t v, uint32_t& first, uint32_t& second) {
+    static_assert(HALF == 16 || HALF == 32, "rows or halves of a wave");
+    const auto r = HALF == 16 ? __builtin_amdgcn_permlane16_swap(v, v, false, false) : __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    first = r[0];
+    second = r[1];
+}
+template <int HALF>
+__device__ __forceinline__ void halves(float v, float& first, float& second) {
+    uint32_t a, b;
+    halves<HALF>(__float_as_uint(v), a, b);
+    first = __uint_as_float(a);
+    second = __uint_as_float(b);
+}
+template <int HALF>
+__device__ __forceinline__ void halves(double v, double& first, double& second) {
+    const uint64_t u = (uint64_t)__double_as_longlong(v);
+    uint32_t al, ah, bl, bh;
+    halves<HALF>((uint32_t)u, al, bl);
+    halves<HALF>((uint32_t)(u >> 32), ah, bh);
+    first = __longlong_as_double((long long)((uint64_t)ah << 32 | al));
+    second = __longlong_as_double((long long)((uint64_t)bh << 32 | bl));
+}
+
+// v of this lane's part of D lanes and of the part beside it, where each part's lanes share one value: `a` and `b` are
+// the same two values in both parts, in either order.
+template <int D, typename T>
+__device__ __forceinline__ void neighbours(T v, T& a, T& b) {
+    static_assert(D == 1 || D == 2 || D == 4 || D == 8 || D == 16 || D == 32, "parts of a wave");
+    a = v;
+    if constexpr (D == 1) b = dpp<DPP_XOR1>(v);
+    else if constexpr (D == 2) b = dpp<DPP_XOR2>(v);
+    else if constexpr (D == 4) b = dpp<DPP_HALF_MIRROR>(v);          // the other quad of eight
+    else if constexpr (D == 8) b = dpp<DPP_ROR8>(v);                 // the other eight of sixteen
+    else halves<D>(v, a, b);
+}
+
+// op over the L lanes of this lane's part; op is symmetric
+template <int L, int D = 1, typename T, typename Op>
 __device__ __forceinline__ T all_lanes(T v, Op op) {
-    static_assert(L >= 1 && L <= 64 && (L & (L - 1)) == 0, "parts of a wave");
-    if constexpr (L >= 2) v = op(v, dpp<DPP_XOR1>(v));
-    if constexpr (L >= 4) v = op(v, dpp<DPP_XOR2>(v));
-    if constexpr (L >= 8) v = op(v, dpp<DPP_HALF_MIRROR>(v));    // quads are uniform: the other quad of eight
-    if constexpr (L >= 16) v = op(v, dpp<DPP_ROR8>(v));          // the other eight of sixteen
-    if constexpr (L >= 32) v = op(v, __shfl_xor(v, 16));
-    if constexpr (L >= 64) v = op(v, __shfl_xor(v, 32));
-    return v;
+    if constexpr (D >= L) return v;
+    else {
+        T a, b;
+        neighbours<D>(v, a, b);
+        return all_lanes<L, 2 * D>(op(a, b), op);
+    }
 }
 
 template <int L, typename T>

@@ -11,7 +11,7 @@ struct RouterArgs {
     int* ids;                  // [T, k]
     float* weights;            // [T, k]
     long long T;
-    int E, k, groups, top_groups;
+    int dt, E, k, groups, top_groups;      // dt: the logits'
     float scale;
     bool sigmoid, sum2, renormalize;
 };
@@ -22,13 +22,13 @@ struct RouterGradArgs {
     const float* d_weights;    // [T, k]
     void* d_logits;            // [T, E], in the logits' type
     long long T;
-    int E, k;
+    int dt, E, k;
     float scale;
     bool sigmoid, renormalize;
 };
 
 int router_max_experts();
-hipError_t choose_launch(const RouterArgs& a, int dt, hipStream_t st);
-hipError_t choose_grad_launch(const RouterGradArgs& a, int dt, hipStream_t st);
+hipError_t choose_launch(const RouterArgs& a, hipStream_t st);
+hipError_t choose_grad_launch(const RouterGradArgs& a, hipStream_t st);
 
 }  // namespace convrot

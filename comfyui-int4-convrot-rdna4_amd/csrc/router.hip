@@ -10,7 +10,12 @@
 // The order is decided in 64 bits: c is rounded to 43 bits, far below what 32-bit scores could tell apart, and equal
 // ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them.  A key
 // holds both: the low ten bits of a double give way to the index (1023 - e, or e where c is negative, so that of
-// equal values the lowest index is the greatest key); keys differ, and the maximum of doubles is one instruction.
+// equal values the lowest index is the greatest key).  Keys are finite and differ, and the greater and the smaller of
+// two are one instruction each, where a pair of value and index would take five.
+//
+// The work is a token's own and small, so what counts is the length of its chain and the instructions of all tokens:
+// L lanes share a token, each with P experts in registers; a lane sorts its keys down to the k greatest, and two
+// lanes' sorted lists merge to one in log2(2 k) steps, log2(L) times over.
 
 #include "lanes.h"
 #include "router.h"
@@ -18,74 +23,124 @@
 namespace convrot {
 
 constexpr int RT_MAX_E = 1024;                         // indexes in ten bits
-constexpr double RT_NONE = -__builtin_inf();           // the key of an expert that is not available
+constexpr double RT_NONE = -0x1.fffffffffffffp1023;    // the choice and the key of an expert that is not available
+constexpr double RT_MOST = 0x1p1022;                   // the choice of one that is +inf or NaN
 constexpr int RT_THREADS = 256;
+constexpr long long RT_FEW = 1 << 19;                  // logits of a call that takes 4 experts a lane
 
-__device__ __forceinline__ double key_max(double a, double b) {      // keys are no NaN: without canonicalizing them
+// The greater and the smaller of two keys; fmax would first canonicalize each operand.  The compiler does not know what
+// the instruction writes: `settle` keeps the two wait states between it and a move across lanes.
+__device__ __forceinline__ double key_max(double a, double b) {
     double r;
     asm("v_max_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
     return r;
 }
+__device__ __forceinline__ double key_min(double a, double b) {
+    double r;
+    asm("v_min_f64 %0, %1, %2" : "=v"(r) : "v"(a), "v"(b));
+    return r;
+}
+template <int N>
+__device__ __forceinline__ void settle(double (&k)[N]) {
+    if constexpr (N == 1) asm volatile("s_nop 1" : "+v"(k[0]));
+    else if constexpr (N == 4) asm volatile("s_nop 1" : "+v"(k[0]), "+v"(k[1]), "+v"(k[2]), "+v"(k[3]));
+    else {
+        static_assert(N == 8, "lists of 1, 4 or 8");
+        asm volatile("s_nop 1" : "+v"(k[0]), "+v"(k[1]), "+v"(k[2]), "+v"(k[3]), "+v"(k[4]), "+v"(k[5]), "+v"(k[6]), "+v"(k[7]));
+    }
+}
 
-__device__ __forceinline__ bool ranks_above(double a, double b) { return a > b || (a != a && b == b); }    // a NaN above all
-
-// The key of choice `c` of number e: NaN above +inf above every other value, -inf RT_NONE.
+// The key of choice c (RT_NONE, or above -2^1000 and at most RT_MOST) of number e
 __device__ __forceinline__ double key_of(double c, int e) {
-    if (c == RT_NONE) return RT_NONE;
-    uint64_t u = (uint64_t)__double_as_longlong(c + 0.0);             // -0 counts as 0
-    if (c != c) u = 0x7fe0000000000000ull;
-    else if (c == __builtin_inf()) u = 0x7fd0000000000000ull;
-    const uint64_t low = (u >> 63) ? (uint64_t)e : (uint64_t)(1023 - e);
-    return __longlong_as_double((long long)((u & ~1023ull) | low));
+    const uint64_t u = (uint64_t)__double_as_longlong(c + 0.0);       // -0 counts as 0
+    const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u;
+    const uint32_t low = (uint32_t)(1023 - e) ^ ((uint32_t)((int)hi >> 31) & 1023u);
+    return __longlong_as_double((long long)((uint64_t)hi << 32 | ((lo & ~1023u) | low)));
 }
+__device__ __forceinline__ bool is_none(double key) { return key < -0x1p1000; }
 
-// The number that a key was made of; -1 of RT_NONE
+// The number that a key was made of; -1 where it is of no expert
 __device__ __forceinline__ int key_number(double key) {
-    if (key == RT_NONE) return -1;
     const uint64_t u = (uint64_t)__double_as_longlong(key);
-    const int low = (int)(u & 1023);
-    return (u >> 63) ? low : 1023 - low;
+    const int low = (int)(((uint32_t)u ^ (uint32_t)((int)(u >> 32) >> 31)) & 1023u);
+    return is_none(key) ? -1 : 1023 - low;
 }
 
-template <int DT>
-__device__ __forceinline__ float logit_at(const void* p, size_t i) {
-    if constexpr (DT == DT_F32) return reinterpret_cast<const float*>(p)[i];
+// exp(x) to 2^-46 of its value, x at most 700; below -700 as at -700: x = n ln 2 + r, a polynomial of exp(r) on
+// |r| <= ln(2) / 2 (its series, whose next term is below 2^-47).  Seventeen instructions where the library's takes
+// forty; the choice keeps 43 bits.
+__device__ __forceinline__ double choice_exp(double x) {
+    x = x < -700.0 ? -700.0 : x;
+    const double t = __builtin_fma(x, 1.4426950408889634, 0x1.8p52);
+    const double r = __builtin_fma(t - 0x1.8p52, -0.6931471805599453, x);
+    double p = 1.0 / 39916800;
+    p = __builtin_fma(p, r, 1.0 / 3628800);
+    p = __builtin_fma(p, r, 1.0 / 362880);
+    p = __builtin_fma(p, r, 1.0 / 40320);
+    p = __builtin_fma(p, r, 1.0 / 5040);
+    p = __builtin_fma(p, r, 1.0 / 720);
+    p = __builtin_fma(p, r, 1.0 / 120);
+    p = __builtin_fma(p, r, 1.0 / 24);
+    p = __builtin_fma(p, r, 1.0 / 6);
+    p = __builtin_fma(p, r, 0.5);
+    p = __builtin_fma(p, r, 1.0);
+    p = __builtin_fma(p, r, 1.0);
+    return __builtin_amdgcn_ldexp(p, (int)(uint32_t)(uint64_t)__double_as_longlong(t));
+}
+
+// 1 / d of a finite d >= 1: the instruction's approximation and two Newton steps
+__device__ __forceinline__ double choice_rcp(double d) {
+    double r = __builtin_amdgcn_rcp(d);
+    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+}
+
+__device__ __forceinline__ float logit_at(const void* p, int dt, size_t i) {
+    if (dt == DT_F32) return reinterpret_cast<const float*>(p)[i];
     const uint32_t h = reinterpret_cast<const uint16_t*>(p)[i];
-    return DT == DT_BF16 ? __uint_as_float(h << 16) : f16bits_to_f32(h);
+    return dt == DT_BF16 ? __uint_as_float(h << 16) : f16bits_to_f32(h);
 }
 
-// Experts e0 .. e0 + P - 1 of a row (-inf past the last).  VEC: E is a multiple of P, so they are there or not together
-// and aligned to their size.
-template <int DT, int P, bool VEC>
-__device__ __forceinline__ void load_logits(const void* row, int e0, int E, float (&l)[P]) {
-    if constexpr (!VEC) {
+// Experts e0 .. e0 + P - 1 of a row, -inf past the last.  Rows of a multiple of 4 are read 4 values at a time, of 16 bytes or
+// 8; others one by one.
+template <int P>
+__device__ __forceinline__ void load_logits(const void* row, int dt, int e0, int E, float (&l)[P]) {
+    if (E % 4 != 0) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) l[p] = e0 + p < E ? logit_at<DT>(row, e0 + p) : -__builtin_inff();
+        for (int p = 0; p < P; ++p) l[p] = e0 + p < E ? logit_at(row, dt, e0 + p) : -__builtin_inff();
+        return;
+    }
+    if (dt == DT_F32) {
+#pragma unroll
+        for (int p = 0; p < P; p += 4) {
+            float4 v = make_float4(-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff());
+            if (e0 + p < E) v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + e0 + p);
+            l[p] = v.x; l[p + 1] = v.y; l[p + 2] = v.z; l[p + 3] = v.w;
+        }
+        return;
+    }
+    const uint32_t none = dt == DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;   // -inf twice
+    uint2 v[P / 4];
+    if (P % 8 == 0 && E % 8 == 0) {
+#pragma unroll
+        for (int p = 0; p < P; p += 8) {
+            uint4 q = make_uint4(none, none, none, none);
+            if (e0 + p < E) q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + e0 + p);
+            v[p / 4] = make_uint2(q.x, q.y);
+            v[(p / 4 + 1) % (P / 4)] = make_uint2(q.z, q.w);
+        }
     } else {
-        constexpr int WORDS = P * (DT == DT_F32 ? 4 : 2) / 4;
-        uint32_t w[WORDS];
-        const bool there = e0 < E;
-        if constexpr (WORDS % 4 == 0) {
-            const uint4* q = reinterpret_cast<const uint4*>(reinterpret_cast<const uint8_t*>(row) + (size_t)e0 * (DT == DT_F32 ? 4 : 2));
 #pragma unroll
-            for (int i = 0; i < WORDS / 4; ++i) {
-                const uint4 v = there ? q[i] : make_uint4(0u, 0u, 0u, 0u);
-                w[4 * i] = v.x; w[4 * i + 1] = v.y; w[4 * i + 2] = v.z; w[4 * i + 3] = v.w;
-            }
-        } else {
-            static_assert(WORDS == 2, "four 16-bit values");
-            const uint2 v = there ? *reinterpret_cast<const uint2*>(reinterpret_cast<const uint8_t*>(row) + (size_t)e0 * 2)
-                                  : make_uint2(0u, 0u);
-            w[0] = v.x; w[1] = v.y;
+        for (int p = 0; p < P; p += 4) {
+            v[p / 4] = make_uint2(none, none);
+            if (e0 + p < E) v[p / 4] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(row) + e0 + p);
         }
+    }
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            float f;
-            if constexpr (DT == DT_F32) f = __uint_as_float(w[p]);
-            else if constexpr (DT == DT_BF16) f = (p & 1) ? bf16hi_to_f32(w[p >> 1]) : bf16lo_to_f32(w[p >> 1]);
-            else f = f16bits_to_f32((p & 1) ? w[p >> 1] >> 16 : w[p >> 1]);
-            l[p] = there ? f : -__builtin_inff();
-        }
+    for (int p = 0; p < P; p += 2) {
+        const uint32_t w = (p & 2) ? v[p / 4].y : v[p / 4].x;
+        l[p] = dt == DT_BF16 ? bf16lo_to_f32(w) : f16bits_to_f32(w);
+        l[p + 1] = dt == DT_BF16 ? bf16hi_to_f32(w) : f16bits_to_f32(w >> 16);
     }
 }
 
@@ -96,104 +151,270 @@ __device__ __forceinline__ float score_over(float l, float m, bool sigmoid) {
 }
 __device__ __forceinline__ float sigmoid_of(float l) { return 1.0f / (1.0f + expf(-l)); }
 
-// L lanes take a token, P experts each, in order.
-template <int DT, int L, int P, bool VEC, bool GROUPS>
+// v[A .. A + N - 1], a list that rises and then falls or the other way round, sorted downwards
+template <int A, int N, int K>
+__device__ __forceinline__ void sort_bitonic(double (&v)[K]) {
+    if constexpr (N > 1) {
+#pragma unroll
+        for (int i = A; i < A + N / 2; ++i) {
+            const double a = v[i], b = v[i + N / 2];
+            v[i] = key_max(a, b);
+            v[i + N / 2] = key_min(a, b);
+        }
+        sort_bitonic<A, N / 2>(v);
+        sort_bitonic<A + N / 2, N / 2>(v);
+    }
+}
+
+// v[A .. A + N - 1] sorted downwards: halves, the second turned round, merged
+template <int A, int N, int K>
+__device__ __forceinline__ void sort_down(double (&v)[K]) {
+    if constexpr (N > 1) {
+        sort_down<A, N / 2>(v);
+        sort_down<A + N / 2, N / 2>(v);
+#pragma unroll
+        for (int i = 0; i < N / 2; ++i) {
+            const double a = v[A + i], b = v[A + N - 1 - i];
+            v[A + i] = key_max(a, b);
+            v[A + N - 1 - i] = key_min(a, b);
+        }
+        sort_bitonic<A, N / 2>(v);
+        sort_bitonic<A + N / 2, N / 2>(v);
+    }
+}
+
+// The K greatest of a lane's P keys, downwards
+template <int K, int P>
+__device__ __forceinline__ void greatest(const double (&key)[P], double (&top)[K]) {
+    if constexpr (P <= K) {
+#pragma unroll
+        for (int i = 0; i < K; ++i) top[i] = i < P ? key[i < P ? i : 0] : RT_NONE;
+        sort_down<0, P>(top);
+    } else {
+        double part[K];
+#pragma unroll
+        for (int i = 0; i < K; ++i) top[i] = key[i];
+        sort_down<0, K>(top);
+#pragma unroll
+        for (int q = K; q < P; q += K) {
+#pragma unroll
+            for (int i = 0; i < K; ++i) part[i] = key[q + i];
+            sort_down<0, K>(part);
+#pragma unroll
+            for (int i = 0; i < K; ++i) top[i] = key_max(top[i], part[K - 1 - i]);
+            sort_bitonic<0, K>(top);
+        }
+    }
+}
+
+// The lists of a token's L lanes made one, which each of them then has
+template <int L, int D, int K>
+__device__ __forceinline__ void merge_lanes(double (&top)[K]) {
+    if constexpr (D < L) {
+        double a[K], b[K];
+        settle(top);
+#pragma unroll
+        for (int i = 0; i < K; ++i) neighbours<D>(top[i], a[i], b[i]);
+#pragma unroll
+        for (int i = 0; i < K; ++i) top[i] = key_max(a[i], b[K - 1 - i]);
+        sort_bitonic<0, K>(top);
+        merge_lanes<L, 2 * D>(top);
+    }
+}
+
+// The greatest key of a token's L lanes
+template <int L>
+__device__ __forceinline__ double greatest_lanes(double key) {
+    return all_lanes<L>(key, [](double a, double b) {
+        double r[1] = {key_max(a, b)};
+        settle(r);
+        return r[0];
+    });
+}
+
+// The two greatest choices of a group that `lanes` lanes share, beside each other
+template <int L, int D = 1>
+__device__ __forceinline__ void two_lanes(double& one, double& two, int lanes) {
+    if constexpr (D < L) {
+        if (D >= lanes) return;                                       // the same for every lane
+        double v[1] = {one}, w[1] = {two}, a1, b1, a2, b2;
+        settle(v);
+        settle(w);
+        neighbours<D>(v[0], a1, b1);
+        neighbours<D>(w[0], a2, b2);
+        one = key_max(a1, b1);
+        two = key_max(key_min(a1, b1), key_max(a2, b2));
+        two_lanes<L, 2 * D>(one, two, lanes);
+    }
+}
+
+// c[p] of experts outside the top_groups greatest groups -> RT_NONE.  `table`: L P doubles of LDS, the token's own.
+template <int L, int P>
+__device__ __forceinline__ void keep_groups(double (&c)[P], const RouterArgs& a, int sub, double* table) {
+    const int size = a.E / a.groups, e0 = sub * P;
+    const int lanes = size / P;
+    const auto score = [&](double one, double two) {
+        return key_min(a.sum2 && !is_none(two) ? one + two : one, RT_MOST);
+    };
+    const auto above = [&](double mine) {                             // groups ranked above
+        int n = 0;
+#pragma unroll 4
+        for (int g = 0; g < a.groups; ++g) n += table[g] > mine ? 1 : 0;
+        return n;
+    };
+    if (size % P == 0 && (lanes & (lanes - 1)) == 0) {                // whole lanes, a power of two of them
+        double one = RT_NONE, two = RT_NONE;
+#pragma unroll
+        for (int p = 0; p < P; ++p) {
+            two = key_max(two, key_min(one, c[p]));
+            one = key_max(one, c[p]);
+        }
+        two_lanes<L>(one, two, lanes);
+        const int g = sub / lanes;
+        const double mine = key_of(score(one, two), g);
+        if (g < a.groups && sub % lanes == 0) table[g] = mine;
+        wave_sync();
+        const bool out = above(mine) >= a.top_groups;
+#pragma unroll
+        for (int p = 0; p < P; ++p) c[p] = out ? RT_NONE : c[p];
+        return;
+    }
+    // any size: a lane reads whole groups; the group's key, and then RT_NONE or not, in the place of its first expert
+#pragma unroll
+    for (int p = 0; p < P; ++p) table[e0 + p] = c[p];
+    wave_sync();
+    double mine[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) {
+        const int g = q * L + sub;
+        double one = RT_NONE, two = RT_NONE;
+        if (g < a.groups) {
+            for (int i = 0; i < size; ++i) {
+                const double v = table[g * size + i];
+                two = key_max(two, key_min(one, v));
+                one = key_max(one, v);
+            }
+        }
+        mine[q] = key_of(score(one, two), g & 1023);
+    }
+    wave_sync();
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+        if (q * L + sub < a.groups) table[q * L + sub] = mine[q];
+    wave_sync();
+    bool out[P];
+#pragma unroll
+    for (int q = 0; q < P; ++q) out[q] = q * L + sub < a.groups && above(mine[q]) >= a.top_groups;
+    wave_sync();
+#pragma unroll
+    for (int q = 0; q < P; ++q)
+        if (q * L + sub < a.groups) table[q * L + sub] = out[q] ? RT_NONE : 0.0;
+    wave_sync();
+#pragma unroll
+    for (int p = 0; p < P; ++p)
+        if (e0 + p < a.E && is_none(table[(e0 + p) / size])) c[p] = RT_NONE;
+}
+
+// L lanes take a token, P experts each, in order.  K: the longest list that is sorted, at least k; 0: any k, one expert
+// after the other.
+template <int L, int P, int K, bool GROUPS>
 __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsigned first) {
-    __shared__ int chosen_lds[RT_THREADS * P];                        // k <= E <= L P of each token
-    __shared__ double choice_lds[GROUPS ? RT_THREADS * P : 1];
+    __shared__ int chosen_lds[K == 0 ? RT_THREADS * P : 1];           // k <= E <= L P of each token
+    __shared__ double table_lds[GROUPS ? RT_THREADS * P : 1];
     const int tid = threadIdx.x, sub = tid % L, e0 = sub * P;
     const long long t = (first + (long long)blockIdx.x) * (RT_THREADS / L) + tid / L;
     if (t >= a.T) return;                                             // a token's lanes are of one wave
-    int* chosen = chosen_lds + tid / L * (L * P);
-    const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + (size_t)t * a.E * (DT == DT_F32 ? 4 : 2);
-    float l[P];
-    load_logits<DT, P, VEC>(row, e0, a.E, l);
-    float m = l[0];
-#pragma unroll
-    for (int p = 1; p < P; ++p) m = fmaxf(m, l[p]);
-    m = max_lanes<L>(m);
-
-    double key[P];
-    bool spoilt = false;                                              // a NaN somewhere: no score is a number
+    const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + (size_t)t * a.E * (a.dt == DT_F32 ? 4 : 2);
     const bool by_score = a.bias != nullptr || (GROUPS && a.sum2);
-    if (by_score) {
-        double s[P], sum = 0.0;
+    float l[P], b[P];
+    load_logits(row, a.dt, e0, a.E, l);
+    if (a.bias != nullptr) load_logits(a.bias, DT_F32, e0, a.E, b);
+    float m = l[0];
+    if (!a.sigmoid) {
 #pragma unroll
-        for (int p = 0; p < P; ++p) {
-            s[p] = a.sigmoid ? 1.0 / (1.0 + exp(-(double)l[p])) : exp((double)l[p] - (double)m);
-            sum += l[p] == -__builtin_inff() ? 0.0 : s[p];
-        }
-        if (!a.sigmoid) {
+        for (int p = 1; p < P; ++p) m = fmaxf(m, l[p]);
+        m = max_lanes<L>(m);
+    }
+    double c[P];
+    bool spoilt = false;                                              // softmax with a NaN: no score is a number
+    if (by_score) {
+        if (a.sigmoid) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                const float x = l[p] < -700.0f ? 700.0f : -l[p];
+                c[p] = choice_rcp(1.0 + choice_exp((double)x));
+            }
+        } else {
+            double sum = 0.0;
+#pragma unroll
+            for (int p = 0; p < P; ++p) {
+                c[p] = choice_exp((double)l[p] - (double)m);
+                sum += l[p] == -__builtin_inff() ? 0.0 : c[p];
+            }
             sum = sum_lanes<L>(sum);
             spoilt = sum != sum;
             const double inv = 1.0 / sum;
 #pragma unroll
-            for (int p = 0; p < P; ++p) s[p] *= inv;
+            for (int p = 0; p < P; ++p) c[p] *= inv;
         }
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const bool out = e0 + p >= a.E || l[p] == -__builtin_inff();
-            const float b = a.bias != nullptr && e0 + p < a.E ? a.bias[e0 + p] : 0.0f;
-            key[p] = out ? RT_NONE : s[p] + (double)b;
+            const bool out = l[p] == -__builtin_inff() || (a.bias != nullptr && b[p] == -__builtin_inff());
+            c[p] = out ? RT_NONE : key_min(a.bias != nullptr ? c[p] + (double)b[p] : c[p], RT_MOST);
         }
     } else {
 #pragma unroll
-        for (int p = 0; p < P; ++p) key[p] = e0 + p < a.E ? (double)l[p] : RT_NONE;
+        for (int p = 0; p < P; ++p) c[p] = l[p] == -__builtin_inff() ? RT_NONE : key_min((double)l[p], RT_MOST);
     }
+    if constexpr (GROUPS) keep_groups<L>(c, a, sub, table_lds + tid / L * (L * P));
+#pragma unroll
+    for (int p = 0; p < P; ++p) c[p] = key_of(c[p], (e0 + p) & 1023);
 
-    if constexpr (GROUPS) {
-        double* choice = choice_lds + tid / L * (L * P);
+    // experts j = sub, sub + L, ...: from the sorted list, which every lane has, or from LDS
+    constexpr int MINE = K == 0 ? 1 : (K + L - 1) / L;
+    double mine[MINE];
+    int* chosen = chosen_lds + (K == 0 ? tid / L * (L * P) : 0);
+    if constexpr (K > 0) {
+        double top[K];
+        greatest<K>(c, top);
+        merge_lanes<L, 1>(top);
 #pragma unroll
-        for (int p = 0; p < P; ++p)
-            if (e0 + p < a.E) choice[e0 + p] = key[p];
-        wave_sync();
-        const int size = a.E / a.groups;
-        for (int g = sub; g < a.groups; g += L) {
-            double one = RT_NONE, two = RT_NONE;
-            for (int i = 0; i < size; ++i) {
-                const double c = choice[g * size + i];
-                const bool above = ranks_above(c, one);
-                two = above ? one : ranks_above(c, two) ? c : two;
-                one = above ? c : one;
-            }
-            choice[g * size] = key_of(a.sum2 && two != RT_NONE ? one + two : one, g);
+        for (int i = 0; i < MINE; ++i) {
+            mine[i] = RT_NONE;
+#pragma unroll
+            for (int j = i * L; j < (i + 1) * L && j < K; ++j) mine[i] = sub == j - i * L ? top[j] : mine[i];
         }
-        wave_sync();
-        double gk[P];
-#pragma unroll
-        for (int p = 0; p < P; ++p) gk[p] = e0 + p < a.groups ? choice[(e0 + p) * size] : RT_NONE;
+    } else {
         double last = __builtin_inf();
-        for (int j = 0; j < a.top_groups; ++j) {
+        for (int j = 0; j < a.k; ++j) {
             double best = RT_NONE;
 #pragma unroll
-            for (int p = 0; p < P; ++p) best = key_max(best, gk[p] < last ? gk[p] : RT_NONE);
-            last = all_lanes<L>(best, key_max);
+            for (int p = 0; p < P; ++p) best = key_max(best, c[p] < last ? c[p] : RT_NONE);
+            double v[1] = {best};
+            settle(v);
+            last = greatest_lanes<L>(v[0]);
+            if (sub == 0) chosen[j] = key_number(last);
         }
-#pragma unroll
-        for (int p = 0; p < P; ++p)
-            if (e0 + p < a.E && choice[(e0 + p) / size * size] < last) key[p] = RT_NONE;
+        wave_sync();
     }
+    // f(j, its expert) for this lane's slots
+    const auto each = [&](auto f) {
+        if constexpr (K > 0) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) key[p] = key_of(key[p], e0 + p);
-    double last = __builtin_inf();
-    for (int j = 0; j < a.k; ++j) {
-        double best = RT_NONE;
-#pragma unroll
-        for (int p = 0; p < P; ++p) best = key_max(best, key[p] < last ? key[p] : RT_NONE);
-        last = all_lanes<L>(best, key_max);
-        if (sub == 0) chosen[j] = key_number(last);
-    }
-    wave_sync();
+            for (int i = 0; i < MINE; ++i)
+                if (i * L + sub < a.k) f(i * L + sub, key_number(mine[i]));
+        } else {
+            for (int j = sub; j < a.k; j += L) f(j, chosen[j]);
+        }
+    };
 
     // the weights, in 32 bits from the chosen logits
     float total = 0.0f;
     if (a.renormalize) {
         float top = -__builtin_inff();
-        for (int j = sub; j < a.k; j += L)
-            if (chosen[j] >= 0) top = fmaxf(top, logit_at<DT>(row, chosen[j]));
+        each([&](int, int e) { if (e >= 0) top = fmaxf(top, logit_at(row, a.dt, e)); });
         m = max_lanes<L>(top);
-        for (int j = sub; j < a.k; j += L)
-            if (chosen[j] >= 0) total += score_over(logit_at<DT>(row, chosen[j]), m, a.sigmoid);
+        each([&](int, int e) { if (e >= 0) total += score_over(logit_at(row, a.dt, e), m, a.sigmoid); });
         total = sum_lanes<L>(total);
     } else if (!a.sigmoid) {
 #pragma unroll
@@ -201,15 +422,46 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
         total = sum_lanes<L>(total);
     }
     if (spoilt) total = __builtin_nanf("");
-    for (int j = sub; j < a.k; j += L) {
-        const int e = chosen[j];
+    each([&](int j, int e) {
         float w = 0.0f;
         if (e >= 0) {
-            const float v = logit_at<DT>(row, e);
-            w = a.sigmoid && !a.renormalize ? sigmoid_of(v) : score_over(v, m, a.sigmoid) / total;
+            const float v = logit_at(row, a.dt, e);
+            w = (a.sigmoid && !a.renormalize ? sigmoid_of(v) : score_over(v, m, a.sigmoid) / total) * a.scale;
         }
         a.ids[t * a.k + j] = e;
-        a.weights[t * a.k + j] = e >= 0 ? w * a.scale : 0.0f;
+        a.weights[t * a.k + j] = w;
+    });
+}
+
+// Values e0 .. e0 + P - 1 of a row of E in type dt
+template <int P>
+__device__ __forceinline__ void store_row(uint8_t* row, int dt, int e0, int E, const float (&v)[P]) {
+    if (dt == DT_F32) {
+        float* out = reinterpret_cast<float*>(row) + e0;
+#pragma unroll
+        for (int p = 0; p < P; p += 4) {
+            if (E % 4 == 0) {
+                if (e0 + p < E) *reinterpret_cast<float4*>(out + p) = make_float4(v[p], v[p + 1], v[p + 2], v[p + 3]);
+            } else {
+#pragma unroll
+                for (int i = p; i < p + 4; ++i)
+                    if (e0 + i < E) out[i] = v[i];
+            }
+        }
+        return;
+    }
+    uint16_t* out = reinterpret_cast<uint16_t*>(row) + e0;
+#pragma unroll
+    for (int p = 0; p < P; p += 4) {
+        const uint32_t lo = dt == DT_BF16 ? pack_bf16x2(v[p], v[p + 1]) : pack_f16x2(v[p], v[p + 1]);
+        const uint32_t hi = dt == DT_BF16 ? pack_bf16x2(v[p + 2], v[p + 3]) : pack_f16x2(v[p + 2], v[p + 3]);
+        if (E % 4 == 0) {
+            if (e0 + p < E) *reinterpret_cast<uint2*>(out + p) = make_uint2(lo, hi);
+        } else {
+#pragma unroll
+            for (int i = 0; i < 4; ++i)
+                if (e0 + p + i < E) out[p + i] = (uint16_t)((i & 2 ? hi : lo) >> (i & 1 ? 16 : 0));
+        }
     }
 }
 
@@ -217,14 +469,14 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
 //   softmax        renormalized p_j (g_j - sum p g), else s_e ([e chosen] g_e - sum s g)
 //   sigmoid        renormalized p_j (1 - s_j) (g_j - sum p g), else s_j (1 - s_j) g_j
 // and 0 for experts that were not chosen (but for softmax as it is).  Scores are computed again from the logits.
-template <int DT, int L, int P, bool VEC>
+template <int L, int P>
 __global__ __launch_bounds__(RT_THREADS) void choose_grad_kernel(RouterGradArgs a, unsigned first) {
     __shared__ float d_lds[RT_THREADS * P];
     const int tid = threadIdx.x, sub = tid % L, e0 = sub * P;
     const long long t = (first + (long long)blockIdx.x) * (RT_THREADS / L) + tid / L;
     if (t >= a.T) return;
     float* d = d_lds + tid / L * (L * P);
-    constexpr int ES = DT == DT_F32 ? 4 : 2;
+    const int ES = a.dt == DT_F32 ? 4 : 2;
     const uint8_t* row = reinterpret_cast<const uint8_t*>(a.logits) + (size_t)t * a.E * ES;
     const int* ids = a.ids + t * a.k;
     const float* dw = a.d_weights + t * a.k;
@@ -233,7 +485,7 @@ __global__ __launch_bounds__(RT_THREADS) void choose_grad_kernel(RouterGradArgs 
     for (int p = 0; p < P; ++p) d[e0 + p] = 0.0f;
     float l[P], m = -__builtin_inff(), total = 0.0f;
     if (all) {
-        load_logits<DT, P, VEC>(row, e0, a.E, l);
+        load_logits(row, a.dt, e0, a.E, l);
 #pragma unroll
         for (int p = 0; p < P; ++p) m = fmaxf(m, l[p]);
         m = max_lanes<L>(m);
@@ -242,81 +494,83 @@ __global__ __launch_bounds__(RT_THREADS) void choose_grad_kernel(RouterGradArgs 
         total = sum_lanes<L>(total);
     } else if (a.renormalize) {
         for (int j = sub; j < a.k; j += L)
-            if ((unsigned)ids[j] < (unsigned)a.E) m = fmaxf(m, logit_at<DT>(row, ids[j]));
+            if ((unsigned)ids[j] < (unsigned)a.E) m = fmaxf(m, logit_at(row, a.dt, ids[j]));
         m = max_lanes<L>(m);
         for (int j = sub; j < a.k; j += L)
-            if ((unsigned)ids[j] < (unsigned)a.E) total += score_over(logit_at<DT>(row, ids[j]), m, a.sigmoid);
+            if ((unsigned)ids[j] < (unsigned)a.E) total += score_over(logit_at(row, a.dt, ids[j]), m, a.sigmoid);
         total = sum_lanes<L>(total);
     }
     float mean = 0.0f;
     if (all || a.renormalize) {
         for (int j = sub; j < a.k; j += L)
             if ((unsigned)ids[j] < (unsigned)a.E)
-                mean += score_over(logit_at<DT>(row, ids[j]), m, a.sigmoid) / total * (dw[j] * a.scale);
+                mean += score_over(logit_at(row, a.dt, ids[j]), m, a.sigmoid) / total * (dw[j] * a.scale);
         mean = sum_lanes<L>(mean);
     }
     wave_sync();
     for (int j = sub; j < a.k; j += L) {
         if ((unsigned)ids[j] >= (unsigned)a.E) continue;
-        const float v = logit_at<DT>(row, ids[j]), g = dw[j] * a.scale;
+        const float v = logit_at(row, a.dt, ids[j]), g = dw[j] * a.scale;
         const float s1 = a.sigmoid ? 1.0f / (1.0f + expf(v)) : 1.0f;                  // 1 - s
         const float p = a.sigmoid && !a.renormalize ? sigmoid_of(v) : score_over(v, m, a.sigmoid) / total;
         d[ids[j]] = all ? p * g : a.renormalize ? p * s1 * (g - mean) : p * s1 * g;
     }
     wave_sync();
-    uint8_t* out = reinterpret_cast<uint8_t*>(a.d_logits) + (size_t)t * a.E * ES;
+    if (all) {
 #pragma unroll
-    for (int p = 0; p < P; ++p) {
-        if (e0 + p >= a.E) break;
-        float v = d[e0 + p];
-        if (all && l[p] != -__builtin_inff()) v -= expf(l[p] - m) / total * mean;
-        if constexpr (DT == DT_F32) reinterpret_cast<float*>(out)[e0 + p] = v;
-        else reinterpret_cast<uint16_t*>(out)[e0 + p] = (uint16_t)(DT == DT_BF16 ? pack_bf16x2(v, 0.0f) : pack_f16x2(v, 0.0f));
+        for (int p = 0; p < P; ++p) d[e0 + p] -= l[p] == -__builtin_inff() ? 0.0f : expf(l[p] - m) / total * mean;
     }
+    float v[P];
+#pragma unroll
+    for (int p = 0; p < P; ++p) v[p] = d[e0 + p];
+    store_row(reinterpret_cast<uint8_t*>(a.d_logits) + (size_t)t * a.E * ES, a.dt, e0, a.E, v);
 }
 
+// f(lanes of a token, experts of a lane): 16 experts a lane, the fewest instructions a token, where the tokens fill the
+// chip so; else 4, the shortest chain.
 template <typename F>
-static hipError_t by_lanes(int dt, int E, F f) {
-    const auto lanes = [&](auto d) {
-        constexpr int DT = decltype(d)::value;
-        using std::integral_constant;
-        const auto vec = [&](auto l) {
-            return E % 16 == 0 ? f(integral_constant<int, DT>{}, l, std::true_type{}) : f(integral_constant<int, DT>{}, l, std::false_type{});
-        };
-        if (E <= 32) return vec(integral_constant<int, 2>{});
-        if (E <= 64) return vec(integral_constant<int, 4>{});
-        if (E <= 128) return vec(integral_constant<int, 8>{});
-        if (E <= 256) return vec(integral_constant<int, 16>{});
-        if (E <= 512) return vec(integral_constant<int, 32>{});
-        return vec(integral_constant<int, 64>{});
-    };
+static hipError_t by_lanes(long long T, int E, F f) {
     using std::integral_constant;
-    if (dt == DT_F32) return lanes(integral_constant<int, DT_F32>{});
-    if (dt == DT_BF16) return lanes(integral_constant<int, DT_BF16>{});
-    return lanes(integral_constant<int, DT_F16>{});
+    const integral_constant<int, 4> few{};
+    const integral_constant<int, 16> many{};
+    if (E <= 256 && T * E <= RT_FEW) {
+        if (E <= 32) return f(integral_constant<int, 8>{}, few);
+        if (E <= 64) return f(integral_constant<int, 16>{}, few);
+        if (E <= 128) return f(integral_constant<int, 32>{}, few);
+        return f(integral_constant<int, 64>{}, few);
+    }
+    if (E <= 32) return f(integral_constant<int, 2>{}, many);
+    if (E <= 64) return f(integral_constant<int, 4>{}, many);
+    if (E <= 128) return f(integral_constant<int, 8>{}, many);
+    if (E <= 256) return f(integral_constant<int, 16>{}, many);
+    if (E <= 512) return f(integral_constant<int, 32>{}, many);
+    return f(integral_constant<int, 64>{}, many);
 }
 
 int router_max_experts() { return RT_MAX_E; }
 
-hipError_t choose_launch(const RouterArgs& a, int dt, hipStream_t st) {
-    return by_lanes(dt, a.E, [&](auto d, auto l, auto v) {
-        constexpr int DT = decltype(d)::value, L = decltype(l)::value;
-        constexpr bool VEC = decltype(v)::value;
-        return launch_parts((a.T * L + RT_THREADS - 1) / RT_THREADS, RT_THREADS, [&](long long first, dim3 grid) {
-            if (a.groups > 1)
-                hipLaunchKernelGGL((choose_kernel<DT, L, 16, VEC, true>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
-            else
-                hipLaunchKernelGGL((choose_kernel<DT, L, 16, VEC, false>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
-        });
+template <int L, int P, int K>
+static hipError_t choose_go(const RouterArgs& a, hipStream_t st) {
+    return launch_parts((a.T * L + RT_THREADS - 1) / RT_THREADS, RT_THREADS, [&](long long first, dim3 grid) {
+        if (a.groups > 1) hipLaunchKernelGGL((choose_kernel<L, P, K, true>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
+        else hipLaunchKernelGGL((choose_kernel<L, P, K, false>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
     });
 }
 
-hipError_t choose_grad_launch(const RouterGradArgs& a, int dt, hipStream_t st) {
-    return by_lanes(dt, a.E, [&](auto d, auto l, auto v) {
-        constexpr int DT = decltype(d)::value, L = decltype(l)::value;
-        constexpr bool VEC = decltype(v)::value;
+hipError_t choose_launch(const RouterArgs& a, hipStream_t st) {
+    return by_lanes(a.T, a.E, [&](auto l, auto p) {
+        constexpr int L = decltype(l)::value, P = decltype(p)::value;
+        if (a.k <= 4) return choose_go<L, P, 4>(a, st);
+        if (a.k <= 8) return choose_go<L, P, 8>(a, st);
+        return choose_go<L, P, 0>(a, st);
+    });
+}
+
+hipError_t choose_grad_launch(const RouterGradArgs& a, hipStream_t st) {
+    return by_lanes(a.T, a.E, [&](auto l, auto p) {
+        constexpr int L = decltype(l)::value, P = decltype(p)::value;
         return launch_parts((a.T * L + RT_THREADS - 1) / RT_THREADS, RT_THREADS, [&](long long first, dim3 grid) {
-            hipLaunchKernelGGL((choose_grad_kernel<DT, L, 16, VEC>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
+            hipLaunchKernelGGL((choose_grad_kernel<L, P>), grid, dim3(RT_THREADS), 0, st, a, (unsigned)first);
         });
     });
 }

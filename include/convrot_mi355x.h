@@ -481,7 +481,7 @@ int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k
  * with group_sum2 by the sum of their two greatest; experts outside the top_groups greatest are left out.  ids[t, 0 .. k - 1]
  * are the k greatest of those left, greatest first, equal ones (in 43 bits) by index; weights[t, j] = s[ids[t, j]], over their
  * sum with `renormalize`, times `scale`.  Without a bias the order is the logits'.  An expert whose logit or bias is -inf is
- * not available; a slot that finds none has id -1 and weight 0.  A NaN logit ranks first, and makes the weights NaN that
+ * not available; a slot that finds none has id -1 and weight 0.  A NaN ranks with +inf, and makes the weights NaN that
  * depend on it.
  * cr_choose_experts_grad: d_logits [T, E] (dtype) from d_weights [T, k]; ids outside [0, E) add nothing.
  * E <= cr_max_experts(), groups divides E, k <= E / groups * top_groups, scale finite.
