@@ -189,6 +189,9 @@ def dequantize_convrot_w4a4_weight(
     in fp32 for anything it does not take."""
     if quant_group_size != _INT4_GROUP_SIZE:
         raise ValueError(f"int4 MMA kernel requires quant_group_size {_INT4_GROUP_SIZE}")
+    w = native.host_dequant(qdata, scales, 4, convrot_groupsize, output_dtype)
+    if w is not None:
+        return w
     if native.dequant_ok(qdata, scales, 4, convrot_groupsize, output_dtype):
         return native.convrot_dequant(qdata, scales, 4, convrot_groupsize, output_dtype)
     w = _unpack_int4_row_major(qdata).to(torch.float32)

@@ -51,6 +51,9 @@ def dequantize_convrot_w8a8_weight(
     (reference _int4/int8_eager.py:50-57).  A load-time / diagnostic helper:
     one kernel on the GPU (csrc/dequant.hip), torch ops in fp32 for anything it
     does not take."""
+    w = native.host_dequant(qdata, scales, 8, convrot_groupsize, output_dtype)
+    if w is not None:
+        return w
     if native.dequant_ok(qdata, scales, 8, convrot_groupsize, output_dtype):
         return native.convrot_dequant(qdata, scales, 8, convrot_groupsize, output_dtype)
     w = qdata.to(torch.float32) * scales.to(qdata.device, torch.float32).reshape(-1, 1)

@@ -146,7 +146,8 @@ def load_library():
 
 _host = None
 _HOST_FUNCTIONS = ("w4a4", "w8a8", "mx_quantize", "mx_dequantize", "mx_linear", "mx_expert_linear", "expert_sort",
-                   "expert_gather", "expert_combine", "choose_experts", "rms_norm", "rms_norm_int8", "w8a8_rows")
+                   "expert_gather", "expert_combine", "choose_experts", "rms_norm", "rms_norm_int8", "w8a8_rows",
+                   "dequant")
 
 
 def host_module():
@@ -701,6 +702,20 @@ def dequant_ok(q, scales, bits: int, convrot_groupsize: int, out_dtype) -> bool:
     return (out_dtype in _IN_DTYPE_CODE and convrot_groupsize in (16, 64, 256) and K > 0 and K % convrot_groupsize == 0
             and N * (K // 16) < 1 << 31 and scales.numel() == N and q.device.index == torch.cuda.current_device()
             and is_available())
+
+
+_found = False        # is_available() has said so once: devices do not change in a process
+
+
+def host_dequant(q, scales, bits: int, convrot_groupsize: int, out_dtype):
+    """convrot_dequant through the host module (12 us a call through dequant_ok and
+    ctypes, 4 here), or None for the forms it leaves."""
+    global _found
+    if torch.compiler.is_compiling() or not q.is_cuda or out_dtype not in _IN_DTYPE_CODE:
+        return None
+    _found = _found or is_available()
+    host = host_or_none() if _found else None
+    return None if host is None else host.dequant(q, scales, bits, convrot_groupsize, _IN_DTYPE_CODE[out_dtype])
 
 
 def convrot_dequant(q, scales, bits: int, convrot_groupsize: int, out_dtype):

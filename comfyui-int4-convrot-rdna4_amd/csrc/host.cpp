@@ -803,7 +803,28 @@ PyObject* w8a8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
     END_HANDLE_TH_ERRORS
 }
 
+// dequant(q, scales, bits, groupsize, dtype code): weights and rows back to the original basis
+PyObject* dequant(PyObject*, PyObject* const* a, Py_ssize_t n) {
+    HANDLE_TH_ERRORS
+    at::Tensor q, s;
+    c10::Device dev(c10::kCPU);
+    long bits, dt;
+    if (n != 5 || !operand(a[0], &q, &dev, true) || !operand(a[1], &s, &dev) || !whole(a[2], &bits) || !whole(a[4], &dt) ||
+        (bits != 4 && bits != 8) || dt < 0 || dt > 2 || q.dim() != 2 || q.scalar_type() != at::kChar || q.numel() == 0 ||
+        s.scalar_type() != at::kFloat || s.numel() != q.size(0) || wants_grad(s))
+        Py_RETURN_NONE;
+    const int G = group_of(a[3]);
+    const int64_t N = q.size(0), K = q.size(1) * (8 / bits);
+    if (G < 0 || K % G != 0 || K > INT32_MAX || N * (K / 16) >= (1LL << 31)) Py_RETURN_NONE;
+    at::Tensor out = like(q, {N, K}, dt == 0 ? at::kFloat : dt == 1 ? at::kBFloat16 : at::kHalf);
+    const int rc = cr_convrot_dequant(q.const_data_ptr(), (int)bits, s.const_data_ptr(), out.mutable_data_ptr(), (int)dt, (int)N, (int)K, G,
+                                      stream_of(dev));
+    return finish(rc, "cr_convrot_dequant", std::move(out));
+    END_HANDLE_TH_ERRORS
+}
+
 PyMethodDef methods[] = {
+    {"dequant", (PyCFunction)(void (*)(void))dequant, METH_FASTCALL, nullptr},
     {"choose_experts", (PyCFunction)(void (*)(void))choose_experts, METH_FASTCALL, nullptr},
     {"rms_norm", (PyCFunction)(void (*)(void))rms_norm, METH_FASTCALL, nullptr},
     {"rms_norm_int8", (PyCFunction)(void (*)(void))rms_norm_int8, METH_FASTCALL, nullptr},

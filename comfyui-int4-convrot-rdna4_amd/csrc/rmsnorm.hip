@@ -221,8 +221,9 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a, int waves, unsig
 // registers; a workgroup adds its teams' parts in LDS, and a second launch the workgroups', all in order.
 //
 // What a row takes of a lane's registers is kept as it lies in memory (`again` makes the compiler unpack it a second time
-// rather than hold the floats across the sums); rows of four and more pieces a lane are not fetched ahead, and read d_h
-// and the weight where they are used.
+// rather than hold the floats across the sums); rows of four and more pieces a lane are not fetched ahead, read d_h and
+// the weight where they are used, and have their part of d_weight in LDS, a slot a piece (2048 x 20000: 248 us with all of
+// it in registers that do not hold it).
 __device__ __forceinline__ void again(v4u_mx& w) { asm volatile("" : "+v"(w)); }
 
 template <int DT, int P, int L, bool RES, bool TINY>
@@ -231,13 +232,14 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
     constexpr int N = V::N;
     constexpr bool AHEAD = P <= 2;
     __shared__ double slots[2][2][16];
-    extern __shared__ float sums[];                          // [teams, D] where there is more than one
-    const Team<L> team(waves);
+    extern __shared__ __attribute__((aligned(16))) float sums[];      // [teams, D] where there is more than one; or the slots
+    Team<L> team(waves);
     const int teams = blockDim.x / team.lanes;
     const long long step = (long long)gridDim.x * teams;
     const bool ragged = a.D % N != 0;                        // the last piece shares elements
-    float w[P][N], dw[P][N] = {};
+    float w[AHEAD ? P : 1][N], dw[AHEAD ? P : 1][N] = {};
     v4u_mx h[P], g[P], d[P], hn[P], gn[P], dn[P];
+    const auto held = [&](int p) { return sums + (size_t)(p * blockDim.x + threadIdx.x) * N; };
     const auto weight = [&](int p, float (&v)[N]) {
         load_weight<N, TINY>(a.weight, a.weight_dt, V::start(p * team.lanes + team.lane, a.D), a.D, v);
     };
@@ -255,7 +257,12 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
     if (AHEAD) {
         fetch(row, hn, gn, dn);
 #pragma unroll
-        for (int p = 0; p < P; ++p) weight(p, w[p]);
+        for (int p = 0; p < P; ++p) weight(p, w[AHEAD ? p : 0]);
+    } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p)
+#pragma unroll
+            for (int j = 0; j < N; j += 4) *reinterpret_cast<float4*>(held(p) + j) = make_float4(0.0f, 0.0f, 0.0f, 0.0f);
     }
     const int trips = (int)((a.M - (long long)blockIdx.x * teams + step - 1) / step);      // of the workgroup's first team
     for (int trip = 0; trip < trips; ++trip, row += step) {
@@ -267,14 +274,17 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
                 d[p] = dn[p];
             }
             if (trip + 1 < trips) fetch(row + step, hn, gn, dn);
-        } else fetch(row, h, g, d);
+        } else {
+            asm volatile("" : "+v"(team.lane));             // addresses are made again, not kept for every piece
+            fetch(row, h, g, d);
+        }
         double ss = 0.0, gh = 0.0;
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             float hf[N], gf[N];
             if (!AHEAD) {
                 asm volatile("" ::: "memory");               // a piece's weights at a time
-                weight(p, w[p]);
+                weight(p, w[0]);
             }
             V::unpack(h[p], hf);
             V::unpack(g[p], gf);
@@ -286,7 +296,7 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 ss = __builtin_fma((double)hf[j], (double)hf[j], ss);
-                gh = __builtin_fma((double)(gf[j] * w[p][j]), (double)hf[j], gh);
+                gh = __builtin_fma((double)(gf[j] * w[AHEAD ? p : 0][j]), (double)hf[j], gh);
             }
         }
         ss = sum_lanes<L>(ss);
@@ -318,7 +328,7 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
             again(g[p]);
             if (!AHEAD) {
                 asm volatile("" ::: "memory");
-                weight(p, w[p]);
+                weight(p, w[0]);
                 if constexpr (RES) d[p] = V::raw(reinterpret_cast<const uint8_t*>(a.d_h) + at, i, a.D);
             }
             V::unpack(h[p], hf);
@@ -327,8 +337,20 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
 #pragma unroll
             for (int j = 0; j < N; ++j) {
                 const float n = __builtin_amdgcn_ldexpf(hf[j], s.n) * s.a;
-                dx[j] = __builtin_amdgcn_ldexpf((gf[j] * w[p][j] - n * mean) * s.a, s.n) + df[j];
-                dw[p][j] = __builtin_fmaf(gf[j], n, dw[p][j]);
+                dx[j] = __builtin_amdgcn_ldexpf((gf[j] * w[AHEAD ? p : 0][j] - n * mean) * s.a, s.n) + df[j];
+                if constexpr (AHEAD) dw[p][j] = __builtin_fmaf(gf[j], n, dw[p][j]);
+                else hf[j] = n;
+            }
+            if constexpr (!AHEAD) {
+#pragma unroll
+                for (int j = 0; j < N; j += 4) {
+                    float4 v = *reinterpret_cast<const float4*>(held(p) + j);
+                    v.x = __builtin_fmaf(gf[j], hf[j], v.x);
+                    v.y = __builtin_fmaf(gf[j + 1], hf[j + 1], v.y);
+                    v.z = __builtin_fmaf(gf[j + 2], hf[j + 2], v.z);
+                    v.w = __builtin_fmaf(gf[j + 3], hf[j + 3], v.w);
+                    *reinterpret_cast<float4*>(held(p) + j) = v;
+                }
             }
             if (a.d_x != nullptr) V::store_raw(reinterpret_cast<uint8_t*>(a.d_x) + at, i, a.D, V::pack(dx));
         }
@@ -342,7 +364,7 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
         if (!V::there(i, a.D)) continue;
 #pragma unroll
         for (int j = 0; j < N; ++j)
-            if (!TINY || j < a.D) part[e + j] = dw[p][j];
+            if (!TINY || j < a.D) part[e + j] = AHEAD ? dw[AHEAD ? p : 0][j] : held(p)[j];
     }
     if (teams == 1) return;
     __syncthreads();
@@ -584,8 +606,23 @@ size_t norm_grad_bytes(int M, int D) {
 template <int DT, int P, int L, bool TINY>
 static hipError_t norm_grad_go(const NormGradArgs& a, const NormGradShape& s, hipStream_t st) {
     // teams share a workgroup of at most 512 threads, of one piece or two a lane: 512 x 2 pieces x 8 values
-    const int threads = s.teams * (L < 64 ? L : 64 * s.team.waves), lds = s.teams > 1 ? s.teams * a.D * (int)sizeof(float) : 0;
+    const int threads = s.teams * (L < 64 ? L : 64 * s.team.waves);
+    int lds = s.teams > 1 ? s.teams * a.D * (int)sizeof(float) : 0;
     if (lds > 512 * 2 * 8 * (int)sizeof(float)) return hipErrorInvalidValue;
+    if constexpr (P > 2) {                                   // the slots: at most 1024 threads' 32 values
+        constexpr int N = NormPiece<DT>::N;
+        static_assert(1024 * P * N <= NORM_MAX_D, "128 KB");
+        if (s.teams > 1 || threads != 1024) return hipErrorInvalidValue;
+        static std::atomic<bool> attr[kMaxDev], attr_res[kMaxDev];
+        lds = threads * P * N * (int)sizeof(float);
+        int dev = 0;
+        hipError_t e = current_device(&dev);
+        if (e != hipSuccess) return e;
+        e = a.d_h != nullptr
+                ? lds_limit_once(attr_res, dev, reinterpret_cast<const void*>(&norm_grad_kernel<DT, P, L, true, TINY>), lds)
+                : lds_limit_once(attr, dev, reinterpret_cast<const void*>(&norm_grad_kernel<DT, P, L, false, TINY>), lds);
+        if (e != hipSuccess) return e;
+    }
     if (a.d_h != nullptr)
         hipLaunchKernelGGL((norm_grad_kernel<DT, P, L, true, TINY>), dim3(s.groups), dim3(threads), lds, st, a, s.team.waves);
     else
