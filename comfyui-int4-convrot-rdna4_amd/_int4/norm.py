@@ -61,7 +61,7 @@ def _check(x, weight, residual, eps):
             raise ValueError(f"weight of shape {tuple(weight.shape)} does not fit: {(D,)} expected")
     if residual is not None and (residual.dtype != x.dtype or residual.shape != x.shape):
         raise ValueError(f"residual {residual.dtype} {tuple(residual.shape)} does not fit x {x.dtype} {tuple(x.shape)}")
-    if not 0.0 <= eps < float("inf"):
+    if not 0.0 <= float(eps) < float("inf"):
         raise ValueError(f"eps must be at least 0 and finite, got {eps}")
     _same_device(x, weight, residual)
     if D > max_norm_width():
@@ -223,7 +223,7 @@ def convrot_w8a8_linear_rows(rows: Int8Rows, qweight: torch.Tensor, wscales: tor
             raise ValueError(f"bias has {bias.numel()} elements, the weight has N={N} rows")
     if qweight_i8t is not None and (qweight_i8t.dtype != torch.int8 or tuple(qweight_i8t.shape) != (native.i8t_rows(N), K)):
         raise ValueError(f"qweight_i8t {qweight_i8t.dtype} {tuple(qweight_i8t.shape)} does not fit: int8 {(native.i8t_rows(N), K)} expected")
-    _no_grad("convrot_w8a8_linear_rows", wscales, bias)
+    _no_grad("convrot_w8a8_linear_rows", rows.scales, wscales, bias)
     _same_device(rows.codes, rows.scales, qweight, wscales, bias, qweight_i8t)
     dev, M = rows.codes.device, rows.scales.shape[0]
     out_shape = (*rows.shape[:-1], N)

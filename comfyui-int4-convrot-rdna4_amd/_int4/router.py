@@ -7,6 +7,7 @@ router's logits, with the gradient of the weights.
 from __future__ import annotations
 
 import math
+import operator
 
 import torch
 
@@ -93,18 +94,19 @@ def choose_experts(logits: torch.Tensor, top_k: int, balance_bias: torch.Tensor 
     if logits.dim() == 0 or logits.shape[-1] == 0:
         raise ValueError(f"logits must be [..., E], got shape {tuple(logits.shape)}")
     E = logits.shape[-1]
+    top_k, num_groups = operator.index(top_k), operator.index(num_groups)
     if scoring not in _SCORING:
         raise ValueError(f"scoring must be one of {_SCORING}, got {scoring!r}")
     if group_score not in _GROUP_SCORES:
         raise ValueError(f"group_score must be one of {_GROUP_SCORES}, got {group_score!r}")
     if not 1 <= num_groups or E % num_groups:
         raise ValueError(f"{E} experts are not num_groups={num_groups} equal groups")
-    if top_groups is None:
-        top_groups = num_groups
+    top_groups = num_groups if top_groups is None else operator.index(top_groups)
     if not 1 <= top_groups <= num_groups:
         raise ValueError(f"top_groups must be 1 to {num_groups}, got {top_groups}")
     if not 1 <= top_k <= E // num_groups * top_groups:
         raise ValueError(f"top_k must be 1 to {E // num_groups * top_groups}, got {top_k}")
+    scale = float(scale)
     if not math.isfinite(scale) or abs(scale) > torch.finfo(torch.float32).max:
         raise ValueError(f"scale must be finite in float32, got {scale}")
     _count(logits.numel() // E * top_k, "slots")
@@ -116,7 +118,7 @@ def choose_experts(logits: torch.Tensor, top_k: int, balance_bias: torch.Tensor 
     if E > max_experts():
         raise ValueError(f"{E} experts are too many: at most {max_experts()} experts")
     _no_tangent("choose_experts", logits, balance_bias)
-    how = (top_k, scoring == "sigmoid", num_groups, top_groups, group_score == "sum2", bool(renormalize), float(scale))
+    how = (top_k, scoring == "sigmoid", num_groups, top_groups, group_score == "sum2", bool(renormalize), scale)
     if torch.is_grad_enabled() and logits.requires_grad:
         return _Choose.apply(logits, balance_bias, *how)
     return _choose(logits, balance_bias, *how)

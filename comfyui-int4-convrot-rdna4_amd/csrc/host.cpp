@@ -788,7 +788,7 @@ PyObject* w8a8_rows(PyObject*, PyObject* const* a, Py_ssize_t n) {
         qw.scalar_type() != at::kChar || qw.size(1) != K || qw.size(0) < 1 || qw.size(0) > INT32_MAX)
         Py_RETURN_NONE;
     const int64_t N = qw.size(0);
-    if (ws.scalar_type() != at::kFloat || ws.numel() != N || wants_grad(ws) || w.scalar_type() != at::kChar || w.dim() != 2 ||
+    if (ws.scalar_type() != at::kFloat || ws.numel() != N || wants_grad(ws) || wants_grad(xs) || w.scalar_type() != at::kChar || w.dim() != 2 ||
         w.size(0) != (N + 255) / 256 * 256 || w.size(1) != K ||
         (b.defined() && (dtype_code(b) < 0 || b.numel() != N || wants_grad(b))) || cr_convrot_w8a8_linear_i8t_split((int)M, (int)N, (int)K))
         Py_RETURN_NONE;

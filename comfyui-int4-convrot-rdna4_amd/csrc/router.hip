@@ -7,7 +7,7 @@
 //   ids = the k experts of the greatest c, greatest first; w = s[ids] (renormalized: over their sum) times `scale`
 // An expert whose logit or bias is -inf is not available; a slot that finds none has id -1 and weight 0.
 //
-// The order is decided in 64 bits: c is rounded to 43 bits, far below what 32-bit scores could tell apart, and equal
+// The order is decided in 64 bits: c is cut to 43 bits, far below what 32-bit scores could tell apart, and equal
 // ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them.  A key
 // holds both: the low ten bits of a double give way to the index (1023 - e, or e where c is negative, so that of
 // equal values the lowest index is the greatest key).  Keys are finite and differ, and the greater and the smaller of
@@ -66,9 +66,9 @@ __device__ __forceinline__ int key_number(double key) {
     return is_none(key) ? -1 : 1023 - low;
 }
 
-// exp(x) to 2^-46 of its value, x at most 700; below -700 as at -700: x = n ln 2 + r, a polynomial of exp(r) on
-// |r| <= ln(2) / 2 (its series, whose next term is below 2^-47).  Seventeen instructions where the library's takes
-// forty; the choice keeps 43 bits.
+// exp(x) to 2^-46 of its value for |x| up to 350, 2^-45 up to 700, x at most 700; below -700 as at -700: x = n ln 2 + r, a
+// polynomial of exp(r) on |r| <= ln(2) / 2 (its series, whose next term is below 2^-47).  Seventeen instructions where the
+// library's takes forty; the choice keeps 43 bits.
 __device__ __forceinline__ double choice_exp(double x) {
     x = x < -700.0 ? -700.0 : x;
     const double t = __builtin_fma(x, 1.4426950408889634, 0x1.8p52);

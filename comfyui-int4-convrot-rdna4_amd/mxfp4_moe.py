@@ -94,7 +94,8 @@ class RoutedMxfp4MoE(torch.nn.Module):
         with torch.no_grad():
             n = _int4.rms_norm(x, self.norm_weight, residual, self.eps)
         n, h = (n, None) if residual is None else n
-        logits = torch.nn.functional.linear(n.to(torch.float32), self.router_weight.to(torch.float32))
+        with torch.autocast(n.device.type, enabled=False):
+            logits = torch.nn.functional.linear(n.to(torch.float32), self.router_weight.to(torch.float32))
         ids, weights = _int4.choose_experts(logits, self.top_k, self.balance_bias, **self.how)
         y = self.moe(n, ids, weights)
         return y if residual is None else (y, h)

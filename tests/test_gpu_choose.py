@@ -370,3 +370,55 @@ def test_many_rows(backend, gpu):
     top = want.values[:, :2].double()
     e = torch.exp(top - top[:, :1])
     assert bool(((w.double() - e / e.sum(-1, keepdim=True)).abs() <= 64 * U).all())
+
+
+def plain_many(logits, k, bias, scoring, num_groups, top_groups, group_score):
+    """The choice of many tokens, in 64 bits with stable sorts."""
+    l = logits.double()
+    T, E = l.shape
+    score = torch.sigmoid(l) if scoring == "sigmoid" else torch.softmax(l, -1)
+    c = l if bias is None else score + bias.double()
+    rank = score if bias is None and group_score == "sum2" else c
+    c, rank = (t.masked_fill(l == -math.inf, -math.inf) for t in (c, rank))
+    if num_groups > 1:
+        two = rank.reshape(T, num_groups, -1).sort(dim=-1, descending=True).values[..., :2]
+        value = two[..., 0] if group_score == "max" or two.shape[-1] < 2 else \
+            torch.where(two[..., 1] == -math.inf, two[..., 0], two.sum(-1))
+        kept = value.sort(dim=-1, descending=True, stable=True).indices[:, :top_groups]
+        mask = torch.zeros_like(value, dtype=torch.bool).scatter_(1, kept, True).repeat_interleave(E // num_groups, 1)
+        c = c.masked_fill(~mask, -math.inf)
+    top = c.sort(dim=-1, descending=True, stable=True)
+    return torch.where(top.values[:, :k] == -math.inf, -1, top.indices[:, :k]).int()
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("E,k,groups,top", [(8, 2, 1, 1), (30, 4, 3, 2), (32, 8, 2, 1), (33, 3, 1, 1), (64, 6, 8, 3), (100, 6, 1, 1), (100, 8, 5, 2),
+                                            (128, 4, 1, 1), (128, 8, 4, 2), (250, 10, 1, 1), (256, 8, 8, 4), (256, 12, 16, 5), (512, 8, 8, 2),
+                                            (1000, 8, 10, 3)])
+def test_many_tokens(backend, gpu, E, k, groups, top, dtype):
+    """Calls of 2^19 logits and more, which give a lane sixteen experts, with some rows masked, and their gradients."""
+    T = (1 << 19) // E + 77
+    g = torch.Generator(device="cuda").manual_seed(E + k)
+    l = (2 * torch.randn(T, E, generator=g, device="cuda") + 0.7 * torch.randn(E, generator=g, device="cuda")).to(dtype)
+    l[::5, ::3] = -math.inf
+    l[11] = -math.inf
+    bias = bias_of(E, k)
+    d_w = torch.randn(T, k, generator=g, device="cuda")
+    for scoring, b, group_score, renormalize in (("softmax", None, "max", True), ("sigmoid", bias, "sum2", True), ("softmax", bias, "max", False),
+                                                 ("softmax", None, "sum2", False), ("sigmoid", None, "max", False)):
+        leaf = l.clone().requires_grad_(True)
+        ids, w = backend.choose_experts(leaf, k, b, scoring=scoring, num_groups=groups, top_groups=top, group_score=group_score,
+                                        renormalize=renormalize, scale=1.5)
+        assert torch.equal(ids, plain_many(l, k, b, scoring, groups, top, group_score))
+        ref = l.double().requires_grad_(True)
+        want = torch.nan_to_num(weights_of(ref, ids, scoring, renormalize, 1.5))           # the row without an expert
+        tol = tolerance(l, E)
+        assert bool(((w.double() - want).abs() <= want.abs() * tol + 1e-37).all())
+        d, = torch.autograd.grad(w, leaf, d_w)
+        keep = torch.ones(T, 1, device="cuda")
+        keep[11] = 0
+        ok = l.double().masked_fill(keep == 0, 0.0).requires_grad_(True)                    # its gradient is zero
+        exact, = torch.autograd.grad(weights_of(ok, ids, scoring, renormalize, 1.5) * keep, ok, d_w.double())
+        size = want.amax(-1, keepdim=True) / 1.5 * 1.5 * d_w.double().abs().amax(-1, keepdim=True)
+        bound = exact.abs() * torch.finfo(dtype).eps / 2 + size * (2 * tol + (k + 8) * U) + torch.finfo(dtype).tiny
+        assert bool(((d.double() - exact).abs() <= bound).all())

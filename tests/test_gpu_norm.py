@@ -528,3 +528,58 @@ def test_past_32_bits(backend, gpu):
     head = x.detach()[:5].clone().requires_grad_(True)
     want, = torch.autograd.grad(backend.rms_norm(head, w), head, x.detach()[:5])
     assert torch.equal(d[:5], want) and torch.equal(d[-5:], want)
+
+
+@pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
+@pytest.mark.parametrize("D", [3, 64, 100, 200, 320, 520, 1024, 2304, 4097, 5120, 8192, 8193, 16384, 20000, 32768])
+def test_many_rows(backend, gpu, D, dtype):
+    """Rows enough for every way they are shared out, several to a workgroup in turn for the gradient; references in 64 bits."""
+    M = 1333 if D > 1024 else 7001
+    g = torch.Generator(device="cuda").manual_seed(D)
+    x, r, dy, dh = (torch.randn(M, D, generator=g, device="cuda").to(dtype) for _ in range(4))
+    w = 1 + 0.2 * torch.randn(D, generator=g, device="cuda")
+    leaves = [t.clone().requires_grad_(True) for t in (x, w, r)]
+    y, h = backend.rms_norm(leaves[0], leaves[1], leaves[2])
+    assert torch.equal(h, kept(x, r))
+    h64, w64 = h.detach().double(), w.double()
+    rstd = 1 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-6)
+    n = h64 * rstd
+    tiny = torch.finfo(dtype).tiny
+    assert bool(((y.double() - n * w64).abs() <= (n * w64).abs() * (half(dtype) + 4 * U) + tiny).all())
+    assert torch.equal(backend.rms_norm(h.detach(), w), y)
+    d_x, d_w, d_r = torch.autograd.grad((y, h), leaves, (dy, dh))
+    assert torch.equal(d_x, d_r)
+    gw = dy.double() * w64
+    mean = (gw * n).mean(-1, keepdim=True)
+    want = rstd * (gw - n * mean) + dh.double()
+    size = rstd * (gw.abs() + n.abs() * mean.abs())                     # as the bound above of each gradient
+    bound = want.abs() * half(dtype) + 8 * U * (size + dh.double().abs()) + tiny
+    bound += 2 * U * rstd * n.abs() * (gw * n).abs().mean(-1, keepdim=True)
+    assert bool(((d_x.double() - want).abs() <= bound).all())
+    terms = dy.double() * n
+    # each sum: a team's rows (M over 256 teams at the least), up to 32 teams, 1024 workgroups' parts in 64 strands
+    depth = math.ceil(M / 256) + 32 + 16 + 2 + 16 + 3
+    assert bool(((d_w.double() - terms.sum(0)).abs() <= depth * U * terms.abs().sum(0) + tiny).all())
+    plain, = torch.autograd.grad(backend.rms_norm(leaves[0], None), leaves[0], dy)
+    h64 = x.double()
+    rstd = 1 / torch.sqrt((h64 * h64).mean(-1, keepdim=True) + 1e-6)
+    n, gw = h64 * rstd, dy.double()
+    mean = (gw * n).mean(-1, keepdim=True)
+    want = rstd * (gw - n * mean)
+    bound = want.abs() * half(dtype) + 8 * U * rstd * (gw.abs() + n.abs() * mean.abs()) + tiny
+    bound += 2 * U * rstd * n.abs() * (gw * n).abs().mean(-1, keepdim=True)
+    assert bool(((plain.double() - want).abs() <= bound).all())
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("G,D", [(16, 208), (16, 2064), (64, 320), (64, 4160), (256, 256), (256, 512), (256, 768), (256, 2304), (256, 5120),
+                                 (256, 8192), (256, 16384), (256, 20480)])
+def test_int8_many_rows(backend, gpu, G, D, dtype):
+    """Rows enough for two chunks a lane, and short rows several to a wave; the codes of a row do not depend on the call's others."""
+    M = 4500 if D < 1024 else 1500
+    x, r = data(M, D, dtype, 1), data(M, D, dtype, 2, 4.0)
+    w = 1 + 0.2 * data(1, D, torch.float32, 3)[0]
+    rows = check_rows(backend, x, w, r, G)
+    few, h = backend.rms_norm_int8(x[-3:], w, r[-3:], convrot_groupsize=G)
+    assert torch.equal(few.codes, rows.codes[-3:]) and torch.equal(few.scales, rows.scales[-3:])
+    check_rows(backend, x, w.to(dtype), None, G, i8t=D % 64 == 0)
