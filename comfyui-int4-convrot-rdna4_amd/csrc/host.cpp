@@ -419,6 +419,7 @@ at::Tensor combine_rows(const at::Tensor& rows, const at::Tensor& weights, const
 
 // A gradient's own form: its values as they are read, contiguous, aligned
 at::Tensor settled(const at::Tensor& t) {
+    if (!t.is_neg() && t.is_contiguous() && reinterpret_cast<uintptr_t>(t.const_data_ptr()) % 16 == 0) return t;
     at::Tensor c = t.resolve_neg().contiguous();
     return reinterpret_cast<uintptr_t>(c.const_data_ptr()) % 16 != 0 ? c.clone() : c;
 }
@@ -428,7 +429,7 @@ at::Tensor restored(const at::Tensor& t, const char* what, at::ScalarType type, 
     TORCH_CHECK(t.defined() && t.layout() == at::kStrided && t.device() == dev && t.scalar_type() == type && t.sizes() == sizes,
                 "the saved ", what, " came back in another form: ", type, " ", sizes, " on ", dev, " expected, got ",
                 t.toString(), " ", t.sizes(), " on ", t.device());
-    return settled(t.detach());
+    return settled(t);                       // under NoGradGuard: its own graph is not looked at
 }
 
 // The saved positions [T, k] of T tokens' slots, or of any number of tokens (T < 0)
