@@ -50,9 +50,9 @@ __device__ __forceinline__ void settle(double (&k)[N]) {
     }
 }
 
-// The key of choice c (RT_NONE, or above -2^1000 and at most RT_MOST) of number e
+// The key of choice c (RT_NONE, or above -2^1000 and at most RT_MOST, no -0) of number e
 __device__ __forceinline__ double key_of(double c, int e) {
-    const uint64_t u = (uint64_t)__double_as_longlong(c + 0.0);       // -0 counts as 0
+    const uint64_t u = (uint64_t)__double_as_longlong(c);
     const uint32_t hi = (uint32_t)(u >> 32), lo = (uint32_t)u;
     const uint32_t low = (uint32_t)(1023 - e) ^ ((uint32_t)((int)hi >> 31) & 1023u);
     return __longlong_as_double((long long)((uint64_t)hi << 32 | ((lo & ~1023u) | low)));
@@ -66,32 +66,30 @@ __device__ __forceinline__ int key_number(double key) {
     return is_none(key) ? -1 : 1023 - low;
 }
 
-// exp(x) to 2^-46 of its value for |x| up to 350, 2^-45 up to 700, x at most 700; below -700 as at -700: x = n ln 2 + r, a
-// polynomial of exp(r) on |r| <= ln(2) / 2 (its series, whose next term is below 2^-47).  Seventeen instructions where the
-// library's takes forty; the choice keeps 43 bits.
+// exp(x) to 2^-47 of its value for |x| up to 200, 2^-45 up to 700, x at most 700; below -700 as at -700: x = n ln 2 + r, and of
+// exp(r) on |r| <= ln(2) / 2 the polynomial of degree 10 that is 1 at 0 and meets exp at the ten Chebyshev points of the
+// interval (off by 2^-50.5 at most).  Sixteen instructions where the library's takes forty; the choice keeps 43 bits.
 __device__ __forceinline__ double choice_exp(double x) {
     x = x < -700.0 ? -700.0 : x;
     const double t = __builtin_fma(x, 1.4426950408889634, 0x1.8p52);
     const double r = __builtin_fma(t - 0x1.8p52, -0.6931471805599453, x);
-    double p = 1.0 / 39916800;
-    p = __builtin_fma(p, r, 1.0 / 3628800);
-    p = __builtin_fma(p, r, 1.0 / 362880);
-    p = __builtin_fma(p, r, 1.0 / 40320);
-    p = __builtin_fma(p, r, 1.0 / 5040);
-    p = __builtin_fma(p, r, 1.0 / 720);
-    p = __builtin_fma(p, r, 1.0 / 120);
-    p = __builtin_fma(p, r, 1.0 / 24);
-    p = __builtin_fma(p, r, 1.0 / 6);
-    p = __builtin_fma(p, r, 0.5);
-    p = __builtin_fma(p, r, 1.0);
+    double p = 0x1.28917c89a43a7p-22;
+    p = __builtin_fma(p, r, 0x1.72e107c874de9p-19);
+    p = __builtin_fma(p, r, 0x1.a019b9149a41cp-16);
+    p = __builtin_fma(p, r, 0x1.a01994c849582p-13);
+    p = __builtin_fma(p, r, 0x1.6c16c17889ef1p-10);
+    p = __builtin_fma(p, r, 0x1.11111123bf154p-7);
+    p = __builtin_fma(p, r, 0x1.5555555553d68p-5);
+    p = __builtin_fma(p, r, 0x1.5555555550d88p-3);
+    p = __builtin_fma(p, r, 0x1.0000000000001p-1);
+    p = __builtin_fma(p, r, 0x1.0000000000006p+0);
     p = __builtin_fma(p, r, 1.0);
     return __builtin_amdgcn_ldexp(p, (int)(uint32_t)(uint64_t)__double_as_longlong(t));
 }
 
-// 1 / d of a finite d >= 1: the instruction's approximation and two Newton steps
+// 1 / d of a finite d >= 1 to 2^-46: the instruction's approximation (to 2^-23 at least) and a Newton step
 __device__ __forceinline__ double choice_rcp(double d) {
-    double r = __builtin_amdgcn_rcp(d);
-    r = __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
+    const double r = __builtin_amdgcn_rcp(d);
     return __builtin_fma(__builtin_fma(-d, r, 1.0), r, r);
 }
 
@@ -329,8 +327,8 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
     float l[P], b[P];
     load_logits(row, a.dt, e0, a.E, l);
     if (a.bias != nullptr) load_logits(a.bias, DT_F32, e0, a.E, b);
-    float m = l[0];
-    if (!a.sigmoid) {
+    float m = l[0];                                                   // softmax: the greatest, which the weights may need too
+    if (!a.sigmoid && (by_score || !a.renormalize)) {
 #pragma unroll
         for (int p = 1; p < P; ++p) m = fmaxf(m, l[p]);
         m = max_lanes<L>(m);
@@ -357,14 +355,16 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
 #pragma unroll
             for (int p = 0; p < P; ++p) c[p] *= inv;
         }
+        // -inf of the logit or the bias, also beside a NaN; scores are no -0, nor is their sum with one
 #pragma unroll
         for (int p = 0; p < P; ++p) {
-            const bool out = l[p] == -__builtin_inff() || (a.bias != nullptr && b[p] == -__builtin_inff());
-            c[p] = out ? RT_NONE : key_min(a.bias != nullptr ? c[p] + (double)b[p] : c[p], RT_MOST);
+            const float add = l[p] == -__builtin_inff() ? l[p] : a.bias != nullptr ? b[p] : 0.0f;
+            const double v = key_min(c[p] + (double)add, RT_MOST);              // of a NaN RT_MOST
+            c[p] = add == -__builtin_inff() ? RT_NONE : v;
         }
     } else {
 #pragma unroll
-        for (int p = 0; p < P; ++p) c[p] = l[p] == -__builtin_inff() ? RT_NONE : key_min((double)l[p], RT_MOST);
+        for (int p = 0; p < P; ++p) c[p] = key_max(key_min((double)l[p] + 0.0, RT_MOST), RT_NONE);      // -0 counts as 0
     }
     if constexpr (GROUPS) keep_groups<L>(c, a, sub, table_lds + tid / L * (L * P));
 #pragma unroll
@@ -397,40 +397,55 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
         }
         wave_sync();
     }
-    // f(j, its expert) for this lane's slots
-    const auto each = [&](auto f) {
-        if constexpr (K > 0) {
-#pragma unroll
-            for (int i = 0; i < MINE; ++i)
-                if (i * L + sub < a.k) f(i * L + sub, key_number(mine[i]));
-        } else {
-            for (int j = sub; j < a.k; j += L) f(j, chosen[j]);
-        }
-    };
-
-    // the weights, in 32 bits from the chosen logits
     float total = 0.0f;
-    if (a.renormalize) {
-        float top = -__builtin_inff();
-        each([&](int, int e) { if (e >= 0) top = fmaxf(top, logit_at(row, a.dt, e)); });
-        m = max_lanes<L>(top);
-        each([&](int, int e) { if (e >= 0) total += score_over(logit_at(row, a.dt, e), m, a.sigmoid); });
-        total = sum_lanes<L>(total);
-    } else if (!a.sigmoid) {
+    if (!a.sigmoid && !a.renormalize) {
 #pragma unroll
         for (int p = 0; p < P; ++p) total += l[p] == -__builtin_inff() ? 0.0f : expf(l[p] - m);
         total = sum_lanes<L>(total);
     }
-    if (spoilt) total = __builtin_nanf("");
-    each([&](int j, int e) {
-        float w = 0.0f;
-        if (e >= 0) {
-            const float v = logit_at(row, a.dt, e);
-            w = (a.sigmoid && !a.renormalize ? sigmoid_of(v) : score_over(v, m, a.sigmoid) / total) * a.scale;
-        }
+    // the weights, in 32 bits from the chosen logits
+    const auto put = [&](int j, int e, float score) {
         a.ids[t * a.k + j] = e;
-        a.weights[t * a.k + j] = w;
-    });
+        a.weights[t * a.k + j] = e >= 0 ? score * a.scale : 0.0f;
+    };
+    const auto score_of = [&](float v) { return a.sigmoid && !a.renormalize ? sigmoid_of(v) : score_over(v, m, a.sigmoid); };
+    const bool over = a.renormalize || !a.sigmoid;                    // over `total`
+    if constexpr (K > 0) {
+        int e[MINE];
+        float v[MINE], s[MINE], top = -__builtin_inff();
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            e[i] = i * L + sub < a.k ? key_number(mine[i]) : -1;
+            v[i] = e[i] >= 0 ? logit_at(row, a.dt, e[i]) : -__builtin_inff();
+            top = fmaxf(top, v[i]);
+        }
+        if (a.renormalize) m = max_lanes<L>(top);
+#pragma unroll
+        for (int i = 0; i < MINE; ++i) {
+            s[i] = score_of(v[i]);
+            if (a.renormalize && e[i] >= 0) total += s[i];
+        }
+        if (a.renormalize) total = sum_lanes<L>(total);
+        if (spoilt) total = __builtin_nanf("");
+#pragma unroll
+        for (int i = 0; i < MINE; ++i)
+            if (i * L + sub < a.k) put(i * L + sub, e[i], over ? s[i] / total : s[i]);
+    } else {
+        if (a.renormalize) {
+            float top = -__builtin_inff();
+            for (int j = sub; j < a.k; j += L)
+                if (chosen[j] >= 0) top = fmaxf(top, logit_at(row, a.dt, chosen[j]));
+            m = max_lanes<L>(top);
+            for (int j = sub; j < a.k; j += L)
+                if (chosen[j] >= 0) total += score_of(logit_at(row, a.dt, chosen[j]));
+            total = sum_lanes<L>(total);
+        }
+        if (spoilt) total = __builtin_nanf("");
+        for (int j = sub; j < a.k; j += L) {
+            const float s = chosen[j] >= 0 ? score_of(logit_at(row, a.dt, chosen[j])) : 0.0f;
+            put(j, chosen[j], over ? s / total : s);
+        }
+    }
 }
 
 // Values e0 .. e0 + P - 1 of a row of E in type dt

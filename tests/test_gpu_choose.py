@@ -201,6 +201,16 @@ def test_values_that_are_not_finite(backend, gpu):
     ids, w = backend.choose_experts(l, k, renormalize=False, scoring="sigmoid")
     assert w[2, 0] == 1 and w[1].isnan().tolist() == [True, False, False, False]
     assert torch.equal(ids[[0, 4, 5]], clean[0][[0, 4, 5]])
+    masked = l.clone()
+    masked[:, 20:] = -math.inf                                         # not chosen beside a NaN either
+    out = torch.zeros(E, device="cuda")
+    out[:12] = -math.inf
+    for scoring in ("softmax", "sigmoid"):
+        for how in ({}, dict(num_groups=4, top_groups=2, group_score="sum2")):
+            assert bool((backend.choose_experts(masked, k, torch.zeros(E, device="cuda"), scoring=scoring, **how)[0] < 20).all())
+            assert bool((backend.choose_experts(masked, k, scoring=scoring, **how)[0] < 20).all())
+            ids = backend.choose_experts(masked, k, out, scoring=scoring, **how)[0]
+            assert bool(((ids < 20) & ((ids >= 12) | (ids == -1))).all())
     bias = torch.zeros(E, device="cuda")
     bias[11] = math.inf                                                # one that is always chosen
     bias[12] = math.nan                                                # ranks with it
