@@ -14,10 +14,17 @@
 
 namespace convrot {
 
-constexpr int NORM_PIECES = 2;             // pieces a lane of a row's norm
-constexpr int NORM_GRAD_ALONE = 3;         // rows of a team that a single workgroup takes
-constexpr int NORM_GRAD_FEW = 2048;        // waves of a gradient that take a piece a lane each
-constexpr int NORM8_FEW = 4096;            // waves of the 8-bit form that take a chunk a lane each
+// Measured on MI355X, graph replays, bf16, us.
+// Pieces a lane of a row's norm: 16384 x 5120 with 1, 2 and 4 127, 115 and 118, without residual 101, 66 and 64; 4096 x 13824
+// 83, 82 and 83.
+constexpr int NORM_PIECES = 2;
+// Rows of a team that a single workgroup takes: 8 x 1024 5.3, in two launches 6.1; 1 x 4096 3.4 and 7.0.
+constexpr int NORM_GRAD_ALONE = 3;
+// Waves of a gradient that take a piece a lane each, others two: 512 x 4096 15.6 and 13.4, 4096 x 5120 57 and 44.
+constexpr int NORM_GRAD_FEW = 2048;
+// Waves of the 8-bit form that take a chunk a lane each, others two: 64 x 4096 4.1 and 5.2, 512 x 4096 6.5 and 7.9, 1024 x 4096
+// 10.1 and 10.1, 8192 x 5120 70.7 and 69.4, 4096 x 16384 144 and 114.
+constexpr int NORM8_FEW = 4096;
 
 // 16 bytes of a row as floats.  Rows of a width that is no whole number of pieces lie at any multiple of their
 // element's size, which loads and stores of 16 bytes may; their last piece ends with the row and shares elements with the
@@ -159,6 +166,10 @@ __device__ __forceinline__ double sum_waves(double v, double* slot, int waves) {
     return s;
 }
 
+// Bound by memory: 16384 x 5120 bf16 with a residual 115 us, 5.8 TB/s of the four tensors, without 66 us, 5.1 TB/s.  The weight
+// is read after the sums: before them its registers cost waves (8192 x 4096 56 us, so 50).  Stores that the caches do not keep
+// make this kernel shorter (512 x 4096 5.7 and 5.3, 16384 x 5120 115 and 109) and whoever reads y and h next longer by more:
+// with a copy of both 2048 x 4096 24.9 and 28.4, 4096 x 5120 58 and 64, 8192 x 4096 90 and 97.
 template <int DT, int P, int L, bool RES, bool TINY>
 __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a, int waves, unsigned first) {
     using V = NormPiece<DT, TINY>;
@@ -219,6 +230,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a, int waves, unsig
 // The gradient: with n = h rstd and g = w d_y,  d_x = rstd (g - n mean(g n)) + d_h,  d_weight = sum over rows of d_y n.
 // Teams walk rows, each row's loads sent out before the row before it is worked on, and keep their part of d_weight in
 // registers; a workgroup adds its teams' parts in LDS, and a second launch the workgroups', all in order.
+// Bound by memory: 8192 x 4096 bf16 with d_h 50 us, 5.4 TB/s of its four tensors, and 4 us of adding up (90 without
+// the loads ahead); 110000 x 128 25 us in all, 3.4 TB/s.
 //
 // What a row takes of a lane's registers is kept as it lies in memory (`again` makes the compiler unpack it a second time
 // rather than hold the floats across the sums); rows of four and more pieces a lane are not fetched ahead, read d_h and
@@ -401,6 +414,8 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 // A lane holds 16 consecutive values.  Everything up to the code is fp64 (full rate here), so a code is the formula's
 // nearest one and not a matter of the order of sums; rstd commutes with the rotation, so it is not waited for.  A row
 // with a value that is not finite (or zeros over eps = 0) gets scale NaN and codes 0.
+// 8192 x 5120 bf16 with a residual 68 us, 4.3 TB/s: memory, and VALU instructions half of the time (28 an element, of which
+// the rotation's are 7); without a residual 48 us, where they are 60%.  LDS for the rotation's transpose holds a CU to 16 waves.
 // ---------------------------------------------------------------------------
 template <int DT, int G, int P, int L, bool TILED>
 __global__ __launch_bounds__(1024) void norm_int8_kernel(NormArgs a, unsigned first) {
