@@ -18,7 +18,7 @@ namespace convrot {
 // Pieces a lane of a row's norm: 16384 x 5120 with 1, 2 and 4 127, 115 and 118, without residual 101, 66 and 64; 4096 x 13824
 // 83, 82 and 83.
 constexpr int NORM_PIECES = 2;
-// Rows of a team that a single workgroup takes: 8 x 1024 5.3, in two launches 6.1; 1 x 4096 3.4 and 7.0.
+// Rows of a team that a single workgroup of several teams takes: 8 x 1024 5.3, in two launches 6.1.
 constexpr int NORM_GRAD_ALONE = 3;
 // Waves of a gradient that take a piece a lane each, others two: 512 x 4096 15.6 and 13.4, 4096 x 5120 57 and 44.
 constexpr int NORM_GRAD_FEW = 2048;
@@ -598,8 +598,8 @@ hipError_t norm_launch(const NormArgs& a, int dt, hipStream_t st) {
 // Teams and workgroups of a gradient, from its shape: workgroups of eight waves or one team.  Each leaves a row of partial
 // sums of d_weight, to be read again: as many workgroups as the chip holds at once (16 waves a CU), but no more than makes
 // that an eighth of the rows' traffic (8192 x 4096: 512 workgroups 55.6 us, 1024 61.6; 2048 x 13824: 256 58.6, 512
-// 69.2; 110000 x 128: 512 30.2, 1024 24.9).  One workgroup where each team has few rows, which then writes d_weight
-// itself.
+// 69.2; 110000 x 128: 512 30.2, 1024 24.9).  One workgroup where it has several teams and each few rows, which then
+// writes d_weight itself.
 struct NormGradShape { NormShape team; int teams, groups; };
 static NormGradShape norm_grad_shape(int M, int D, int piece) {
     const int pieces = (D + piece - 1) / piece;
@@ -653,7 +653,8 @@ hipError_t norm_grad_launch(const NormGradArgs& a, int dt, hipStream_t st) {
             return norm_grad_go<DT, decltype(p)::value, decltype(l)::value, decltype(t)::value>(a, s, st);
         });
     });
-    if (e != hipSuccess || a.d_weight == nullptr || s.groups == 1) return e;
+    // several teams of one workgroup have written d_weight themselves
+    if (e != hipSuccess || a.d_weight == nullptr || (s.groups == 1 && s.teams > 1)) return e;
     hipLaunchKernelGGL(norm_weight_grad_kernel, dim3((a.D + 15) / 16), dim3(1024), 0, st, a.partial, a.d_weight, a.weight_dt, a.D,
                        s.groups);
     return hipGetLastError();

@@ -583,3 +583,14 @@ def test_int8_many_rows(backend, gpu, G, D, dtype):
     few, h = backend.rms_norm_int8(x[-3:], w, r[-3:], convrot_groupsize=G)
     assert torch.equal(few.codes, rows.codes[-3:]) and torch.equal(few.scales, rows.scales[-3:])
     check_rows(backend, x, w.to(dtype), None, G, i8t=D % 64 == 0)
+
+
+@pytest.mark.parametrize("dtype", DTYPES)
+@pytest.mark.parametrize("D", [40, 512, 1024, 2048, 4096, 5000, 8192, 13824, 16384, 32768])
+def test_gradient_of_few_rows(backend, gpu, D, dtype):
+    """One workgroup, of one team or several, and the few beside it: the weight's gradient is there in each."""
+    w = 1 + 0.2 * data(1, D, torch.float32, 9)[0]
+    for M in (1, 2, 3, 4, 7, 25):
+        x, r, dy, dh = (data(M, D, dtype, s) for s in range(4))
+        check_gradient(backend, x, w, r, dy, dh)
+        check_gradient(backend, x, w.to(dtype), None, dy, None)
