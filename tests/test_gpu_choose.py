@@ -432,3 +432,21 @@ def test_many_tokens(backend, gpu, E, k, groups, top, dtype):
         size = want.amax(-1, keepdim=True) / 1.5 * 1.5 * d_w.double().abs().amax(-1, keepdim=True)
         bound = exact.abs() * torch.finfo(dtype).eps / 2 + size * (2 * tol + (k + 8) * U) + torch.finfo(dtype).tiny
         assert bool(((d.double() - exact).abs() <= bound).all())
+
+
+def test_past_32_bits(backend, gpu):
+    """Logits whose numbers pass 2^31 and bytes 2^32; the last tokens are the first ones' copies."""
+    T, E = (1 << 23) + 77, 264
+    l = torch.empty(T, E, dtype=torch.bfloat16, device="cuda").normal_()
+    l[-9:] = l[:9]
+    bias = bias_of(E, 1)
+    how = dict(scoring="sigmoid", num_groups=8, top_groups=3, group_score="sum2")
+    few = backend.choose_experts(l[:9], 5, bias, **how)
+    leaf = l.requires_grad_(True)
+    ids, w = backend.choose_experts(leaf, 5, bias, **how)
+    for got, want in zip((ids, w), few):
+        assert torch.equal(got[:9], want) and torch.allclose(got[-9:].float(), want.float(), rtol=32 * U)
+    d_w = torch.randn(9, 5, device="cuda").repeat(T // 9 + 1, 1)[:T]
+    d_w[-9:] = d_w[:9]
+    d, = torch.autograd.grad(w, leaf, d_w)
+    assert bool(d[:9].any()) and torch.allclose(d[-9:].float(), d[:9].float(), rtol=2.0 ** -6)
