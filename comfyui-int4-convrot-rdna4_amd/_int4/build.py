@@ -112,7 +112,7 @@ def _compile_host() -> str:
 def _link_host(obj: str, lib: str, out: str) -> None:
     """The CPython module, bound to the kernel library next to it."""
     _run([_hipcc(), "-shared", "-fPIC", "-Wl,--as-needed", obj, "-L" + os.path.join(_torch_dir(), "lib"), "-ltorch_python", "-ltorch_cpu",
-          "-lc10", "-lc10_hip", "-L" + os.path.dirname(lib), "-l:" + os.path.basename(lib), "-Wl,-rpath,$ORIGIN"],
+          "-ltorch_hip", "-lc10", "-lc10_hip", "-L" + os.path.dirname(lib), "-l:" + os.path.basename(lib), "-Wl,-rpath,$ORIGIN"],
          out, "linking the host module")
 
 

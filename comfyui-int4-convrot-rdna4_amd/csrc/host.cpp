@@ -19,6 +19,7 @@
 #include <torch/csrc/autograd/python_variable.h>
 #include <torch/csrc/jit/frontend/tracer.h>
 #include <ATen/ATen.h>
+#include <ATen/hip/EmptyTensor.h>
 #include <c10/core/impl/TorchDispatchModeTLS.h>
 #include <c10/hip/HIPStream.h>
 #include <pybind11/pybind11.h>
@@ -238,8 +239,10 @@ int mx_group(PyObject* o, int64_t K) {
     return G > 0 && K % G == 0 ? G : -1;
 }
 
+// A GPU tensor beside t, from the caching allocator without the dispatcher between (0.3 us each: a choice of one token
+// 4.95 us a call, 4.45 so; the norm's 8-bit form with its three outputs 6.3 and 5.65).
 at::Tensor like(const at::Tensor& t, at::IntArrayRef sizes, at::ScalarType type) {
-    return at::empty(sizes, t.options().dtype(type).requires_grad(false));
+    return at::Tensor(at::detail::empty_cuda(sizes, type, t.device(), std::nullopt));
 }
 
 void* stream_of(c10::Device dev) { return c10::hip::getCurrentHIPStream(dev.index()).stream(); }
