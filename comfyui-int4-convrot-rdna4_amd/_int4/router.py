@@ -42,11 +42,14 @@ class _Choose(torch.autograd.Function):
         ctx.save_for_backward(logits, ids)
         ctx.shape, ctx.dtype, ctx.how = logits.shape, logits.dtype, (sigmoid, renormalize, scale)
         ctx.mark_non_differentiable(ids)
+        ctx.set_materialize_grads(False)
         return ids, weights
 
     @staticmethod
     @torch.autograd.function.once_differentiable
     def backward(ctx, _, d_weights):
+        if d_weights is None:
+            return (None,) * 9
         logits, ids = ctx.saved_tensors
         dev, (sigmoid, renormalize, scale) = d_weights.device, ctx.how
         logits = _restored(logits, "logits", ctx.dtype, ctx.shape, dev)

@@ -586,11 +586,12 @@ struct Choose : torch::autograd::Function<Choose> {
         ctx->mark_non_differentiable({ids});
         ctx->saved_data["how"] = std::vector<int64_t>{c.sigmoid, c.renormalize, logits.size(-1), (int64_t)logits.scalar_type()};
         ctx->saved_data["scale"] = (double)c.scale;
+        ctx->set_materialize_grads(false);                       // zeros for the ids would be filled, and not read
         return {ids, weights};
     }
     static torch::autograd::variable_list backward(torch::autograd::AutogradContext* ctx, torch::autograd::variable_list g) {
         at::Tensor d_logits;
-        {
+        if (g[1].defined()) {
             at::NoGradGuard no_grad;
             const auto saved = ctx->get_saved_variables();
             const auto how = ctx->saved_data["how"].toIntVector();

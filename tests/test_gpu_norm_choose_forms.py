@@ -97,6 +97,31 @@ def test_arguments_of_other_types(backend, path):
         backend.convrot_w8a8_linear_rows(rows._replace(scales=rows.scales.clone().requires_grad_()), rows.codes, rows.scales)
 
 
+class _Stop(torch.autograd.Function):
+    """Its input without a gradient."""
+    @staticmethod
+    def forward(ctx, x):
+        return x.clone()
+
+    @staticmethod
+    def backward(ctx, d):
+        return None
+
+
+def test_outputs_without_a_gradient(backend, path):
+    """A gradient that does not arrive is none, and those of the other outputs are as they were."""
+    t = tensors(torch.float32)
+    logits, x, r = (t[n].clone().requires_grad_() for n in ("logits", "x", "residual"))
+    _Stop.apply(backend.choose_experts(logits, 3)[1]).sum().backward()
+    assert logits.grad is None
+    y, h = backend.rms_norm(x, None, r)
+    (_Stop.apply(y).sum() + _Stop.apply(h).sum()).backward()
+    assert x.grad is None and r.grad is None
+    y, h = backend.rms_norm(x, None, r)
+    (_Stop.apply(y).sum() + (h * t["d_h"]).sum()).backward()
+    assert torch.equal(x.grad, t["d_h"]) and torch.equal(r.grad, t["d_h"])
+
+
 def test_parameters_and_subclasses(backend, path):
     """Parameters count as tensors; a weight that is frozen takes no gradient."""
     t = tensors(torch.float32)
