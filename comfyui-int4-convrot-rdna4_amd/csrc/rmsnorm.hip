@@ -15,15 +15,16 @@
 namespace convrot {
 
 // Measured on MI355X, graph replays, bf16, us.
-// Pieces a lane of a row's norm: 16384 x 5120 with 1, 2 and 4 127, 115 and 118, without residual 101, 66 and 64; 4096 x 13824
-// 83, 82 and 83.
+// Pieces a lane of a row's norm: 16384 x 5120 with 1, 2 and 4 117, 116 and 119, without residual 92, 62 and 60; 4096 x 13824
+// 81, 81 and 82.
 constexpr int NORM_PIECES = 2;
 // Rows of a team that a single workgroup of several teams takes: 8 x 1024 5.3, in two launches 6.1.
 constexpr int NORM_GRAD_ALONE = 3;
 // Waves of a gradient that take a piece a lane each, others two: 512 x 4096 15.6 and 13.4, 4096 x 5120 57 and 44.
 constexpr int NORM_GRAD_FEW = 2048;
-// Waves of the 8-bit form that take a chunk a lane each, others two: 64 x 4096 4.1 and 5.2, 512 x 4096 6.5 and 7.9, 1024 x 4096
-// 10.1 and 10.1, 8192 x 5120 70.7 and 69.4, 4096 x 16384 144 and 114.
+// Waves of the 8-bit form that take a chunk a lane each, others two: 64 x 4096 3.8 and 4.6, 512 x 4096 6.2 and 7.2, 1024 x 8192
+// without a residual 10.7 and 10.6, 8192 x 5120 45 and 39, 4096 x 16384 89 and 63.  With a residual rows of up to four waves
+// always do: 4096 x 4096 26.8 and 29.6, 8192 x 4096 47 and 49; 8192 x 5120 61.7 and 59.5, 3000 x 13824 87 and 65.
 constexpr int NORM8_FEW = 4096;
 
 // 16 bytes of a row as floats.  Rows of a width that is no whole number of pieces lie at any multiple of their
@@ -118,14 +119,18 @@ __device__ __forceinline__ void load_weight(const void* w, int dt, int e, int D,
             for (int i = 0; i < 4; ++i) v[j + i] = __uint_as_float(q[i]);
         }
     } else {
+        v2u_mx q[N / 4];
 #pragma unroll
-        for (int j = 0; j < N; j += 4) {
-            const v2u_mx q = *reinterpret_cast<const v2u_any*>(reinterpret_cast<const uint16_t*>(w) + e + j);
+        for (int j = 0; j < N / 4; ++j) q[j] = *reinterpret_cast<const v2u_any*>(reinterpret_cast<const uint16_t*>(w) + e + 4 * j);
+        if (dt == DT_BF16) {
 #pragma unroll
-            for (int i = 0; i < 4; ++i) {
-                const uint32_t h = q[i / 2];
-                v[j + i] = dt == DT_BF16 ? (i % 2 ? bf16hi_to_f32(h) : bf16lo_to_f32(h)) : f16bits_to_f32(h >> (i % 2 * 16));
+            for (int j = 0; j < N; j += 2) {
+                v[j] = bf16lo_to_f32(q[j / 4][j / 2 % 2]);
+                v[j + 1] = bf16hi_to_f32(q[j / 4][j / 2 % 2]);
             }
+        } else {
+#pragma unroll
+            for (int j = 0; j < N; ++j) v[j] = f16bits_to_f32(q[j / 4][j / 2 % 2] >> (j % 2 * 16));
         }
     }
 }
@@ -268,9 +273,9 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
     };
     long long row = (long long)blockIdx.x * teams + team.number;
     if (AHEAD) {
-        fetch(row, hn, gn, dn);
 #pragma unroll
         for (int p = 0; p < P; ++p) weight(p, w[AHEAD ? p : 0]);
+        fetch(row, hn, gn, dn);
     } else {
 #pragma unroll
         for (int p = 0; p < P; ++p)
@@ -311,6 +316,7 @@ __global__ __launch_bounds__(1024) void norm_grad_kernel(NormGradArgs a, int wav
                 ss = __builtin_fma((double)hf[j], (double)hf[j], ss);
                 gh = __builtin_fma((double)(gf[j] * w[AHEAD ? p : 0][j]), (double)hf[j], gh);
             }
+            if (!AHEAD) asm volatile("" : "+v"(ss), "+v"(gh));           // added up before the next piece's are read
         }
         ss = sum_lanes<L>(ss);
         gh = sum_lanes<L>(gh);
@@ -418,7 +424,7 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 // the rotation's are 7); without a residual 48 us, where they are 60%.  LDS for the rotation's transpose holds a CU to 16 waves.
 // ---------------------------------------------------------------------------
 template <int DT, int G, int P, int L, bool TILED>
-__global__ __launch_bounds__(1024) void norm_int8_kernel(NormArgs a, unsigned first) {
+__global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(P > 1 && DT != DT_F32 ? 5 : 4))) void norm_int8_kernel(NormArgs a, unsigned first) {
     using V = NormPiece<DT>;
     constexpr int N = V::N, LPG = G / kChunk, PIECES = kChunk / N;
     static_assert(L >= LPG && (L == 64 || P == 1), "groups of whole teams");
@@ -678,7 +684,7 @@ static hipError_t norm_int8_go(const NormArgs& a, int waves, hipStream_t st) {
 
 hipError_t norm_int8_launch(const NormArgs& a, int dt, int G, bool tiled, hipStream_t st) {
     const int nchunks = a.D / kChunk, waves = (nchunks + 63) / 64;
-    const bool one = waves == 1 || (waves <= 16 && (long long)a.M * waves < NORM8_FEW);      // one chunk a lane
+    const bool one = waves == 1 || (waves <= 16 && ((long long)a.M * waves < NORM8_FEW || (a.residual != nullptr && waves <= 4)));
     return by_type(dt, [&](auto d) {
         constexpr int DT = decltype(d)::value;
         const auto go = [&](auto g) {

@@ -101,46 +101,62 @@ __device__ __forceinline__ float logit_at(const void* p, int dt, size_t i) {
     return dt == DT_BF16 ? __uint_as_float(h << 16) : f16bits_to_f32(h);
 }
 
-// Experts e0 .. e0 + P - 1 of a row, -inf past the last.  Rows of a multiple of 4 are read 4 values at a time, of 16 bytes or
-// 8; others one by one.
+// Rows whose width is no multiple of 4 lie at any multiple of their element's size, which loads and stores of 8 and 16 bytes may.
+typedef float f4_any __attribute__((ext_vector_type(4), aligned(4)));
+typedef unsigned u2_any __attribute__((ext_vector_type(2), aligned(2)));
+
+// Experts e0 .. e0 + P - 1 of a row, -inf past the last: 4 values at a time, of 16 bytes or 8 (where rows allow it 8 of 16),
+// and the last one to three one by one.  The loads are sent out before a value is looked at, and the type is asked for once,
+// not for every value.
 template <int P>
 __device__ __forceinline__ void load_logits(const void* row, int dt, int e0, int E, float (&l)[P]) {
-    if (E % 4 != 0) {
-#pragma unroll
-        for (int p = 0; p < P; ++p) l[p] = e0 + p < E ? logit_at(row, dt, e0 + p) : -__builtin_inff();
-        return;
-    }
     if (dt == DT_F32) {
+        const float* x = reinterpret_cast<const float*>(row) + e0;
+        const float none = -__builtin_inff();
 #pragma unroll
         for (int p = 0; p < P; p += 4) {
-            float4 v = make_float4(-__builtin_inff(), -__builtin_inff(), -__builtin_inff(), -__builtin_inff());
-            if (e0 + p < E) v = *reinterpret_cast<const float4*>(reinterpret_cast<const float*>(row) + e0 + p);
-            l[p] = v.x; l[p + 1] = v.y; l[p + 2] = v.z; l[p + 3] = v.w;
+            f4_any v = {none, none, none, none};
+            if (e0 + p + 4 <= E) v = *reinterpret_cast<const f4_any*>(x + p);
+            else if (E % 4 != 0) {
+#pragma unroll
+                for (int i = 0; i < 3; ++i)
+                    if (e0 + p + i < E) v[i] = x[p + i];
+            }
+#pragma unroll
+            for (int i = 0; i < 4; ++i) l[p + i] = v[i];
         }
         return;
     }
+    const uint16_t* x = reinterpret_cast<const uint16_t*>(row) + e0;
     const uint32_t none = dt == DT_BF16 ? 0xff80ff80u : 0xfc00fc00u;   // -inf twice
-    uint2 v[P / 4];
+    uint32_t v[P / 2];
     if (P % 8 == 0 && E % 8 == 0) {
 #pragma unroll
         for (int p = 0; p < P; p += 8) {
             uint4 q = make_uint4(none, none, none, none);
-            if (e0 + p < E) q = *reinterpret_cast<const uint4*>(reinterpret_cast<const uint16_t*>(row) + e0 + p);
-            v[p / 4] = make_uint2(q.x, q.y);
-            v[(p / 4 + 1) % (P / 4)] = make_uint2(q.z, q.w);
+            if (e0 + p < E) q = *reinterpret_cast<const uint4*>(x + p);
+            v[p / 2] = q.x; v[p / 2 + 1] = q.y; v[(p / 2 + 2) % (P / 2)] = q.z; v[(p / 2 + 3) % (P / 2)] = q.w;
         }
     } else {
 #pragma unroll
         for (int p = 0; p < P; p += 4) {
-            v[p / 4] = make_uint2(none, none);
-            if (e0 + p < E) v[p / 4] = *reinterpret_cast<const uint2*>(reinterpret_cast<const uint16_t*>(row) + e0 + p);
+            u2_any q = {none, none};
+            if (e0 + p + 4 <= E) q = *reinterpret_cast<const u2_any*>(x + p);
+            else if (E % 4 != 0) {
+                const uint32_t high = none & 0xffff0000u;
+                if (e0 + p < E) q[0] = x[p] | high;
+                if (e0 + p + 1 < E) q[0] = (q[0] & 0xffffu) | (uint32_t)x[p + 1] << 16;
+                if (e0 + p + 2 < E) q[1] = x[p + 2] | high;
+            }
+            v[p / 2] = q[0]; v[p / 2 + 1] = q[1];
         }
     }
+    if (dt == DT_BF16) {
 #pragma unroll
-    for (int p = 0; p < P; p += 2) {
-        const uint32_t w = (p & 2) ? v[p / 4].y : v[p / 4].x;
-        l[p] = dt == DT_BF16 ? bf16lo_to_f32(w) : f16bits_to_f32(w);
-        l[p + 1] = dt == DT_BF16 ? bf16hi_to_f32(w) : f16bits_to_f32(w >> 16);
+        for (int p = 0; p < P; ++p) l[p] = p % 2 ? bf16hi_to_f32(v[p / 2]) : bf16lo_to_f32(v[p / 2]);
+    } else {
+#pragma unroll
+        for (int p = 0; p < P; ++p) l[p] = f16bits_to_f32(p % 2 ? v[p / 2] >> 16 : v[p / 2]);
     }
 }
 
@@ -454,34 +470,39 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
     }
 }
 
-// Values e0 .. e0 + P - 1 of a row of E in type dt
-template <int P>
-__device__ __forceinline__ void store_row(uint8_t* row, int dt, int e0, int E, const float (&v)[P]) {
+// A row of E in type dt from a token's lanes, every L-th four of each
+template <int L, int Q>
+__device__ __forceinline__ void store_row(uint8_t* row, int dt, int sub, int E, const float (&v)[Q][4]) {
+    const auto at = [&](int q) { return (q * L + sub) * 4; };
     if (dt == DT_F32) {
-        float* out = reinterpret_cast<float*>(row) + e0;
+        float* out = reinterpret_cast<float*>(row);
 #pragma unroll
-        for (int p = 0; p < P; p += 4) {
-            if (E % 4 == 0) {
-                if (e0 + p < E) *reinterpret_cast<float4*>(out + p) = make_float4(v[p], v[p + 1], v[p + 2], v[p + 3]);
-            } else {
+        for (int q = 0; q < Q; ++q) {
+            if (at(q) + 4 <= E) *reinterpret_cast<f4_any*>(out + at(q)) = f4_any{v[q][0], v[q][1], v[q][2], v[q][3]};
+            else if (E % 4 != 0) {
 #pragma unroll
-                for (int i = p; i < p + 4; ++i)
-                    if (e0 + i < E) out[i] = v[i];
+                for (int i = 0; i < 3; ++i)
+                    if (at(q) + i < E) out[at(q) + i] = v[q][i];
             }
         }
         return;
     }
-    uint16_t* out = reinterpret_cast<uint16_t*>(row) + e0;
+    u2_any w[Q];
+    if (dt == DT_BF16) {
 #pragma unroll
-    for (int p = 0; p < P; p += 4) {
-        const uint32_t lo = dt == DT_BF16 ? pack_bf16x2(v[p], v[p + 1]) : pack_f16x2(v[p], v[p + 1]);
-        const uint32_t hi = dt == DT_BF16 ? pack_bf16x2(v[p + 2], v[p + 3]) : pack_f16x2(v[p + 2], v[p + 3]);
-        if (E % 4 == 0) {
-            if (e0 + p < E) *reinterpret_cast<uint2*>(out + p) = make_uint2(lo, hi);
-        } else {
+        for (int q = 0; q < Q; ++q) w[q] = u2_any{pack_bf16x2(v[q][0], v[q][1]), pack_bf16x2(v[q][2], v[q][3])};
+    } else {
 #pragma unroll
-            for (int i = 0; i < 4; ++i)
-                if (e0 + p + i < E) out[p + i] = (uint16_t)((i & 2 ? hi : lo) >> (i & 1 ? 16 : 0));
+        for (int q = 0; q < Q; ++q) w[q] = u2_any{pack_f16x2(v[q][0], v[q][1]), pack_f16x2(v[q][2], v[q][3])};
+    }
+    uint16_t* out = reinterpret_cast<uint16_t*>(row);
+#pragma unroll
+    for (int q = 0; q < Q; ++q) {
+        if (at(q) + 4 <= E) *reinterpret_cast<u2_any*>(out + at(q)) = w[q];
+        else if (E % 4 != 0) {
+#pragma unroll
+            for (int i = 0; i < 3; ++i)
+                if (at(q) + i < E) out[at(q) + i] = (uint16_t)(w[q][i / 2] >> (i % 2 * 16));
         }
     }
 }
@@ -564,16 +585,17 @@ __global__ __launch_bounds__(RT_THREADS) void choose_grad_kernel(RouterGradArgs 
     }
     wave_sync();
     const float share = total == 0.0f ? 0.0f : mean / total;           // no expert: all are 0
+    float out[P / 4][4];
 #pragma unroll
     for (int q = 0; q < P / 4; ++q) {
         const float4 f = fours[q * L + sub];
-        float out[4] = {f.x, f.y, f.z, f.w};
-        if (all) {
-#pragma unroll
-            for (int i = 0; i < 4; ++i) out[i] -= l[q][i] * share;
-        }
-        store_row(reinterpret_cast<uint8_t*>(a.d_logits) + (size_t)t * a.E * ES, a.dt, (q * L + sub) * 4, a.E, out);
+        out[q][0] = f.x; out[q][1] = f.y; out[q][2] = f.z; out[q][3] = f.w;
     }
+    if (all) {
+#pragma unroll
+        for (int q = 0; q < P; ++q) out[q / 4][q % 4] -= l[q / 4][q % 4] * share;
+    }
+    store_row<L>(reinterpret_cast<uint8_t*>(a.d_logits) + (size_t)t * a.E * ES, a.dt, sub, a.E, out);
 }
 
 // f(lanes of a token, experts of a lane): 16 experts a lane, the fewest instructions a token, where the tokens fill the
