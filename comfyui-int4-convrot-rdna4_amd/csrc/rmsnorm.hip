@@ -101,7 +101,8 @@ __device__ __forceinline__ void store_weight(void* w, int dt, int e, float v) {
     else reinterpret_cast<uint16_t*>(w)[e] = (uint16_t)(dt == DT_BF16 ? pack_bf16x2(v, 0.0f) : pack_f16x2(v, 0.0f));
 }
 
-// N values of the weight from element e on (ones without a weight); TINY: of a weight of D < N
+// N values of the weight from element e on (ones without a weight); TINY: of a weight of D < N.  The type is asked for once: a
+// branch for every pair of values costs the 8-bit form of 8192 x 5120 10 us of 70.
 template <int N, bool TINY = false>
 __device__ __forceinline__ void load_weight(const void* w, int dt, int e, int D, float (&v)[N]) {
     static_assert(N % 4 == 0, "whole pieces");
@@ -171,8 +172,8 @@ __device__ __forceinline__ double sum_waves(double v, double* slot, int waves) {
     return s;
 }
 
-// Bound by memory: 16384 x 5120 bf16 with a residual 115 us, 5.8 TB/s of the four tensors, without 66 us, 5.1 TB/s.  The weight
-// is read after the sums: before them its registers cost waves (8192 x 4096 56 us, so 50).  Stores that the caches do not keep
+// Bound by memory: 16384 x 5120 bf16 with a residual 115 us, 5.8 TB/s of the four tensors, without 61 us, 5.5 TB/s.  The weight
+// is read after the sums: before them its registers cost waves (8192 x 4096 51 us, so 48).  Stores that the caches do not keep
 // make this kernel shorter (512 x 4096 5.7 and 5.3, 16384 x 5120 115 and 109) and whoever reads y and h next longer by more:
 // with a copy of both 2048 x 4096 24.9 and 28.4, 4096 x 5120 58 and 64, 8192 x 4096 90 and 97.
 template <int DT, int P, int L, bool RES, bool TINY>
@@ -240,8 +241,8 @@ __global__ __launch_bounds__(1024) void norm_kernel(NormArgs a, int waves, unsig
 //
 // What a row takes of a lane's registers is kept as it lies in memory (`again` makes the compiler unpack it a second time
 // rather than hold the floats across the sums); rows of four and more pieces a lane are not fetched ahead, read d_h and
-// the weight where they are used, and have their part of d_weight in LDS, a slot a piece (2048 x 20000: 248 us with all of
-// it in registers that do not hold it).
+// the weight where they are used, and have their part of d_weight in LDS, a slot a piece (2048 x 20000 107 us: 248 with all of
+// it in registers that do not hold it, 167 where a row's sums wait for all of its weights).
 __device__ __forceinline__ void again(v4u_mx& w) { asm volatile("" : "+v"(w)); }
 
 template <int DT, int P, int L, bool RES, bool TINY>
@@ -420,8 +421,10 @@ __global__ __launch_bounds__(1024) void norm_weight_grad_kernel(const float* __r
 // A lane holds 16 consecutive values.  Everything up to the code is fp64 (full rate here), so a code is the formula's
 // nearest one and not a matter of the order of sums; rstd commutes with the rotation, so it is not waited for.  A row
 // with a value that is not finite (or zeros over eps = 0) gets scale NaN and codes 0.
-// 8192 x 5120 bf16 with a residual 68 us, 4.3 TB/s: memory, and VALU instructions half of the time (28 an element, of which
-// the rotation's are 7); without a residual 48 us, where they are 60%.  LDS for the rotation's transpose holds a CU to 16 waves.
+// 8192 x 5120 bf16 with a residual 59.5 us, 4.9 TB/s: memory, and VALU instructions 65% of the time (22 an element, of which the
+// rotation's are 7); without a residual 39 us, where they are 80%.  LDS for the rotation's transpose holds a CU to 18 waves;
+// registers are kept to what five waves a SIMD have (of two chunks a lane: 4096 x 10240 76 us with four, 66 so), but for 32-bit
+// values, which would spill.
 // ---------------------------------------------------------------------------
 template <int DT, int G, int P, int L, bool TILED>
 __global__ __launch_bounds__(1024) __attribute__((amdgpu_waves_per_eu(P > 1 && DT != DT_F32 ? 5 : 4))) void norm_int8_kernel(NormArgs a, unsigned first) {

@@ -107,7 +107,7 @@ typedef unsigned u2_any __attribute__((ext_vector_type(2), aligned(2)));
 
 // Experts e0 .. e0 + P - 1 of a row, -inf past the last: 4 values at a time, of 16 bytes or 8 (where rows allow it 8 of 16),
 // and the last one to three one by one.  The loads are sent out before a value is looked at, and the type is asked for once,
-// not for every value.
+// not for every value (16384 x 250 in 16 bits, sigmoid and a bias, 12.2 us; 19.0 one by one).
 template <int P>
 __device__ __forceinline__ void load_logits(const void* row, int dt, int e0, int E, float (&l)[P]) {
     if (dt == DT_F32) {
@@ -335,8 +335,8 @@ __device__ __forceinline__ void keep_groups(double (&c)[P], const RouterArgs& a,
 // after the other.
 // Few tokens are bound by the chain of one (us, graph replays on MI355X): 1 of 32 experts 2.4, 16 of 256 in groups 4.2 (18
 // with a greatest key looked for k times over 16 experts a lane, and groups read from LDS); many by instructions: 16384 tokens
-// of 256 experts in 8 groups with sigmoid scores and a bias 12.4 (43 so), 1345 VALU instructions a wave of four tokens,
-// 60% of the cycles; without a bias or groups 6.8.  Their logits are 8 MB, 1.6 us.
+// of 256 experts in 8 groups with sigmoid scores and a bias 12.1 (43 so), 1330 VALU instructions a wave of four tokens,
+// three quarters of the cycles; without a bias or groups 6.6.  Their logits are 8 MB, 1.6 us.
 template <int L, int P, int K, bool GROUPS>
 __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsigned first) {
     __shared__ int chosen_lds[K == 0 ? RT_THREADS * P : 1];           // k <= E <= L P of each token
@@ -512,8 +512,8 @@ __device__ __forceinline__ void store_row(uint8_t* row, int dt, int sub, int E, 
 //   sigmoid        renormalized p_j (1 - s_j) (g_j - sum p g), else s_j (1 - s_j) g_j
 // and 0 for experts that were not chosen (but for softmax as it is).  Scores are computed again from the logits.
 // A lane's experts are every L-th four, so that lanes beside each other write beside each other, in LDS and in memory: 65536
-// tokens of 256 experts 12.1 us (20.0 with sixteen experts in a row to a lane), where the stores and the lines that the chosen
-// logits lie in are 67 MB; 16384 tokens 5.3 (8.0), of softmax as it is 8.7.
+// tokens of 256 experts 11.9 us (20.0 with sixteen experts in a row to a lane), where the stores and the lines that the chosen
+// logits lie in are 67 MB; 16384 tokens 5.0 (8.0), of softmax as it is 8.1.
 template <int L, int P, int K>
 __global__ __launch_bounds__(RT_THREADS) void choose_grad_kernel(RouterGradArgs a, unsigned first) {
     __shared__ float4 d_lds[RT_THREADS * P / 4];
