@@ -404,7 +404,8 @@ def plain_many(logits, k, bias, scoring, num_groups, top_groups, group_score):
 @pytest.mark.parametrize("dtype", [torch.bfloat16, torch.float32])
 @pytest.mark.parametrize("E,k,groups,top", [(8, 2, 1, 1), (30, 4, 3, 2), (32, 8, 2, 1), (33, 3, 1, 1), (64, 6, 8, 3), (100, 6, 1, 1), (100, 8, 5, 2),
                                             (128, 4, 1, 1), (128, 8, 4, 2), (250, 10, 1, 1), (256, 8, 8, 4), (256, 12, 16, 5), (512, 8, 8, 2),
-                                            (1000, 8, 10, 3)])
+                                            (1000, 8, 10, 3), (14, 12, 1, 1), (32, 9, 1, 1), (64, 16, 4, 3), (128, 16, 1, 1), (128, 20, 1, 1),
+                                            (130, 33, 10, 4), (254, 10, 2, 1), (512, 10, 1, 1), (1024, 17, 1, 1)])
 def test_many_tokens(backend, gpu, E, k, groups, top, dtype):
     """Calls of 2^19 logits and more, which give a lane sixteen experts, with some rows masked, and their gradients."""
     T = (1 << 19) // E + 77
