@@ -25,6 +25,9 @@ namespace convrot {
 constexpr int RT_MAX_E = 1024;                         // indexes in ten bits
 constexpr double RT_NONE = -0x1.fffffffffffffp1023;    // the choice and the key of an expert that is not available
 constexpr double RT_MOST = 0x1p1022;                   // the choice of one that is +inf or NaN
+// Sums that are equal but for their last bits are often round numbers, the two scores of x and -x for one, which lie where
+// the cut parts values: a step of 2^-44 puts them between a quarter and a half into what the 43 bits keep together.
+constexpr double RT_ASIDE = 1.0 + 0x1p-44;
 constexpr int RT_THREADS = 256;
 // Logits of a call that takes 4 experts a lane (us, 4 and 16 a lane): 1 x 256 in groups 4.4 and 6.2, 2048 x 256 6.5 and 6.6,
 // 4096 x 256 8.9 and 6.7; 4096 x 128 5.1 and 5.6, 8192 x 128 7.1 and 5.8; 16384 x 32 3.4 and 4.6.
@@ -384,7 +387,7 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
 #pragma unroll
         for (int p = 0; p < P; ++p) {
             const float add = l[p] == -__builtin_inff() ? l[p] : a.bias != nullptr ? b[p] : 0.0f;
-            const double v = key_min(c[p] + (double)add, RT_MOST);              // of a NaN RT_MOST
+            const double v = key_min((c[p] + (double)add) * RT_ASIDE, RT_MOST); // of a NaN RT_MOST
             c[p] = add == -__builtin_inff() ? RT_NONE : v;
         }
     } else {

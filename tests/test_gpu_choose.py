@@ -181,6 +181,19 @@ def test_ties_go_to_the_lowest_index(backend, gpu):
         compare(backend, l, k, num_groups=8, top_groups=3, group_score="sum2")
 
 
+@pytest.mark.parametrize("dtype", [torch.float32, torch.bfloat16])
+@pytest.mark.parametrize("T", [60, 70000])
+def test_ties_of_sums(backend, gpu, T, dtype):
+    """The scores of x and -x make 1, whatever x is: of such groups the lowest."""
+    x = (3.0 * torch.randn(T, 4, generator=torch.Generator().manual_seed(5))).to(dtype).cuda()
+    pairs = torch.stack((x, -x), -1).reshape(T, 8)
+    ids, _ = backend.choose_experts(pairs, 4, scoring="sigmoid", num_groups=4, top_groups=2, group_score="sum2")
+    assert bool((ids < 4).all())
+    ids, _ = backend.choose_experts(pairs.flip(1), 2, torch.zeros(8, device="cuda"), scoring="sigmoid", num_groups=4, top_groups=1,
+                                    group_score="sum2")
+    assert bool((ids < 2).all())
+
+
 def test_values_that_are_not_finite(backend, gpu):
     E, k = 40, 4
     l = logits_of(6, E, torch.float32, 5)
