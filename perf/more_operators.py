@@ -14,7 +14,6 @@ over a taste of the router's own.
 """
 from __future__ import annotations
 
-import functools
 import importlib
 import math
 
@@ -263,14 +262,8 @@ def _plain_norm8(s):
     return out
 
 
-@functools.lru_cache(maxsize=None)
-def _module(name):
-    """Looked up once, as a program's imports are: the lookup is 3 us, a third of a small call."""
-    return importlib.import_module(_PKG + name)
-
-
 def _own_pass(s):
-    q = _module("._int4")
+    q = importlib.import_module(_PKG + "._int4")
     c = s["case"]
     if c["kind"] == "choose":
         ids, weights = q.choose_experts(
@@ -281,7 +274,7 @@ def _own_pass(s):
             out["d_logits"], = torch.autograd.grad(weights, s["logits"], s["d_weights"])
         return out
     if c["kind"] == "norm8":
-        int8 = _module("._int4.int8_eager")
+        int8 = importlib.import_module(_PKG + "._int4.int8_eager")
         rows = q.rms_norm_int8(s["x"], s["weight"], s["residual"], _EPS, convrot_groupsize=c["G"])
         rows, h = rows if c["residual"] else (rows, None)
         out = {"values": int8.dequantize_convrot_w8a8_weight(rows.codes, rows.scales, c["G"], torch.bfloat16),
