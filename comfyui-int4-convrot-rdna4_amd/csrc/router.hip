@@ -8,7 +8,8 @@
 // An expert whose logit or bias is -inf is not available; a slot that finds none has id -1 and weight 0.
 //
 // The order is decided in 64 bits: c is cut to 43 bits, far below what 32-bit scores could tell apart, and equal
-// ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them.  A key
+// ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them; scores
+// then rank groups by their sums at most.  A key
 // holds both: the low ten bits of a double give way to the index (1023 - e, or e where c is negative, so that of
 // equal values the lowest index is the greatest key).  Keys are finite and differ, and the greater and the smaller of
 // two are one instruction each, where a pair of value and index would take five.
@@ -73,6 +74,9 @@ __device__ __forceinline__ int key_number(double key) {
     const int low = (int)(((uint32_t)u ^ (uint32_t)((int)(u >> 32) >> 31)) & 1023u);
     return is_none(key) ? -1 : 1023 - low;
 }
+
+// The choice of a logit where the order is the logits' own: -0 counts as 0, a NaN as +inf, -inf is not available
+__device__ __forceinline__ double choice_of(float l) { return key_max(key_min((double)l + 0.0, RT_MOST), RT_NONE); }
 
 // exp(x) to 2^-47 of its value for |x| up to 200, 2^-45 up to 700, x at most 700; below -700 as at -700: x = n ln 2 + r, and of
 // exp(r) on |r| <= ln(2) / 2 the polynomial of degree 10 that is 1 at 0 and meets exp at the ten Chebyshev points of the
@@ -392,9 +396,15 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
         }
     } else {
 #pragma unroll
-        for (int p = 0; p < P; ++p) c[p] = key_max(key_min((double)l[p] + 0.0, RT_MOST), RT_NONE);      // -0 counts as 0
+        for (int p = 0; p < P; ++p) c[p] = choice_of(l[p]);
     }
-    if constexpr (GROUPS) keep_groups<L>(c, a, sub, table_lds + tid / L * (L * P));
+    if constexpr (GROUPS) {
+        keep_groups<L>(c, a, sub, table_lds + tid / L * (L * P));
+        if (by_score && a.bias == nullptr) {
+#pragma unroll
+            for (int p = 0; p < P; ++p) c[p] = is_none(c[p]) ? RT_NONE : choice_of(l[p]);
+        }
+    }
 #pragma unroll
     for (int p = 0; p < P; ++p) c[p] = key_of(c[p], (e0 + p) & 1023);
 
