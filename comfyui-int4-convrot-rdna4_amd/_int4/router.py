@@ -77,8 +77,8 @@ def choose_experts(logits: torch.Tensor, top_k: int, balance_bias: torch.Tensor 
     their greatest choice (``group_score`` "max") or the sum of their two greatest
     ("sum2"), and only experts of the ``top_groups`` greatest groups are chosen (None:
     of all).  The k greatest are returned greatest first; ties, of choices that
-    agree to 43 bits, go to the lowest index, and without a bias the order is the
-    logits' own.  The weights are the chosen scores, divided by their sum where
+    agree to 43 bits (or to 2^-1064: a bias of 0 and a score below exp(-737)), go to
+    the lowest index, and without a bias the order is the logits' own.  The weights are the chosen scores, divided by their sum where
     ``renormalize``, times ``scale``.
 
     An expert whose logit (or bias) is -inf is not available.  A slot for which no

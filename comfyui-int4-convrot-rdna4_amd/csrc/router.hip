@@ -7,8 +7,8 @@
 //   ids = the k experts of the greatest c, greatest first; w = s[ids] (renormalized: over their sum) times `scale`
 // An expert whose logit or bias is -inf is not available; a slot that finds none has id -1 and weight 0.
 //
-// The order is decided in 64 bits: c is cut to 43 bits, far below what 32-bit scores could tell apart, and equal
-// ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them; scores
+// The order is decided in 64 bits: c is cut to 43 bits (past the range to whole 2^-1064), far below what 32-bit scores could
+// tell apart, and equal ones go to the lowest index.  Without a bias the order is the logits' own, since scores rise with them; scores
 // then rank groups by their sums at most.  A key
 // holds both: the low ten bits of a double give way to the index (1023 - e, or e where c is negative, so that of
 // equal values the lowest index is the greatest key).  Keys are finite and differ, and the greater and the smaller of
@@ -78,11 +78,12 @@ __device__ __forceinline__ int key_number(double key) {
 // The choice of a logit where the order is the logits' own: -0 counts as 0, a NaN as +inf, -inf is not available
 __device__ __forceinline__ double choice_of(float l) { return key_max(key_min((double)l + 0.0, RT_MOST), RT_NONE); }
 
-// exp(x) to 2^-47 of its value for |x| up to 200, 2^-45 up to 700, x at most 700; below -700 as at -700: x = n ln 2 + r, and of
-// exp(r) on |r| <= ln(2) / 2 the polynomial of degree 10 that is 1 at 0 and meets exp at the ten Chebyshev points of the
-// interval (off by 2^-50.5 at most).  Sixteen instructions where the library's takes forty; the choice keeps 43 bits.
+// exp(x) to 2^-46 of its value for |x| up to 200, 2^-45 up to 708, x at most 708; below -708 rounded to whole 2^-1074 besides,
+// 0 from -746 on: x = n ln 2 + r, and of exp(r) on |r| <= ln(2) / 2 the polynomial of degree 10 that is 1 at 0 and meets exp at
+// the ten Chebyshev points of the interval (off by 2^-50.5 at most; ln 2 in one double by 2^-55.3 a unit of n).  Sixteen instructions where
+// the library's takes forty; the choice keeps 43 bits.
 __device__ __forceinline__ double choice_exp(double x) {
-    x = x < -700.0 ? -700.0 : x;
+    x = x < -746.0 ? -746.0 : x;
     const double t = __builtin_fma(x, 1.4426950408889634, 0x1.8p52);
     const double r = __builtin_fma(t - 0x1.8p52, -0.6931471805599453, x);
     double p = 0x1.28917c89a43a7p-22;
@@ -369,10 +370,16 @@ __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsign
     bool spoilt = false;                                              // softmax with a NaN: no score is a number
     if (by_score) {
         if (a.sigmoid) {
+            bool far = false;
 #pragma unroll
             for (int p = 0; p < P; ++p) {
                 const float x = l[p] < -700.0f ? 700.0f : -l[p];
                 c[p] = choice_rcp(1.0 + choice_exp((double)x));
+                far |= l[p] < -700.0f && l[p] != -__builtin_inff();
+            }
+            if (far) {                                                // 1 + exp(-l) leaves the range, exp(l) is the score
+#pragma unroll
+                for (int p = 0; p < P; ++p) c[p] = l[p] < -700.0f ? choice_exp((double)l[p]) : c[p];
             }
         } else {
             double sum = 0.0;

@@ -479,7 +479,7 @@ int cr_mxfp4_expert_linear(const void* x, int dtype, const int* order, int top_k
  * Of token t's logits l [E] (dtype) and a bias b [E] (f32; NULL: 0): scores s = softmax(l), or 1 / (1 + exp(-l)) with
  * `sigmoid`; choices c = s + b.  The `groups` groups of E / groups experts in order are ranked by their greatest c, or
  * with group_sum2 by the sum of their two greatest; experts outside the top_groups greatest are left out.  ids[t, 0 .. k - 1]
- * are the k greatest of those left, greatest first, equal ones (in 43 bits) by index; weights[t, j] = s[ids[t, j]], over their
+ * are the k greatest of those left, greatest first, equal ones (in 43 bits, or to 2^-1064) by index; weights[t, j] = s[ids[t, j]], over their
  * sum with `renormalize`, times `scale`.  Without a bias the order is the logits'.  An expert whose logit or bias is -inf is
  * not available; a slot that finds none has id -1 and weight 0.  A NaN ranks with +inf, and makes the weights NaN that
  * depend on it.

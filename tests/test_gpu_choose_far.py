@@ -55,3 +55,32 @@ def test_unavailable_experts_stay_so_in_groups_by_sums(backend, gpu):
     ids, _ = backend.choose_experts(l, 12, group_score="sum2", **how)
     assert torch.equal(ids, backend.choose_experts(l, 12, group_score="max", **how)[0])
     assert bool((ids[5:10, 0] == 8).all()) and bool((ids[15] == -1).all()) and bool((ids[:, 11] == -1).any())
+
+
+@pytest.mark.parametrize("T", [1, 60, (1 << 13) + 77])
+@pytest.mark.parametrize("E,groups,top", [(64, 1, 1), (64, 8, 3), (20, 5, 2)])
+@pytest.mark.parametrize("scoring", ["softmax", "sigmoid"])
+def test_scores_down_to_the_end_of_the_range(backend, gpu, monkeypatch, scoring, E, groups, top, T):
+    """With a bias of zeros the order is the scores', as far as 64 bits hold them: logits of whole numbers down to -730,
+    whose scores (2^-1053) lie a factor e apart, well above the 2^-1064 that the keys keep; at -800 and below a score is 0,
+    and still available."""
+    g = torch.Generator().manual_seed(E + T)
+    l = -torch.rand(T, E, generator=g).argsort(1).float() - (731 - E)            # whole numbers, each once
+    top_one = -800.0 if scoring == "sigmoid" else 0.0                             # softmax: what the others are far below
+    l[:, 0] = top_one
+    if T > 1:
+        l[1::4, 5:9] = -math.inf
+        l[2::4, 9:12] = -1000.0
+    l = l.cuda()
+    # torch's own is 0 below -709.8, where its exp(-l) leaves the range; exp(l) is within a factor 1 + exp(-667) of it
+    monkeypatch.setattr(torch, "sigmoid", torch.exp)
+    zeros, k = torch.zeros(E, device="cuda"), E // groups * top
+    for group_score in ("max", "sum2"):
+        ids, _ = backend.choose_experts(l, k, zeros, scoring=scoring, num_groups=groups, top_groups=top, group_score=group_score)
+        want = plain_many(l, k, zeros, scoring, groups, top, group_score)
+        assert torch.equal(ids, want)
+    if groups == 1:
+        there = ids >= 0
+        picked = torch.where(there, l.gather(1, ids.clamp(min=0).long()), -math.inf)
+        low = picked < -745.2                                                     # scores of 0: by index
+        assert bool(((picked[:, 1:] <= picked[:, :-1]) | low[:, :-1]).all())
