@@ -773,11 +773,11 @@ API size_t cr_rms_norm_grad_workspace(int M, int D) {
 API int cr_rms_norm_grad(const void* d_y, const void* d_h, const void* h, int dtype, const void* weight, int weight_dtype, void* d_x,
                          void* d_weight, int M, int D, double eps, void* workspace, size_t workspace_bytes, void* stream) {
     if (!norm_ok(dtype, weight_dtype, M, D, eps) || (d_weight != nullptr && weight == nullptr)) return -1;
-    if (M == 0) return 0;
+    if (M == 0 && d_weight == nullptr) return 0;
     convrot::NormGradArgs a{};
     a.d_y = d_y; a.d_h = d_h; a.h = h; a.weight = weight; a.d_x = d_x; a.d_weight = d_weight;
     a.eps = eps; a.M = M; a.D = D; a.weight_dt = weight_dtype;
-    if (d_weight != nullptr) {
+    if (d_weight != nullptr && M > 0) {
         if (workspace == nullptr || workspace_bytes < cr_rms_norm_grad_workspace(M, D)) return -1;
         a.partial = reinterpret_cast<float*>(reinterpret_cast<uint8_t*>(workspace) + kSplitCounterBytes);
     }

@@ -654,7 +654,13 @@ static hipError_t norm_grad_go(const NormGradArgs& a, const NormGradShape& s, hi
     return hipGetLastError();
 }
 
+static hipError_t norm_weight_grad_launch(const NormGradArgs& a, int parts, hipStream_t st) {
+    hipLaunchKernelGGL(norm_weight_grad_kernel, dim3((a.D + 15) / 16), dim3(1024), 0, st, a.partial, a.d_weight, a.weight_dt, a.D, parts);
+    return hipGetLastError();
+}
+
 hipError_t norm_grad_launch(const NormGradArgs& a, int dt, hipStream_t st) {
+    if (a.M == 0) return a.d_weight == nullptr ? hipSuccess : norm_weight_grad_launch(a, 0, st);      // zeros: a sum of no rows
     const NormGradShape s = norm_grad_shape(a.M, a.D, dt == DT_F32 ? 4 : 8);
     const hipError_t e = by_type(dt, [&](auto d) {
         constexpr int DT = decltype(d)::value;
@@ -664,9 +670,7 @@ hipError_t norm_grad_launch(const NormGradArgs& a, int dt, hipStream_t st) {
     });
     // several teams of one workgroup have written d_weight themselves
     if (e != hipSuccess || a.d_weight == nullptr || (s.groups == 1 && s.teams > 1)) return e;
-    hipLaunchKernelGGL(norm_weight_grad_kernel, dim3((a.D + 15) / 16), dim3(1024), 0, st, a.partial, a.d_weight, a.weight_dt, a.D,
-                       s.groups);
-    return hipGetLastError();
+    return norm_weight_grad_launch(a, s.groups, st);
 }
 
 template <int DT, int G, int P, int L, bool TILED>

@@ -497,7 +497,8 @@ int cr_choose_experts_grad(const void* logits, int dtype, const int* ids, const 
  * h = dtype(x + residual) (residual NULL: h is x, and not written); y = dtype(h w / sqrt(mean(h^2) + eps)), w [D] of
  * weight_dtype (NULL: 1).  D <= cr_max_norm_width().
  * cr_rms_norm_grad: d_x of x, and of the residual, from d_y and the sum's own gradient d_h (NULL: 0); d_weight [D] in
- *   weight_dtype; either may be NULL.  workspace: >= cr_rms_norm_grad_workspace(M, D) bytes where d_weight is asked for.
+ *   weight_dtype, zeros for M = 0; either may be NULL.  workspace: >= cr_rms_norm_grad_workspace(M, D) bytes where d_weight
+ *   is asked for (0 for M = 0).
  * cr_rms_norm_int8: z = H_G(h w) / sqrt(mean(h^2) + eps), scales[m] = f32(max(max|z|, 1e-10) / 127), codes the nearest of
  *   z / scale, ties to even; [M, D] int8, or with `tiled` in the I8T layout (D % 64 == 0; padding rows zero).  A row that is
  *   not finite gets scale NaN and codes 0.
