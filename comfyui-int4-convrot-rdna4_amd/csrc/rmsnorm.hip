@@ -5,7 +5,8 @@
 // The norm is of the sum as it is kept, so norm and residual stream agree, and the gradient needs h alone.
 //
 // Squares are added in fp64 (full rate here): they cannot overflow, and no order of the sum shows in the result.  y is
-// made in fp32 as ((h 2^n) a) w with rstd = a 2^n: no step leaves the range where the result does not.
+// made in fp32 as ((h 2^n) a) w with rstd = a 2^n: no step overflows where the result does not, and a product with rstd
+// that falls below 2^-126 is off by 2^-149 at most before the weight's.
 
 #include "b6t_layout.h"
 #include "lanes.h"
@@ -18,9 +19,15 @@ namespace convrot {
 // Pieces a lane of a row's norm: 16384 x 5120 with 1, 2 and 4 117, 116 and 119, without residual 92, 62 and 60; 4096 x 13824
 // 81, 81 and 82.
 constexpr int NORM_PIECES = 2;
-// Rows of a team that a single workgroup of several teams takes: 8 x 1024 5.3, in two launches 6.1.
+// Rows of a team that a single workgroup of several teams takes (us so, and in two launches): two rows 8 x 1024 5.2 and 5.8,
+// 16 x 256 3.8 and 4.9, 64 x 64 4.0 and 5.1; three 24 x 256 4.6 and 4.9, 96 x 64 4.7 and 5.1, 12 x 1024 6.6 and 5.8; four 128 x 64
+// 5.4 and 5.1, 16 x 1024 7.7 and 5.9.
 constexpr int NORM_GRAD_ALONE = 3;
-// Waves of a gradient that take a piece a lane each, others two: 512 x 4096 15.6 and 13.4, 4096 x 5120 57 and 44.
+// Waves of a gradient that take a piece a lane each, others two (us, one piece and two).  Below: 64 x 4096 6.4 and 8.1, 256 x 1024
+// 6.1 and 6.8, 256 x 2048 7.2 and 7.9, 128 x 4096 7.7 and 8.9.  Above: 2048 x 1024 10.9 and 10.0, 2048 x 2048 17.4 and 16.0,
+// 2048 x 4096 27.9 and 24.7, 8192 x 2048 34.5 and 32.6.  Within 5% of the other at the border: 256 x 4096 10.0 and 10.3, 512 x 4096 12.9
+// and 13.5, 1024 x 4096 18.5 and 18.0; rows of 5120, in workgroups of five waves and not ten, are 2% to 4% slower so
+// above it.
 constexpr int NORM_GRAD_FEW = 2048;
 // Waves of the 8-bit form that take a chunk a lane each, others two: 64 x 4096 3.8 and 4.6, 512 x 4096 6.2 and 7.2, 1024 x 8192
 // without a residual 10.7 and 10.6, 8192 x 5120 45 and 39, 4096 x 16384 89 and 63.  With a residual rows of up to four waves
@@ -605,9 +612,10 @@ hipError_t norm_launch(const NormArgs& a, int dt, hipStream_t st) {
 }
 
 // Teams and workgroups of a gradient, from its shape: workgroups of eight waves or one team.  Each leaves a row of partial
-// sums of d_weight, to be read again: as many workgroups as the chip holds at once (16 waves a CU), but no more than makes
-// that an eighth of the rows' traffic (8192 x 4096: 512 workgroups 55.6 us, 1024 61.6; 2048 x 13824: 256 58.6, 512
-// 69.2; 110000 x 128: 512 30.2, 1024 24.9).  One workgroup where it has several teams and each few rows, which then
+// sums of d_weight, to be read again: as many workgroups as the chip holds at once (16 waves a CU), but past 256, one a
+// CU, no more than makes that an eighth of the rows' traffic (8192 x 4096: 512 workgroups 55.6 us, 1024 61.6; 2048 x 13824: 256
+// 58.6, 512 69.2; 110000 x 128: 512 30.2, 1024 24.9).  256 workgroups of fewer than 2048 rows M make it 256 / M of them: a
+// quarter at 1024 rows, half at 512.  One workgroup where it has several teams and each few rows, which then
 // writes d_weight itself.
 struct NormGradShape { NormShape team; int teams, groups; };
 static NormGradShape norm_grad_shape(int M, int D, int piece) {

@@ -344,10 +344,10 @@ __device__ __forceinline__ void keep_groups(double (&c)[P], const RouterArgs& a,
 
 // L lanes take a token, P experts each, in order.  K: the longest list that is sorted, at least k; 0: any k, one expert
 // after the other (4096 tokens' 10 of 512 7.8 us so and 6.6 with lists of 16, 16 of 1024 15.5 and 10.5).
-// Few tokens are bound by the chain of one (us, graph replays on MI355X): 1 of 32 experts 2.4, 16 of 256 in groups 4.2 (18
+// Few tokens are bound by the chain of one (us, graph replays on MI355X): 1 of 32 experts 2.4, 16 of 256 in groups 4.3 (18
 // with a greatest key looked for k times over 16 experts a lane, and groups read from LDS); many by instructions: 16384 tokens
-// of 256 experts in 8 groups with sigmoid scores and a bias 12.1 (43 so), 1330 VALU instructions a wave of four tokens,
-// three quarters of the cycles; without a bias or groups 6.6.  Their logits are 8 MB, 1.6 us.
+// of 256 experts in 8 groups with sigmoid scores and a bias 12.8 (43 so), 1360 VALU instructions a wave of four tokens,
+// three quarters of the cycles; without a bias or groups 6.3.  Their logits are 8 MB, 1.6 us.
 template <int L, int P, int K, bool GROUPS>
 __global__ __launch_bounds__(RT_THREADS) void choose_kernel(RouterArgs a, unsigned first) {
     __shared__ int chosen_lds[K == 0 ? RT_THREADS * P : 1];           // k <= E <= L P of each token
